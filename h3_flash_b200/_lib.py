@@ -21,7 +21,7 @@ H3B_OK = 0
 H3B_ERR_VALUE = 1
 H3B_ERR_CUDA = 2
 H3B_ERR_UNSUPPORTED = 3
-ABI_VERSION = 8
+ABI_VERSION = 9
 IPC_HANDLE_BYTES = 64
 
 _p = ctypes.c_void_p
@@ -36,6 +36,7 @@ SIGNATURES: dict[str, list[Any]] = {
                                            _i64, _i64, _i64, _i64, _i64, _f32, _p],
     "h3b_modulate": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p],
     "h3b_gated_residual": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p],
+    "h3b_sandwich_residual_rmsnorm_modulate": [_p] * 10 + [_i64] * 10 + [_f32] * 3 + [_i64, _p],
     "h3b_swiglu": [_p, _p, _i64, _i64, _i64, _i64, _p],
     "h3b_gelu_tanh": [_p, _p, _i64, _i64, _i64, _i64, _p],
     "h3b_qknorm_rope": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f32, _p],
@@ -47,6 +48,10 @@ SIGNATURES: dict[str, list[Any]] = {
     "h3b_attention": [_p, _p, _p, _p] + [_i64] * 17 + [_f32, _p, _i64, _p],
     "h3b_attention_workspace_size": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "h3b_attention_noalloc": [_p, _p, _p, _p] + [_i64] * 17 + [_f32, _p],
+    "h3b_select_key_blocks": [_p] * 4 + [_i64] * 15 + [_p] * 3 + [_i64, _p, _i64, _p],
+    "h3b_select_key_blocks_workspace_size": [_i64] * 8 + [ctypes.POINTER(_i64)],
+    "h3b_block_sparse_attention": [_p] * 7 + [_i64] * 21 + [_p] * 2 + [_f32, _i64, _p, _i64, _p],
+    "h3b_block_sparse_attention_workspace_size": [_i64] * 6 + [ctypes.POINTER(_i64)],
     "h3b_clear_device_status": [_p],
     "h3b_qknorm_rope_pack_p2p": [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p,
                                  _p, _i64, _i64, _i64, _i64, _f32, _f32, _p],

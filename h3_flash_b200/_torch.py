@@ -35,6 +35,29 @@ def require_bf16(op: str, *tensors: torch.Tensor) -> None:
             raise TypeError(f"{op}: expected bfloat16 tensors, got {t.dtype}")
 
 
+# Element types of the entry points that take one (H3B_DTYPE_* in include/h3b.h).
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def dtype_code(op: str, allowed: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> int:
+    """The dtype argument for tensors that all have one of the ``allowed`` types."""
+
+    dtype = tensors[0].dtype
+    if dtype not in allowed:
+        raise TypeError(f"{op}: expected {' or '.join(str(d) for d in allowed)} tensors, got {dtype}")
+    for t in tensors:
+        if t.dtype != dtype:
+            raise TypeError(f"{op}: tensors have different types ({dtype}, {t.dtype})")
+    return DTYPE_CODES[dtype]
+
+
+def require_no_grad(op: str, *tensors: torch.Tensor) -> None:
+    """Inference only: a result that silently lost its gradient is refused."""
+
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op}: inference only; call it under torch.no_grad() or on detached tensors")
+
+
 def rows_view(t: torch.Tensor) -> torch.Tensor:
     """Flatten to [rows, cols] without copying when the last dim is contiguous and
     the leading dims collapse; otherwise copy (the reference's reshape().contiguous())."""

@@ -3,12 +3,16 @@
 #pragma once
 
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <stdint.h>
 
 #include "common.cuh"
 
 namespace h3b {
 namespace attn {
+
+// The driver's tensor-map encoder, or nullptr (defined in attention.cu).
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 
 // Limit of one mbarrier wait: 2 s.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;

@@ -1,0 +1,376 @@
+// Which key blocks each block of queries attends to: mean query and mean key of every
+// block, their products, the top_k best per query block.
+//
+//   Qm[i] = mean of the rows of query block i that exist     (fp64 sum, held in fp32)
+//   Km[j] = mean of the rows of key block j that exist       (the same)
+//   s[i, j] = Qm[i] . Km[j]                                  (fp64)
+//   list[i] = the top_k blocks by (kept, s, lowest index), written in ascending order
+//
+// The choice is discrete, so scores are compared where rounding cannot move them: a mean
+// of at most 256 16-bit values is summed in fp64 and the products of two fp32 means are
+// exact in fp64, which leaves 2^-52 relative in a score. Two devices, two batch layouts
+// or another summation order then choose alike.
+//
+// Two kernels. block_means reads q and k once (bound by HBM: everything else is small);
+// one warp per (block, head), heads of one block in neighbouring warps so that whole rows
+// are read together. score_select holds the scores of a few query blocks in shared memory
+// as order-preserving 64-bit keys and selects with one warp per row.
+#include <cuda_fp16.h>
+
+#include <cstdio>
+
+#include "common.cuh"
+
+namespace h3b {
+namespace select {
+
+constexpr int kMeanWarps = 4;
+
+struct MeanSide {
+  const void* x;
+  float* mean;  // q: [batch, heads, blocks, D]; k: [batch, heads, D, pitch]
+  int64_t batch_stride, row_stride, head_stride;
+  const int32_t* lens;
+  int seq, heads, block, blocks, pitch;
+  bool transposed;
+  int64_t warps;  // batch * blocks * heads
+};
+
+struct MeanArgs {
+  MeanSide side[2];
+  int64_t total;
+};
+
+__device__ __forceinline__ int rows_of(const int32_t* lens, int b, int seq) {
+  if (lens == nullptr) return seq;
+  const int n = lens[b];
+  return n < 0 ? 0 : (n > seq ? seq : n);
+}
+
+template <bool FP16>
+__device__ __forceinline__ void add8(double (&acc)[8], uint4 u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float2 f;
+    if (FP16) {
+      f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+    } else {
+      f = make_float2(bf16lo(w[j]), bf16hi(w[j]));
+    }
+    acc[2 * j] += (double)f.x;
+    acc[2 * j + 1] += (double)f.y;
+  }
+}
+
+// One warp per (batch, block, head): D/8 lanes hold the columns of a row, the others further rows.
+template <bool FP16, int D>
+__global__ void __launch_bounds__(kMeanWarps * 32) block_means(MeanArgs a) {
+  int64_t w = (int64_t)blockIdx.x * kMeanWarps + (threadIdx.x >> 5);
+  if (w >= a.total) return;
+  const int lane = threadIdx.x & 31;
+  const bool is_k = w >= a.side[0].warps;
+  const MeanSide& s = a.side[is_k ? 1 : 0];
+  if (is_k) w -= a.side[0].warps;
+  const int head = (int)(w % s.heads);
+  const int block = (int)(w / s.heads % s.blocks);
+  const int b = (int)(w / s.heads / s.blocks);
+  constexpr int kLanes = D / 8;          // lanes per row
+  constexpr int kRows = 32 / kLanes;     // rows per load
+  constexpr int kUnroll = 8;
+  const int col = (lane % kLanes) * 8;
+  const int row0 = block * s.block;
+  const int count = min(s.block, rows_of(s.lens, b, s.seq) - row0);
+  double acc[8] = {};
+  const char* base = (const char*)s.x + 2 * ((int64_t)b * s.batch_stride +
+                                             (int64_t)row0 * s.row_stride +
+                                             (int64_t)head * s.head_stride + col);
+  for (int r0 = lane / kLanes; r0 < count; r0 += kRows * kUnroll) {
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int r = r0 + i * kRows;
+      u[i] = r < count ? ld_cached(base + 2 * (int64_t)r * s.row_stride) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) add8<FP16>(acc, u[i]);
+  }
+#pragma unroll
+  for (int o = 16; o >= kLanes; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+  if (lane >= kLanes) return;
+  const double n = count > 0 ? (double)count : 1.0;
+  if (s.transposed) {
+    float* out = s.mean + (((int64_t)b * s.heads + head) * D + col) * s.pitch + block;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[(int64_t)j * s.pitch] = (float)(acc[j] / n);
+  } else {
+    float* out = s.mean + (((int64_t)b * s.heads + head) * s.blocks + block) * D + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = (float)(acc[j] / n);
+  }
+}
+
+struct SelectArgs {
+  int32_t* indices;
+  int32_t* counts;
+  const float* q_mean;
+  const float* k_mean;
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  const uint8_t* keep;
+  int heads, kv_heads, seq_q, seq_k, block_q, block_k, nq, nk, pitch, top_k;
+  int row_groups;  // CTAs per (batch, head)
+};
+
+// Order-preserving 64-bit key of a score; 0 is left for blocks that do not compete, the
+// largest value for kept ones that all fit. -0 and +0 are the same score, NaN ranks as -inf.
+__device__ __forceinline__ unsigned long long score_key(double s) {
+  if (s != s) s = -INFINITY;
+  s += 0.0;
+  const long long bits = __double_as_longlong(s);
+  return bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | (1ull << 63);
+}
+constexpr unsigned long long kKeepKey = ~0ull;
+
+constexpr int kSelectThreads = 256;
+
+// ROWS query blocks of one (batch, head) per CTA.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kSelectThreads) score_select(SelectArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  double* q_tile = reinterpret_cast<double*>(smem);  // [D][ROWS]
+  auto* keys = reinterpret_cast<unsigned long long*>(smem + sizeof(double) * D * ROWS);  // [ROWS][nk]
+  const int group = blockIdx.x % a.row_groups;
+  const int64_t bh = blockIdx.x / a.row_groups;
+  const int head = (int)(bh % a.heads);
+  const int b = (int)(bh / a.heads);
+  const int row0 = group * ROWS;
+  const int q_rows = rows_of(a.q_lens, b, a.seq_q);
+  const int k_rows = rows_of(a.k_lens, b, a.seq_k);
+  const int k_blocks = (k_rows + a.block_k - 1) / a.block_k;  // blocks that exist
+
+  for (int i = threadIdx.x; i < D * ROWS; i += kSelectThreads) {
+    const int r = i / D, d = i % D;
+    q_tile[d * ROWS + r] = row0 + r < a.nq ? (double)a.q_mean[(bh * a.nq + row0 + r) * D + d] : 0.0;
+  }
+  // More kept blocks than a list holds: only they compete, by score.
+  int kept_count = 0;
+  if (a.keep != nullptr)
+    for (int c = threadIdx.x; c < (k_blocks + kSelectThreads - 1) / kSelectThreads * kSelectThreads;
+         c += kSelectThreads)
+      kept_count += __syncthreads_count(c < k_blocks && a.keep[c] != 0);
+  const bool only_kept = kept_count > a.top_k;
+  __syncthreads();
+  const float* km = a.k_mean +
+                    ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * D * a.pitch;
+  for (int col = threadIdx.x; col < a.nk; col += kSelectThreads) {
+    double acc[ROWS] = {};
+#pragma unroll 8
+    for (int d = 0; d < D; ++d) {
+      const double kd = (double)km[(int64_t)d * a.pitch + col];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) acc[r] = fma(q_tile[d * ROWS + r], kd, acc[r]);
+    }
+    const bool kept = a.keep != nullptr && a.keep[col] != 0;
+    const bool competes = col < k_blocks && (kept || !only_kept);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      keys[(int64_t)r * a.nk + col] =
+          !competes ? 0ull : (kept && !only_kept ? kKeepKey : score_key(acc[r]));
+  }
+  __syncthreads();
+
+  const int lane = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < ROWS; r += kSelectThreads / 32) {
+    if (row0 + r >= a.nq) break;
+    const unsigned long long* row = keys + (int64_t)r * a.nk;
+    const int64_t list = bh * a.nq + row0 + r;
+    int32_t* out = a.indices + list * a.top_k;
+    const bool exists = (row0 + r) * a.block_q < q_rows;
+    const int want = exists ? min(a.top_k, k_blocks) : 0;
+    int done = 0;
+    if (want > 0) {
+      // Largest threshold t with at least `want` keys >= t, found bit by bit from the top:
+      // `prefix` holds the bits decided, `above` the keys whose decided bits are larger.
+      unsigned long long prefix = 0;
+      int above = 0, equal = a.nk;
+      int bit = 63;
+      for (; bit >= 0 && above + equal > want; --bit) {
+        const unsigned long long probe = prefix | (1ull << bit);
+        int n = 0;
+        for (int c = lane; c < a.nk; c += 32) n += (row[c] >> bit) == (probe >> bit);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (above + n >= want) {
+          prefix = probe;
+          equal = n;
+        } else {
+          above += n;
+          equal -= n;
+        }
+      }
+      // Keys above the decided prefix, then the lowest-index ones that equal it.
+      const int shift = bit + 1;
+      int ties = want - above;
+      for (int c0 = 0; c0 < a.nk && done < want; c0 += 32) {
+        const int c = c0 + lane;
+        const unsigned long long key = c < a.nk ? row[c] : 0ull;
+        const unsigned long long top = shift < 64 ? key >> shift : 0ull;
+        const unsigned long long ref = shift < 64 ? prefix >> shift : 0ull;
+        const bool tie = c < a.nk && top == ref;
+        const unsigned tie_mask = __ballot_sync(0xffffffffu, tie);
+        const bool take = (c < a.nk && top > ref) ||
+                          (tie && __popc(tie_mask & ((1u << lane) - 1u)) < ties);
+        const unsigned mask = __ballot_sync(0xffffffffu, take);
+        if (take) out[done + __popc(mask & ((1u << lane) - 1u))] = c;
+        done += __popc(mask);
+        ties -= min(ties, __popc(tie_mask));
+      }
+    }
+    for (int c = done + lane; c < a.top_k; c += 32) out[c] = -1;
+    if (lane == 0) a.counts[list] = done;
+  }
+}
+
+constexpr int kMaxKeyBlocks = 24576;  // scores of one query block fit in shared memory
+
+size_t select_smem(int head_dim, int rows, int64_t nk) {
+  return sizeof(double) * (size_t)head_dim * rows + 8 * (size_t)nk * rows;
+}
+
+template <int D, int ROWS>
+int launch_select(const SelectArgs& a, int64_t batch, size_t smem, cudaStream_t s) {
+  static ContextSlot slots[kMaxDevices];
+  cudaError_t e = cudaErrorInvalidDevice;
+  if (context_cached(slots, [&]() -> void* {
+        e = cudaFuncSetAttribute(score_select<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 227 * 1024);
+        return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
+      }) == nullptr) {
+    set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
+              cudaGetErrorString(e));
+    return H3B_ERR_CUDA;
+  }
+  const int64_t grid = batch * a.heads * a.row_groups;
+  H3B_REQUIRE(grid <= 0x7fffffffLL, "select_key_blocks: shape exceeds launch limits");
+  score_select<D, ROWS><<<(unsigned)grid, kSelectThreads, smem, s>>>(a);
+  return check_launch("h3b_select_key_blocks");
+}
+
+template <bool FP16, int D>
+int launch_all(const MeanArgs& m, SelectArgs a, int64_t batch, cudaStream_t s) {
+  const int64_t grid = (m.total + kMeanWarps - 1) / kMeanWarps;
+  H3B_REQUIRE(grid <= 0x7fffffffLL, "select_key_blocks: shape exceeds launch limits");
+  block_means<FP16, D><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
+  int rc = check_launch("h3b_select_key_blocks");
+  if (rc != H3B_OK) return rc;
+  // Query blocks per CTA: as many as there are and as shared memory holds; each reads the
+  // key means once.
+  int rows = 16;
+  while (rows > 1 && (rows / 2 >= a.nq || select_smem(D, rows, a.nk) > 200 * 1024)) rows /= 4;
+  a.row_groups = (a.nq + rows - 1) / rows;
+  const size_t smem = select_smem(D, rows, a.nk);
+  if (rows == 16) return launch_select<D, 16>(a, batch, smem, s);
+  if (rows == 4) return launch_select<D, 4>(a, batch, smem, s);
+  return launch_select<D, 1>(a, batch, smem, s);
+}
+
+}  // namespace select
+}  // namespace h3b
+
+extern "C" int h3b_select_key_blocks_workspace_size(int64_t batch, int64_t seq_q, int64_t seq_k,
+                                                    int64_t heads, int64_t kv_heads,
+                                                    int64_t head_dim, int64_t block_q,
+                                                    int64_t block_k, int64_t* bytes_out) {
+  H3B_REQUIRE(bytes_out != nullptr, "select_key_blocks_workspace_size: null output pointer");
+  H3B_REQUIRE(batch >= 0 && seq_q >= 0 && seq_k >= 0 && heads >= 0 && kv_heads >= 0 &&
+                  head_dim >= 0 && block_q > 0 && block_k > 0,
+              "select_key_blocks: negative shape");
+  const int64_t nq = (seq_q + block_q - 1) / block_q, nk = (seq_k + block_k - 1) / block_k;
+  const int64_t pitch = (nk + 31) / 32 * 32;
+  *bytes_out = 4 * batch * head_dim * (heads * nq + kv_heads * pitch);
+  return H3B_OK;
+}
+
+extern "C" int h3b_select_key_blocks(
+    int32_t* indices, int32_t* counts, const void* q, const void* k, int64_t batch, int64_t seq_q,
+    int64_t seq_k, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t block_q,
+    int64_t block_k, int64_t top_k, int64_t q_batch_stride, int64_t q_row_stride,
+    int64_t q_head_stride, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride,
+    const int32_t* q_lens, const int32_t* k_lens, const uint8_t* keep, int64_t dtype,
+    void* workspace, int64_t workspace_bytes, h3b_stream_t stream) {
+  using namespace h3b::select;
+  int64_t need = 0;
+  H3B_REQUIRE(batch >= 0 && seq_q >= 0 && seq_k >= 0 && heads >= 0 && kv_heads >= 0,
+              "select_key_blocks: negative shape");
+  if (!(head_dim == 64 || head_dim == 128) || !(block_q == 128 || block_q == 256) ||
+      !(block_k == 64 || block_k == 128) ||
+      !(dtype == H3B_DTYPE_BF16 || dtype == H3B_DTYPE_FP16)) {
+    h3b::set_error("h3b_select_key_blocks: needs bf16 or fp16, head_dim 64 or 128, block_q 128 or "
+                   "256, block_k 64 or 128");
+    return H3B_ERR_UNSUPPORTED;
+  }
+  if (batch == 0 || seq_q == 0 || heads == 0) return H3B_OK;
+  H3B_REQUIRE(seq_k > 0, "select_key_blocks: empty key sequence");
+  H3B_REQUIRE(kv_heads > 0 && heads % kv_heads == 0,
+              "select_key_blocks: heads (%lld) must be a multiple of kv_heads (%lld)",
+              (long long)heads, (long long)kv_heads);
+  H3B_REQUIRE(seq_q < (1LL << 31) - 256 && seq_k < (1LL << 31) - 256,
+              "select_key_blocks: shape exceeds launch limits");
+  const int64_t nq = (seq_q + block_q - 1) / block_q, nk = (seq_k + block_k - 1) / block_k;
+  H3B_REQUIRE(top_k >= 1 && top_k <= nk, "select_key_blocks: top_k (%lld) must be 1..%lld",
+              (long long)top_k, (long long)nk);
+  if (nk > kMaxKeyBlocks) {
+    h3b::set_error("h3b_select_key_blocks: more than 24576 key blocks");
+    return H3B_ERR_UNSUPPORTED;
+  }
+  H3B_REQUIRE(batch <= (1LL << 31) / heads && batch * heads <= (1LL << 31) / nq,
+              "select_key_blocks: shape exceeds launch limits");
+  H3B_REQUIRE(indices != nullptr && counts != nullptr && q != nullptr && k != nullptr,
+              "select_key_blocks: null argument");
+  H3B_REQUIRE(h3b::aligned16(q) && h3b::aligned16(k), "select_key_blocks: q and k must be 16-byte aligned");
+  const int64_t strides[6] = {q_batch_stride, q_row_stride, q_head_stride,
+                              k_batch_stride, k_row_stride, k_head_stride};
+  for (int i = 0; i < 6; ++i)
+    H3B_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0,
+                "select_key_blocks: strides must be multiples of 8 elements");
+  int rc = h3b_select_key_blocks_workspace_size(batch, seq_q, seq_k, heads, kv_heads, head_dim,
+                                                block_q, block_k, &need);
+  if (rc != H3B_OK) return rc;
+  H3B_REQUIRE(workspace != nullptr && workspace_bytes >= need && h3b::aligned16(workspace),
+              "select_key_blocks: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  const int pitch = (int)((nk + 31) / 32 * 32);
+  float* q_mean = static_cast<float*>(workspace);
+  float* k_mean = q_mean + batch * heads * nq * head_dim;
+  MeanArgs m{};
+  m.side[0] = MeanSide{q, q_mean, q_batch_stride, q_row_stride, q_head_stride, q_lens,
+                       (int)seq_q, (int)heads, (int)block_q, (int)nq, 0, false, batch * nq * heads};
+  m.side[1] = MeanSide{k, k_mean, k_batch_stride, k_row_stride, k_head_stride, k_lens,
+                       (int)seq_k, (int)kv_heads, (int)block_k, (int)nk, pitch, true,
+                       batch * nk * kv_heads};
+  m.total = m.side[0].warps + m.side[1].warps;
+  SelectArgs a{};
+  a.indices = indices;
+  a.counts = counts;
+  a.q_mean = q_mean;
+  a.k_mean = k_mean;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.keep = keep;
+  a.heads = (int)heads;
+  a.kv_heads = (int)kv_heads;
+  a.seq_q = (int)seq_q;
+  a.seq_k = (int)seq_k;
+  a.block_q = (int)block_q;
+  a.block_k = (int)block_k;
+  a.nq = (int)nq;
+  a.nk = (int)nk;
+  a.pitch = pitch;
+  a.top_k = (int)top_k;
+  if (dtype == H3B_DTYPE_FP16)
+    return head_dim == 128 ? launch_all<true, 128>(m, a, batch, stream)
+                           : launch_all<true, 64>(m, a, batch, stream);
+  return head_dim == 128 ? launch_all<false, 128>(m, a, batch, stream)
+                         : launch_all<false, 64>(m, a, batch, stream);
+}

@@ -1,0 +1,224 @@
+// Norms after and before a branch fused with its gate and the scaled residual.
+//
+//   b      = RMSNorm(branch) * post_weight
+//   hidden = residual_scale * residual + gate[idx] * b                        (out0)
+//   normed = RMSNorm(hidden) * weight * (1 + scale[idx]) + shift[idx]         (out1, optional)
+//
+// Bound by HBM: a row of branch and of residual is read once, hidden and normed are
+// written once; the two reductions and everything between them stay in registers. Sums of
+// squares and all products are fp32, each output is rounded once to its own type, and
+// normed is taken from the unrounded hidden.
+#include <cuda_fp16.h>
+
+#include <cstdio>
+
+#include "common.cuh"
+
+namespace h3b {
+namespace {
+
+struct SandwichArgs {
+  void* hidden;
+  void* normed;  // null: no second norm
+  const void* residual;
+  const void* branch;
+  const void* post_weight;
+  const void* gate;
+  const void* weight;
+  const void* scale;
+  const void* shift;
+  const int64_t* index;
+  int64_t rows, cols, n_index, n_table;
+  int64_t residual_stride, branch_stride, hidden_stride, normed_stride;
+  int64_t gate_stride, scale_stride, shift_stride;
+  float residual_scale, post_eps, eps;
+};
+
+// 16 bytes of T as floats and back.
+template <class T>
+struct Vec;
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kN]) {
+    const f8 r = unpack8(u);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) v[j] = r.v[j];
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[kN]) { return pack8(v); }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kN]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[kN]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ void unpack(uint4 u, float (&v)[kN]) {
+    v[0] = __uint_as_float(u.x);
+    v[1] = __uint_as_float(u.y);
+    v[2] = __uint_as_float(u.z);
+    v[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[kN]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                      __float_as_uint(v[3]));
+  }
+};
+
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(float x) { return x; }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_float(float x) {
+  return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ float from_float(float x) {
+  return x;
+}
+
+// Table row of activation row `row`. An entry outside the table reads the nearest row
+// instead of memory past it.
+__device__ __forceinline__ int64_t table_row(const SandwichArgs& a, int64_t row) {
+  const int64_t t = a.index[a.n_index == 1 ? 0 : row % a.n_index];
+  return t < 0 ? 0 : (t >= a.n_table ? a.n_table - 1 : t);
+}
+
+// Sum over the whole CTA (`warps` warps); red holds one float per warp.
+template <int WARPS>
+__device__ __forceinline__ float cta_sum(float v, float* red) {
+  v = warp_sum(v);
+  if (WARPS == 1) return v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) s += red[w];
+  return s;
+}
+
+// Any width and alignment: one CTA per row, scalar accesses, hidden recomputed from L1/L2.
+constexpr int kScalarWarps = 8;
+template <class T>
+__global__ void __launch_bounds__(kScalarWarps * 32) sandwich_scalar(SandwichArgs a) {
+  __shared__ float red[2][kScalarWarps];
+  const int64_t row = blockIdx.x;
+  const int64_t t = table_row(a, row);
+  const T* residual = (const T*)a.residual + row * a.residual_stride;
+  const T* branch = (const T*)a.branch + row * a.branch_stride;
+  const T* gate = (const T*)a.gate + t * a.gate_stride;
+  const T* post_weight = (const T*)a.post_weight;
+  float ss = 0.f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+    const float x = to_float(branch[c]);
+    ss += x * x;
+  }
+  ss = cta_sum<kScalarWarps>(ss, red[0]);
+  const float post_rstd = rsqrtf(ss / (float)a.cols + a.post_eps);
+  auto hidden_at = [&](int64_t c) {
+    return a.residual_scale * to_float(residual[c]) +
+           to_float(gate[c]) * (to_float(branch[c]) * post_rstd * to_float(post_weight[c]));
+  };
+  T* hidden = (T*)a.hidden + row * a.hidden_stride;
+  float hh = 0.f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+    const float h = hidden_at(c);
+    hidden[c] = from_float<T>(h);
+    hh += h * h;
+  }
+  if (a.normed == nullptr) return;
+  hh = cta_sum<kScalarWarps>(hh, red[1]);
+  const float rstd = rsqrtf(hh / (float)a.cols + a.eps);
+  const T* weight = (const T*)a.weight;
+  const T* scale = (const T*)a.scale + t * a.scale_stride;
+  const T* shift = (const T*)a.shift + t * a.shift_stride;
+  T* normed = (T*)a.normed + row * a.normed_stride;
+  for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x)
+    normed[c] = from_float<T>(hidden_at(c) * rstd * to_float(weight[c]) *
+                                  (1.f + to_float(scale[c])) + to_float(shift[c]));
+}
+
+template <class T>
+int launch_sandwich(const SandwichArgs& a, cudaStream_t s, const char* name) {
+  H3B_REQUIRE(a.rows <= 0x7fffffffLL, "%s: too many rows (%lld)", name, (long long)a.rows);
+  sandwich_scalar<T><<<(unsigned)a.rows, kScalarWarps * 32, 0, s>>>(a);
+  return check_launch(name);
+}
+
+}  // namespace
+}  // namespace h3b
+
+extern "C" int h3b_sandwich_residual_rmsnorm_modulate(
+    void* hidden_out, void* normed_out, const void* residual, const void* branch,
+    const void* post_weight, const void* gate, const void* weight, const void* scale,
+    const void* shift, const int64_t* index, int64_t rows, int64_t cols, int64_t n_index,
+    int64_t n_table, int64_t residual_row_stride, int64_t branch_row_stride,
+    int64_t out_row_stride, int64_t gate_row_stride, int64_t scale_row_stride,
+    int64_t shift_row_stride, float residual_scale, float post_eps, float eps, int64_t dtype,
+    h3b_stream_t stream) {
+  const char* name = "h3b_sandwich_residual_rmsnorm_modulate";
+  H3B_REQUIRE(rows >= 0 && cols >= 0, "sandwich_residual_rmsnorm_modulate: negative shape");
+  H3B_REQUIRE(dtype >= 0 && dtype <= 2, "sandwich_residual_rmsnorm_modulate: unknown dtype %lld",
+              (long long)dtype);
+  if (rows == 0 || cols == 0) return H3B_OK;
+  H3B_REQUIRE(n_index > 0 && n_table > 0,
+              "sandwich_residual_rmsnorm_modulate: empty index or table");
+  H3B_REQUIRE(hidden_out != nullptr && residual != nullptr && branch != nullptr &&
+                  post_weight != nullptr && gate != nullptr && index != nullptr,
+              "sandwich_residual_rmsnorm_modulate: null argument");
+  H3B_REQUIRE(normed_out == nullptr ||
+                  (weight != nullptr && scale != nullptr && shift != nullptr),
+              "sandwich_residual_rmsnorm_modulate: normed needs weight, scale and shift");
+  h3b::SandwichArgs a{};
+  a.hidden = hidden_out;
+  a.normed = normed_out;
+  a.residual = residual;
+  a.branch = branch;
+  a.post_weight = post_weight;
+  a.gate = gate;
+  a.weight = weight;
+  a.scale = scale;
+  a.shift = shift;
+  a.index = index;
+  a.rows = rows;
+  a.cols = cols;
+  a.n_index = n_index;
+  a.n_table = n_table;
+  a.residual_stride = residual_row_stride;
+  a.branch_stride = branch_row_stride;
+  a.hidden_stride = a.normed_stride = out_row_stride;
+  a.gate_stride = gate_row_stride;
+  a.scale_stride = scale_row_stride;
+  a.shift_stride = shift_row_stride;
+  a.residual_scale = residual_scale;
+  a.post_eps = post_eps;
+  a.eps = eps;
+  if (dtype == H3B_DTYPE_BF16) return h3b::launch_sandwich<__nv_bfloat16>(a, stream, name);
+  if (dtype == H3B_DTYPE_FP16) return h3b::launch_sandwich<__half>(a, stream, name);
+  return h3b::launch_sandwich<float>(a, stream, name);
+}

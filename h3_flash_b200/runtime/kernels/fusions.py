@@ -18,10 +18,12 @@ import torch
 from ... import _lib
 from ..._torch import (
     call,
+    dtype_code,
     index64,
     ptr,
     require_bf16,
     require_cuda,
+    require_no_grad,
     rows_view,
     stream_of,
     table_rows,
@@ -89,6 +91,73 @@ def fused_residual_gate_rmsnorm_modulate(residual, branch, gate, weight, scale, 
         scale_stride, shift_stride, float(eps), stream_of(residual),
     )
     return hidden.view(residual.shape), normed.view(residual.shape)
+
+
+_FLOAT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps, residual_scale):
+    """Checks and launch shared by the sandwich-norm ops; ``pre`` is (weight, scale, shift)
+    of the norm before the next branch, or None."""
+
+    tensors = (residual, branch, post_weight, gate, *(pre or ()))
+    require_cuda(op, *tensors)
+    dtype = dtype_code(op, _FLOAT_TYPES, *tensors)
+    require_no_grad(op, *tensors)
+    columns = residual.shape[-1]
+    if branch.shape != residual.shape:
+        raise ValueError(f"{op}: residual and branch must have the same shape")
+    for name, t in (("post_weight", post_weight), *((("weight", pre[0]),) if pre else ())):
+        if t.shape != (columns,):
+            raise ValueError(f"{op}: {name} must have shape ({columns},), got {tuple(t.shape)}")
+    tables = [table_rows(t) for t in (gate, *(pre[1:] if pre else ()))]
+    if any(t.shape[-1] != columns for t, _ in tables):
+        raise ValueError(f"{op}: tables must be {columns} wide")
+    n_table = tables[0][0].numel() // columns if columns else 0
+    if any(t.numel() != tables[0][0].numel() for t, _ in tables):
+        raise ValueError(f"{op}: gate, scale and shift must have the same rows")
+    residual_flat, branch_flat = rows_view(residual), rows_view(branch)
+    idx = index64(index, residual.device)
+    rows = residual_flat.shape[0]
+    hidden = torch.empty((rows, columns), dtype=residual.dtype, device=residual.device)
+    normed = torch.empty_like(hidden) if pre else None
+    if rows == 0 or columns == 0:
+        return hidden.view(residual.shape), normed.view(residual.shape) if pre else None
+    if idx.numel() == 0 or n_table == 0:
+        raise ValueError(f"{op}: empty index or table")
+    post_weight = post_weight.contiguous()
+    weight = pre[0].contiguous() if pre else None
+    with torch.cuda.device(residual.device):
+        call("h3b_sandwich_residual_rmsnorm_modulate", ptr(hidden), ptr(normed) if pre else None,
+             ptr(residual_flat), ptr(branch_flat), ptr(post_weight), ptr(tables[0][0]),
+             ptr(weight) if pre else None, ptr(tables[1][0]) if pre else None,
+             ptr(tables[2][0]) if pre else None, ptr(idx), rows, columns, idx.numel(), n_table,
+             residual_flat.stride(0), branch_flat.stride(0), columns, tables[0][1],
+             tables[1][1] if pre else 0, tables[2][1] if pre else 0, float(residual_scale),
+             float(post_eps), float(eps), dtype, stream_of(residual))
+    return hidden.view(residual.shape), normed.view(residual.shape) if pre else None
+
+
+def fused_sandwich_residual_rmsnorm_modulate(residual, branch, post_weight, gate, weight, scale, shift,
+                                             index, post_eps, eps, residual_scale=1.0):
+    """The joint between two branches that end in a norm:
+    hidden = residual_scale*residual + gate[idx]*(RMSNorm(branch)*post_weight);
+    normed = RMSNorm(hidden)*weight*(1+scale[idx])+shift[idx], idx = index[row % len(index)].
+    Returns (hidden, normed). bf16, fp16 or fp32, one type for all tensors; any width and
+    row strides. ``index`` entries outside the tables read the nearest row; None is row 0.
+    Inference only: tensors that require grad are refused outside torch.no_grad()."""
+
+    return _sandwich("fused_sandwich_residual_rmsnorm_modulate", residual, branch, post_weight, gate,
+                     (weight, scale, shift), index, post_eps, eps, residual_scale)
+
+
+def fused_sandwich_residual(residual, branch, post_weight, gate, index, post_eps, residual_scale=1.0):
+    """residual_scale*residual + gate[idx]*(RMSNorm(branch)*post_weight): the end of a block
+    whose last branch ends in a norm. Types, widths and ``index`` as in
+    ``fused_sandwich_residual_rmsnorm_modulate``."""
+
+    return _sandwich("fused_sandwich_residual", residual, branch, post_weight, gate, None, index, post_eps,
+                     0.0, residual_scale)[0]
 
 
 def fused_swiglu(x):

@@ -8,7 +8,7 @@
  *   - is stream-ordered: it never synchronises the host and never allocates;
  *   - returns H3B_OK (0) or an error code; h3b_last_error() then returns a
  *     message for the calling thread.
- * Tensors are bf16 (IEEE bfloat16 bit patterns) unless stated; RoPE tables are
+ * Tensors are bf16 (IEEE bfloat16 bit patterns) unless stated or a dtype argument says otherwise; RoPE tables are
  * fp32; AdaLN table indices are int64. Strides are in elements.
  *
  * Each declaration names the reference interface it replaces
@@ -30,7 +30,13 @@ typedef struct CUstream_st* h3b_stream_t; /* == cudaStream_t */
 #define H3B_ERR_CUDA 2        /* CUDA launch or driver error: RuntimeError         */
 #define H3B_ERR_UNSUPPORTED 3 /* valid input this build does not handle: RuntimeError */
 
-#define H3B_ABI_VERSION 8
+/* Element types of the entry points that take a `dtype` argument (all their
+ * activations, weights and tables have that type). */
+#define H3B_DTYPE_BF16 0
+#define H3B_DTYPE_FP16 1
+#define H3B_DTYPE_FP32 2
+
+#define H3B_ABI_VERSION 9
 
 int h3b_abi_version(void);
 /* Kernels launched through this library by this process (all devices and host
@@ -47,7 +53,8 @@ const char* h3b_last_error(void);
  * h3b_clear_device_status() zeroes it (stream-ordered). Bits:
  *   1 = attention pipeline wait timed out;
  *   2 = h3b_peer_barrier gave up waiting for a peer (10 s);
- *   4 = QKV GEMM pipeline wait timed out. */
+ *   4 = QKV GEMM pipeline wait timed out.
+ * Bit 1 also reports a pipeline wait of the block-sparse attention. */
 int h3b_device_status(int* status_out);
 int h3b_clear_device_status(h3b_stream_t stream);
 
@@ -94,6 +101,24 @@ int h3b_gated_residual(void* out, const void* residual, const void* branch,
                        const void* gate, const int64_t* index, int64_t rows,
                        int64_t cols, int64_t n_index, int64_t row_stride,
                        int64_t gate_row_stride, h3b_stream_t stream);
+
+/* The joint between two branches that end in a norm ("sandwich" norm):
+ *   hidden = residual_scale*residual + gate[idx] * (RMSNorm(branch)*post_weight)  (stored)
+ *   normed = RMSNorm(hidden_fp32)*weight*(1+scale[idx])+shift[idx]
+ * With normed_out NULL only hidden is written (the end of a block; weight, scale, shift
+ * and eps are then unused). dtype is H3B_DTYPE_*, of every tensor. An index entry outside
+ * [0, n_table) reads the nearest table row. hidden_out and normed_out share
+ * out_row_stride and must not overlap an input.
+ * The gated-residual chain of kernels/transformer.py:75-111 for blocks with a norm
+ * after the branch; no reference kernel */
+int h3b_sandwich_residual_rmsnorm_modulate(
+    void* hidden_out, void* normed_out, const void* residual, const void* branch,
+    const void* post_weight, const void* gate, const void* weight, const void* scale,
+    const void* shift, const int64_t* index, int64_t rows, int64_t cols, int64_t n_index,
+    int64_t n_table, int64_t residual_row_stride, int64_t branch_row_stride,
+    int64_t out_row_stride, int64_t gate_row_stride, int64_t scale_row_stride,
+    int64_t shift_row_stride, float residual_scale, float post_eps, float eps, int64_t dtype,
+    h3b_stream_t stream);
 
 /* out[r, :n] = x[r, :n] * silu(x[r, n:2n])
  * replaces fused_swiglu  fusions.py:251 (_swiglu_kernel fusions.py:98-123) */
@@ -262,6 +287,66 @@ int h3b_attention_noalloc(void* out, const void* q, const void* k, const void* v
                           int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride,
                           int64_t o_batch_stride, int64_t o_row_stride, int64_t o_head_stride,
                           float softmax_scale, h3b_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Block-sparse attention: every block of block_q query rows attends to its own
+ * list of blocks of block_k keys.
+ * q [batch, seq_q, heads, head_dim], k and v [batch, seq_k, kv_heads, head_dim] are
+ * views by element strides as for h3b_attention; heads is a multiple of kv_heads
+ * and query head h reads key head h / (heads / kv_heads). dtype is
+ * H3B_DTYPE_BF16 or _FP16, head_dim 64 or 128, block_q 128 or 256, block_k 64 or
+ * 128 (else H3B_ERR_UNSUPPORTED). q_lens / k_lens (int32 [batch], or NULL: all
+ * rows) give the rows of each batch entry that exist; what lies behind them may
+ * be anything, NaN included. nq = ceil(seq_q / block_q), nk = ceil(seq_k / block_k).
+ * No reference counterpart: the reference's attention is dense.
+ * ------------------------------------------------------------------------- */
+
+/* The top_k key blocks of every query block, by the product of the block's mean
+ * query with the block's mean key (sums in fp64, means held in fp32, products
+ * summed in fp64). Blocks marked in keep (bool [nk], or NULL) come first; ties go to the lowest
+ * index; a NaN product ranks as -inf; blocks without rows are never taken.
+ * indices int32 [batch, heads, nq, top_k], ascending, -1 behind the last;
+ * counts int32 [batch, heads, nq] (0 for query blocks without rows).
+ * 1 <= top_k <= nk. workspace: h3b_select_key_blocks_workspace_size bytes,
+ * 16-byte aligned, used only during the call's kernels. */
+int h3b_select_key_blocks(int32_t* indices, int32_t* counts, const void* q, const void* k,
+                          int64_t batch, int64_t seq_q, int64_t seq_k, int64_t heads,
+                          int64_t kv_heads, int64_t head_dim, int64_t block_q,
+                          int64_t block_k, int64_t top_k,
+                          int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+                          int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride,
+                          const int32_t* q_lens, const int32_t* k_lens, const uint8_t* keep,
+                          int64_t dtype, void* workspace, int64_t workspace_bytes,
+                          h3b_stream_t stream);
+int h3b_select_key_blocks_workspace_size(int64_t batch, int64_t seq_q, int64_t seq_k,
+                                         int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t block_q, int64_t block_k, int64_t* bytes_out);
+
+/* out = softmax(q k^T * softmax_scale) v over the keys of the listed blocks.
+ * indices int32 [batch, heads, nq, list_len]: the first counts[...] entries of a list
+ * count (counts int32 [batch, heads, nq], or NULL: all of them), in any order; an
+ * entry outside [0, nk) adds nothing, an entry that is there twice counts twice.
+ * Query rows that have no key, and rows behind q_lens, get zeros. lse (fp32
+ * [batch, heads, seq_q], or NULL) gets log(sum(exp(score))), -inf for those rows.
+ * softmax_scale must be positive and finite. workspace as for h3b_attention
+ * (h3b_block_sparse_attention_workspace_size). */
+int h3b_block_sparse_attention(void* out, float* lse, const void* q, const void* k,
+                               const void* v, const int32_t* indices, const int32_t* counts,
+                               int64_t list_len, int64_t batch, int64_t seq_q, int64_t seq_k,
+                               int64_t heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t block_q, int64_t block_k,
+                               int64_t q_batch_stride, int64_t q_row_stride,
+                               int64_t q_head_stride, int64_t k_batch_stride,
+                               int64_t k_row_stride, int64_t k_head_stride,
+                               int64_t v_batch_stride, int64_t v_row_stride,
+                               int64_t v_head_stride, int64_t o_batch_stride,
+                               int64_t o_row_stride, int64_t o_head_stride,
+                               const int32_t* q_lens, const int32_t* k_lens,
+                               float softmax_scale, int64_t dtype, void* workspace,
+                               int64_t workspace_bytes, h3b_stream_t stream);
+int h3b_block_sparse_attention_workspace_size(int64_t batch, int64_t seq_q, int64_t heads,
+                                              int64_t head_dim, int64_t block_k,
+                                              int64_t list_len, int64_t* bytes_out);
 
 /* ---------------------------------------------------------------------------
  * Packed-Ulysses exchange over NVLink peer memory. Each rank owns one receive
