@@ -10,7 +10,7 @@ from . import _lib
 def stream_of(tensor: torch.Tensor) -> int:
     """Raw cudaStream_t of the current torch stream on the tensor's device."""
 
-    return torch.cuda.current_stream(tensor.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 def require_cuda(op: str, *tensors: torch.Tensor) -> None:
@@ -39,23 +39,27 @@ def require_bf16(op: str, *tensors: torch.Tensor) -> None:
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def dtype_code(op: str, allowed: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> int:
-    """The dtype argument for tensors that all have one of the ``allowed`` types."""
+def check_inputs(op: str, allowed: tuple[torch.dtype, ...], tensors: tuple[torch.Tensor, ...]) -> int:
+    """The dtype argument for CUDA tensors of one device that all have one of the ``allowed``
+    types. Inference only: under grad mode a tensor that requires grad is refused, since the
+    result would silently lose its gradient. One loop: this is on the path of calls that
+    take a few microseconds on the GPU."""
 
-    dtype = tensors[0].dtype
+    first = tensors[0]
+    grad = torch.is_grad_enabled()
+    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        require_cuda(op, *tensors)
+    dtype, device = first.dtype, first.device
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.device != device:
+            require_cuda(op, *tensors)
+        if t.dtype is not dtype:
+            raise TypeError(f"{op}: tensors have different types ({dtype}, {t.dtype})")
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{op}: inference only; call it under torch.no_grad() or on detached tensors")
     if dtype not in allowed:
         raise TypeError(f"{op}: expected {' or '.join(str(d) for d in allowed)} tensors, got {dtype}")
-    for t in tensors:
-        if t.dtype != dtype:
-            raise TypeError(f"{op}: tensors have different types ({dtype}, {t.dtype})")
     return DTYPE_CODES[dtype]
-
-
-def require_no_grad(op: str, *tensors: torch.Tensor) -> None:
-    """Inference only: a result that silently lost its gradient is refused."""
-
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op}: inference only; call it under torch.no_grad() or on detached tensors")
 
 
 def rows_view(t: torch.Tensor) -> torch.Tensor:
@@ -106,3 +110,14 @@ def ptr(t: torch.Tensor) -> int:
 
 def call(name: str, *args) -> None:
     _lib.call(name, *args)
+
+
+def call_on(tensor: torch.Tensor, name: str, *args) -> None:
+    """``call`` with the tensor's device current, on its current stream (the last argument)."""
+
+    device = tensor.get_device()
+    if torch.cuda.current_device() == device:
+        _lib.call(name, *args, stream_of(tensor))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream_of(tensor))

@@ -163,10 +163,130 @@ __global__ void __launch_bounds__(kScalarWarps * 32) sandwich_scalar(SandwichArg
                                   (1.f + to_float(scale[c])) + to_float(shift[c]));
 }
 
+// The row in registers: WARPS warps per row, NCH 16-byte chunks per thread. Both inputs and
+// the first tables are loaded up front; after the first reduction the 8 registers that held
+// a chunk of branch and residual hold hidden in fp32.
+template <class T, int WARPS, int NCH, bool NORMED>
+__global__ void __launch_bounds__(WARPS * 32) sandwich_vec(SandwichArgs a) {
+  constexpr int kN = Vec<T>::kN;
+  constexpr int kThreads = WARPS * 32;
+  __shared__ float red[2][WARPS];
+  const int64_t row = blockIdx.x;
+  const int cols = (int)a.cols;
+  const T* residual = (const T*)a.residual + row * a.residual_stride;
+  const T* branch = (const T*)a.branch + row * a.branch_stride;
+  uint4 raw_b[NCH], raw_r[NCH];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * kThreads + threadIdx.x) * kN;
+    if (col < cols) {
+      raw_b[c] = ld_stream(branch + col);
+      raw_r[c] = ld_stream(residual + col);
+    } else {
+      raw_b[c] = raw_r[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int64_t t = table_row(a, row);
+  const T* gate = (const T*)a.gate + t * a.gate_stride;
+  const T* post_weight = (const T*)a.post_weight;
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    float x[kN];
+    Vec<T>::unpack(raw_b[c], x);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) ss += x[j] * x[j];
+  }
+  ss = cta_sum<WARPS>(ss, red[0]);
+  const float post_rstd = rsqrtf(ss / (float)cols + a.post_eps);
+  T* hidden = (T*)a.hidden + row * a.hidden_stride;
+  float h[NCH][kN];
+  float hh = 0.f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * kThreads + threadIdx.x) * kN;
+    if (col < cols) {
+      float x[kN], r[kN], g[kN], w[kN];
+      Vec<T>::unpack(raw_b[c], x);
+      Vec<T>::unpack(raw_r[c], r);
+      Vec<T>::unpack(ld_cached(gate + col), g);
+      Vec<T>::unpack(ld_cached(post_weight + col), w);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        h[c][j] = a.residual_scale * r[j] + g[j] * (x[j] * post_rstd * w[j]);
+        hh += h[c][j] * h[c][j];
+      }
+      st_stream(hidden + col, Vec<T>::pack(h[c]));
+    }
+  }
+  if (!NORMED) return;
+  hh = cta_sum<WARPS>(hh, red[1]);
+  const float rstd = rsqrtf(hh / (float)cols + a.eps);
+  const T* weight = (const T*)a.weight;
+  const T* scale = (const T*)a.scale + t * a.scale_stride;
+  const T* shift = (const T*)a.shift + t * a.shift_stride;
+  T* normed = (T*)a.normed + row * a.normed_stride;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * kThreads + threadIdx.x) * kN;
+    if (col < cols) {
+      float w[kN], sc[kN], sh[kN], o[kN];
+      Vec<T>::unpack(ld_cached(weight + col), w);
+      Vec<T>::unpack(ld_cached(scale + col), sc);
+      Vec<T>::unpack(ld_cached(shift + col), sh);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) o[j] = h[c][j] * rstd * w[j] * (1.f + sc[j]) + sh[j];
+      st_stream(normed + col, Vec<T>::pack(o));
+    }
+  }
+}
+
+template <class T, int WARPS, int NCH>
+void launch_vec(const SandwichArgs& a, cudaStream_t s) {
+  if (a.normed != nullptr)
+    sandwich_vec<T, WARPS, NCH, true><<<(unsigned)a.rows, WARPS * 32, 0, s>>>(a);
+  else
+    sandwich_vec<T, WARPS, NCH, false><<<(unsigned)a.rows, WARPS * 32, 0, s>>>(a);
+}
+
+// Fewest chunks per thread that up to four keep the row in registers: threads first.
+template <class T, int WARPS>
+void launch_chunks(const SandwichArgs& a, int chunks, cudaStream_t s) {
+  const int nch = (chunks + WARPS * 32 - 1) / (WARPS * 32);
+  if (nch == 1) launch_vec<T, WARPS, 1>(a, s);
+  else if (nch == 2) launch_vec<T, WARPS, 2>(a, s);
+  else if (nch == 3) launch_vec<T, WARPS, 3>(a, s);
+  else launch_vec<T, WARPS, 4>(a, s);
+}
+
+template <class T>
+bool vector_rows(const SandwichArgs& a) {
+  constexpr int kN = Vec<T>::kN;
+  const bool second = a.normed != nullptr;
+  const void* bases[] = {a.hidden, a.residual, a.branch, a.post_weight, a.gate,
+                         second ? a.normed : a.hidden, second ? a.weight : a.gate,
+                         second ? a.scale : a.gate, second ? a.shift : a.gate};
+  for (const void* p : bases)
+    if (!aligned16(p)) return false;
+  const int64_t strides[] = {a.hidden_stride, a.residual_stride, a.branch_stride, a.gate_stride,
+                             second ? a.scale_stride : 0, second ? a.shift_stride : 0};
+  for (int64_t v : strides)
+    if (v % kN != 0) return false;
+  return a.cols % kN == 0 && a.cols / kN <= 4 * 512;
+}
+
 template <class T>
 int launch_sandwich(const SandwichArgs& a, cudaStream_t s, const char* name) {
   H3B_REQUIRE(a.rows <= 0x7fffffffLL, "%s: too many rows (%lld)", name, (long long)a.rows);
-  sandwich_scalar<T><<<(unsigned)a.rows, kScalarWarps * 32, 0, s>>>(a);
+  if (!vector_rows<T>(a)) {
+    sandwich_scalar<T><<<(unsigned)a.rows, kScalarWarps * 32, 0, s>>>(a);
+    return check_launch(name);
+  }
+  const int chunks = (int)(a.cols / Vec<T>::kN);
+  if (chunks <= 4 * 32) launch_chunks<T, 1>(a, chunks, s);
+  else if (chunks <= 4 * 128) launch_chunks<T, 4>(a, chunks, s);
+  else if (chunks <= 4 * 256) launch_chunks<T, 8>(a, chunks, s);
+  else launch_chunks<T, 16>(a, chunks, s);
   return check_launch(name);
 }
 

@@ -15,13 +15,13 @@ into a result. All ops are inference only and run on the current stream of the t
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
-from ... import _lib
-from ..._torch import call, dtype_code, ptr, require_cuda, require_no_grad, stream_of
-from .dense import HEAD_DIM, _check_view
+from ..._torch import call, call_on, check_inputs, require_cuda
+from .dense import HEAD_DIM
 
 BLOCK_Q = (128, 256)
 BLOCK_K = (64, 128)
@@ -29,22 +29,31 @@ HEAD_DIMS = (64, 128)
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _check_heads(op: str, q: torch.Tensor, k: torch.Tensor, block_q: int, block_k: int) -> int:
-    require_cuda(op, q, k)
-    dtype = dtype_code(op, _TYPES, q, k)
+def _check_shapes(op: str, q: torch.Tensor, k: torch.Tensor, block_q: int, block_k: int) -> None:
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"{op}: expected [batch, seq, heads, head_dim] tensors")
     b, _, h, d = q.shape
-    if k.shape[0] != b or k.shape[3] != d:
+    kb, _, hk, kd = k.shape
+    if kb != b or kd != d:
         raise ValueError(f"{op}: q {tuple(q.shape)} and k {tuple(k.shape)} disagree")
     if d not in HEAD_DIMS:
         raise RuntimeError(f"{op}: head_dim must be one of {HEAD_DIMS}, got {d}")
     if block_q not in BLOCK_Q or block_k not in BLOCK_K:
         raise ValueError(f"{op}: block_q must be one of {BLOCK_Q} and block_k one of {BLOCK_K}, got "
                          f"{block_q} and {block_k}")
-    if k.shape[2] == 0 or h % k.shape[2]:
-        raise ValueError(f"{op}: {h} query heads are not a multiple of {k.shape[2]} key heads")
-    return dtype
+    if hk == 0 or h % hk:
+        raise ValueError(f"{op}: {h} query heads are not a multiple of {hk} key heads")
+
+
+def _strides(op: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(batch, row, head) strides of a view the kernels can address."""
+
+    *strides, last = t.stride()
+    if last != 1:
+        raise ValueError(f"{op}: {name}: head_dim must be contiguous")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{op}: {name}: base address must be 16-byte aligned")
+    return strides
 
 
 def _side_tensor(op: str, name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple[int, ...],
@@ -53,14 +62,24 @@ def _side_tensor(op: str, name: str, t: torch.Tensor | None, dtype: torch.dtype,
 
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device:
+    require_cuda(op, t)
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
         raise ValueError(f"{op}: {name} must be a {dtype} tensor of shape {shape} on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t.contiguous()
 
 
 def _opt(t: torch.Tensor | None) -> int | None:
-    return ptr(t) if t is not None else None
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes(name: str, *shape: int) -> int:
+    """Workspace bytes of a shape on B200."""
+
+    value = ctypes.c_int64(0)
+    call(name, *shape, ctypes.byref(value))
+    return value.value
 
 
 def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: int = 128, block_k: int = 128,
@@ -76,11 +95,9 @@ def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: 
     equal inputs give equal lists on any device and in any batch."""
 
     op = "select_key_blocks"
-    dtype = _check_heads(op, q, k, block_q, block_k)
-    require_no_grad(op, q, k)
-    for name, t in (("q", q), ("k", k)):
-        _check_view(name, t)
-    (b, sq, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
+    dtype = check_inputs(op, _TYPES, (q, k))
+    _check_shapes(op, q, k, block_q, block_k)
+    (b, sq, h, d), (_, sk, hk, _) = q.shape, k.shape
     nq, nk = -(-sq // block_q), -(-sk // block_k)
     if isinstance(top_k, bool) or not isinstance(top_k, int) or top_k < 1:
         raise ValueError(f"{op}: top_k must be a positive integer, got {top_k!r}")
@@ -94,13 +111,11 @@ def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: 
     counts = torch.empty((b, h, nq), dtype=torch.int32, device=q.device)
     if counts.numel() == 0:
         return indices, counts
-    need = ctypes.c_int64(0)
-    call("h3b_select_key_blocks_workspace_size", b, sq, sk, h, hk, d, block_q, block_k, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        call("h3b_select_key_blocks", ptr(indices), ptr(counts), ptr(q), ptr(k), b, sq, sk, h, hk, d, block_q,
-             block_k, top_k, q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
-             _opt(q_lens), _opt(k_lens), _opt(keep), dtype, ptr(ws), need.value, stream_of(q))
+    need = _bytes("h3b_select_key_blocks_workspace_size", b, sq, sk, h, hk, d, block_q, block_k)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    call_on(q, "h3b_select_key_blocks", indices.data_ptr(), counts.data_ptr(), q.data_ptr(), k.data_ptr(), b, sq, sk,
+            h, hk, d, block_q, block_k, top_k, *_strides(op, "q", q), *_strides(op, "k", k), _opt(q_lens),
+            _opt(k_lens), _opt(keep), dtype, ws.data_ptr(), need)
     return indices, counts
 
 
@@ -120,51 +135,38 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     the softmax sums."""
 
     op = "block_sparse_attention"
-    dtype = _check_heads(op, q, k, block_q, block_k)
-    require_cuda(op, q, v, indices)
-    dtype_code(op, _TYPES, q, v)
-    require_no_grad(op, q, k, v)
+    dtype = check_inputs(op, _TYPES, (q, k, v) if out is None else (q, k, v, out))
+    _check_shapes(op, q, k, block_q, block_k)
     if v.shape != k.shape:
         raise ValueError(f"{op}: k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
-    (b, sq, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
+    (b, sq, h, d), (_, sk, hk, _) = q.shape, k.shape
     nq = -(-sq // block_q)
-    if indices.dim() != 4:
+    if not isinstance(indices, torch.Tensor) or indices.dim() != 4:
         raise ValueError(f"{op}: indices must be [batch, heads, query blocks, entries]")
     entries = indices.shape[3]
     indices = _side_tensor(op, "indices", indices, torch.int32, (b, h, nq, entries), q.device)
     counts = _side_tensor(op, "counts", counts, torch.int32, (b, h, nq), q.device)
     q_lens = _side_tensor(op, "q_lens", q_lens, torch.int32, (b,), q.device)
     k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_view(name, t)
     if out is None:
         out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
-    else:
-        require_cuda(op, q, out)
-        dtype_code(op, _TYPES, q, out)
-        require_no_grad(op, out)
-        if out.shape != q.shape:
-            raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
-        _check_view("out", out)
+    elif out.shape != q.shape:
+        raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
     lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device) if return_lse else None
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(d)
-    if not (0.0 < scale < math.inf):
+    if not 0.0 < scale < math.inf:
         raise ValueError(f"{op}: softmax_scale must be positive and finite, got {scale}")
-    if out.numel():
-        if sk == 0 or entries == 0:
-            out.zero_()
-            if lse is not None:
-                lse.fill_(-math.inf)
-        else:
-            with torch.cuda.device(q.device):
-                need = ctypes.c_int64(0)
-                call("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, entries, ctypes.byref(need))
-                ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-                call("h3b_block_sparse_attention", ptr(out), _opt(lse), ptr(q), ptr(k), ptr(v), ptr(indices),
-                     _opt(counts), entries, b, sq, sk, h, hk, d, block_q, block_k, q.stride(0), q.stride(1),
-                     q.stride(2), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
-                     out.stride(0), out.stride(1), out.stride(2), _opt(q_lens), _opt(k_lens), scale, dtype,
-                     _opt(ws), need.value, stream_of(q))
+    if out.numel() and (sk == 0 or entries == 0):
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-math.inf)
+    elif out.numel():
+        need = _bytes("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, entries)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        call_on(q, "h3b_block_sparse_attention", out.data_ptr(), _opt(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                indices.data_ptr(), _opt(counts), entries, b, sq, sk, h, hk, d, block_q, block_k,
+                *_strides(op, "q", q), *_strides(op, "k", k), *_strides(op, "v", v), *_strides(op, "out", out),
+                _opt(q_lens), _opt(k_lens), scale, dtype, _opt(ws), need)
     return (out, lse) if return_lse else out
 
 

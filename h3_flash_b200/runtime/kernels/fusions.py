@@ -18,12 +18,12 @@ import torch
 from ... import _lib
 from ..._torch import (
     call,
-    dtype_code,
+    call_on,
+    check_inputs,
     index64,
     ptr,
     require_bf16,
     require_cuda,
-    require_no_grad,
     rows_view,
     stream_of,
     table_rows,
@@ -96,46 +96,69 @@ def fused_residual_gate_rmsnorm_modulate(residual, branch, gate, weight, scale, 
 _FLOAT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _row_stride(t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
+    """The tensor as rows of ``columns`` (copied only if they do not step evenly) and the step."""
+
+    if t.is_contiguous():
+        return t, columns
+    t = rows_view(t)
+    return t, t.stride(0)
+
+
+def _table(op: str, t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int, int]:
+    """An AdaLN table, its row stride and its number of rows."""
+
+    if t.shape[-1] != columns:
+        raise ValueError(f"{op}: tables must be {columns} wide")
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0), t.shape[0]
+    t, stride = table_rows(t)
+    return t, stride, 1 if t.dim() == 1 else t.shape[0]
+
+
 def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps, residual_scale):
     """Checks and launch shared by the sandwich-norm ops; ``pre`` is (weight, scale, shift)
     of the norm before the next branch, or None."""
 
-    tensors = (residual, branch, post_weight, gate, *(pre or ()))
-    require_cuda(op, *tensors)
-    dtype = dtype_code(op, _FLOAT_TYPES, *tensors)
-    require_no_grad(op, *tensors)
-    columns = residual.shape[-1]
-    if branch.shape != residual.shape:
+    code = check_inputs(op, _FLOAT_TYPES, (residual, branch, post_weight, gate, *pre) if pre else
+                        (residual, branch, post_weight, gate))
+    shape = residual.shape
+    if branch.shape != shape:
         raise ValueError(f"{op}: residual and branch must have the same shape")
-    for name, t in (("post_weight", post_weight), *((("weight", pre[0]),) if pre else ())):
-        if t.shape != (columns,):
-            raise ValueError(f"{op}: {name} must have shape ({columns},), got {tuple(t.shape)}")
-    tables = [table_rows(t) for t in (gate, *(pre[1:] if pre else ()))]
-    if any(t.shape[-1] != columns for t, _ in tables):
-        raise ValueError(f"{op}: tables must be {columns} wide")
-    n_table = tables[0][0].numel() // columns if columns else 0
-    if any(t.numel() != tables[0][0].numel() for t, _ in tables):
-        raise ValueError(f"{op}: gate, scale and shift must have the same rows")
-    residual_flat, branch_flat = rows_view(residual), rows_view(branch)
+    columns = shape[-1]
+    if post_weight.shape != (columns,):
+        raise ValueError(f"{op}: post_weight must have shape ({columns},), got {tuple(post_weight.shape)}")
+    gate, gate_stride, n_table = _table(op, gate, columns)
+    weight_ptr = scale_ptr = shift_ptr = normed_ptr = normed = None
+    scale_stride = shift_stride = 0
+    if pre is not None:
+        weight, scale, shift = pre
+        if weight.shape != (columns,):
+            raise ValueError(f"{op}: weight must have shape ({columns},), got {tuple(weight.shape)}")
+        weight = weight.contiguous()
+        scale, scale_stride, n_scale = _table(op, scale, columns)
+        shift, shift_stride, n_shift = _table(op, shift, columns)
+        if n_scale != n_table or n_shift != n_table:
+            raise ValueError(f"{op}: gate, scale and shift must have the same rows")
+        weight_ptr, scale_ptr, shift_ptr = weight.data_ptr(), scale.data_ptr(), shift.data_ptr()
+        normed = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+        normed_ptr = normed.data_ptr()
+    hidden = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+    cells = hidden.numel()
+    if cells == 0:
+        return hidden, normed
     idx = index64(index, residual.device)
-    rows = residual_flat.shape[0]
-    hidden = torch.empty((rows, columns), dtype=residual.dtype, device=residual.device)
-    normed = torch.empty_like(hidden) if pre else None
-    if rows == 0 or columns == 0:
-        return hidden.view(residual.shape), normed.view(residual.shape) if pre else None
-    if idx.numel() == 0 or n_table == 0:
+    n_index = idx.numel()
+    if n_index == 0 or n_table == 0:
         raise ValueError(f"{op}: empty index or table")
+    residual, residual_stride = _row_stride(residual, columns)
+    branch, branch_stride = _row_stride(branch, columns)
     post_weight = post_weight.contiguous()
-    weight = pre[0].contiguous() if pre else None
-    with torch.cuda.device(residual.device):
-        call("h3b_sandwich_residual_rmsnorm_modulate", ptr(hidden), ptr(normed) if pre else None,
-             ptr(residual_flat), ptr(branch_flat), ptr(post_weight), ptr(tables[0][0]),
-             ptr(weight) if pre else None, ptr(tables[1][0]) if pre else None,
-             ptr(tables[2][0]) if pre else None, ptr(idx), rows, columns, idx.numel(), n_table,
-             residual_flat.stride(0), branch_flat.stride(0), columns, tables[0][1],
-             tables[1][1] if pre else 0, tables[2][1] if pre else 0, float(residual_scale),
-             float(post_eps), float(eps), dtype, stream_of(residual))
-    return hidden.view(residual.shape), normed.view(residual.shape) if pre else None
+    call_on(hidden, "h3b_sandwich_residual_rmsnorm_modulate", hidden.data_ptr(), normed_ptr, residual.data_ptr(),
+            branch.data_ptr(), post_weight.data_ptr(), gate.data_ptr(), weight_ptr, scale_ptr, shift_ptr,
+            idx.data_ptr(), cells // columns, columns, n_index, n_table, residual_stride, branch_stride, columns,
+            gate_stride, scale_stride, shift_stride, residual_scale, post_eps, eps, code)
+    return hidden, normed
 
 
 def fused_sandwich_residual_rmsnorm_modulate(residual, branch, post_weight, gate, weight, scale, shift,
