@@ -9,12 +9,13 @@
 // The choice is discrete, so scores are compared where rounding cannot move them: a mean
 // of at most 256 16-bit values is summed in fp64 and the products of two fp32 means are
 // exact in fp64, which leaves 2^-52 relative in a score. Two devices, two batch layouts
-// or another summation order then choose alike.
+// or another summation order then choose alike. Most of it is done in fp32 all the same:
+// only scores too close to the border for fp32 to tell are taken in fp64 (score_select).
 //
 // Two kernels. block_means reads q and k once (bound by HBM: everything else is small);
 // one warp per (block, head), heads of one block in neighbouring warps so that whole rows
-// are read together. score_select holds the scores of a few query blocks in shared memory
-// as order-preserving 64-bit keys and selects with one warp per row.
+// are read together. score_select holds the scores of up to 16 query blocks in shared
+// memory as order-preserving keys and selects with one warp per row.
 #include <cuda_fp16.h>
 
 #include <cstdio>
@@ -124,24 +125,69 @@ struct SelectArgs {
   int row_groups;  // CTAs per (batch, head)
 };
 
-// Order-preserving 64-bit key of a score; 0 is left for blocks that do not compete, the
-// largest value for kept ones that all fit. -0 and +0 are the same score, NaN ranks as -inf.
+// Order-preserving keys of a score. -0 and +0 are the same score, NaN ranks as -inf.
 __device__ __forceinline__ unsigned long long score_key(double s) {
   if (s != s) s = -INFINITY;
   s += 0.0;
   const long long bits = __double_as_longlong(s);
   return bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | (1ull << 63);
 }
-constexpr unsigned long long kKeepKey = ~0ull;
+__device__ __forceinline__ uint32_t score_key(float s) {
+  if (s != s) s = -INFINITY;
+  s += 0.f;
+  const int bits = __float_as_int(s);
+  return bits < 0 ? ~(uint32_t)bits : (uint32_t)bits | (1u << 31);
+}
+__device__ __forceinline__ float key_score(uint32_t key) {
+  return __int_as_float((key >> 31) ? (int)(key & 0x7fffffffu) : (int)~key);
+}
+// Besides scores: 0 for blocks that are out, kInKey for blocks that are in.
+constexpr uint32_t kInKey = 0xffffffffu;
 
-constexpr int kSelectThreads = 256;
+// Highest key t such that at least `want` of the warp's keys are >= t, and how many exceed
+// it: bit by bit from the first bit in which keys differ. count(key, mask) gives the number
+// of keys that equal `key` in the bits of `mask`.
+template <class Key, class Count>
+__device__ __forceinline__ Key kth_key(Key common, int bit, int n_keys, int want, int& above,
+                                       Key& decided, Count count) {
+  Key prefix = common;
+  int equal = n_keys;
+  above = 0;
+  for (; bit >= 0 && above + equal > want; --bit) {
+    const Key probe = prefix | ((Key)1 << bit);
+    const int n = count(probe, ~(((Key)1 << bit) - 1));
+    if (above + n >= want) {
+      prefix = probe;
+      equal = n;
+    } else {
+      above += n;
+      equal -= n;
+    }
+  }
+  decided = bit < 0 ? ~(Key)0 : ~((((Key)1 << bit) << 1) - 1);  // bits of prefix above `bit`
+  return prefix;
+}
 
-// ROWS query blocks of one (batch, head) per CTA.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(kSelectThreads) score_select(SelectArgs a) {
+struct SelectShape {
+  static constexpr int kThreads = ROWS == 1 ? 512 : 256;
+  static constexpr int kCols = ROWS == 1 ? 1 : 2;  // columns per thread
+  static constexpr int kWarps = kThreads / 32;
+};
+
+// ROWS query blocks of one (batch, head) per CTA. Scores are first taken in fp32, whose
+// rounding leaves at most E = D 2^-24 |q| max|k| (Cauchy-Schwarz). An order statistic moves
+// by no more than the values do, so with T the k-th largest fp32 score, blocks above T + 2E
+// are in and blocks below T - 2E are out whatever the rounding did; the few between are
+// scored again in fp64 and ranked. A bound that is not finite makes every block one of those.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(SelectArgs a) {
+  using S = SelectShape<D, ROWS>;
   extern __shared__ __align__(16) unsigned char smem[];
-  double* q_tile = reinterpret_cast<double*>(smem);  // [D][ROWS]
-  auto* keys = reinterpret_cast<unsigned long long*>(smem + sizeof(double) * D * ROWS);  // [ROWS][nk]
+  float* q_tile = reinterpret_cast<float*>(smem);                 // [D][ROWS]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(q_tile + D * ROWS);  // [ROWS][pitch]
+  __shared__ unsigned int k_square;                               // bits of max |k|^2
+  __shared__ int close[S::kWarps][32];                            // columns to score again
   const int group = blockIdx.x % a.row_groups;
   const int64_t bh = blockIdx.x / a.row_groups;
   const int head = (int)(bh % a.heads);
@@ -151,82 +197,215 @@ __global__ void __launch_bounds__(kSelectThreads) score_select(SelectArgs a) {
   const int k_rows = rows_of(a.k_lens, b, a.seq_k);
   const int k_blocks = (k_rows + a.block_k - 1) / a.block_k;  // blocks that exist
 
-  for (int i = threadIdx.x; i < D * ROWS; i += kSelectThreads) {
+  if (threadIdx.x == 0) k_square = 0u;
+  for (int i = threadIdx.x; i < D * ROWS; i += S::kThreads) {
     const int r = i / D, d = i % D;
-    q_tile[d * ROWS + r] = row0 + r < a.nq ? (double)a.q_mean[(bh * a.nq + row0 + r) * D + d] : 0.0;
+    q_tile[d * ROWS + r] = row0 + r < a.nq ? a.q_mean[(bh * a.nq + row0 + r) * D + d] : 0.f;
   }
   // More kept blocks than a list holds: only they compete, by score.
   int kept_count = 0;
   if (a.keep != nullptr)
-    for (int c = threadIdx.x; c < (k_blocks + kSelectThreads - 1) / kSelectThreads * kSelectThreads;
-         c += kSelectThreads)
+    for (int c = threadIdx.x; c < (k_blocks + S::kThreads - 1) / S::kThreads * S::kThreads;
+         c += S::kThreads)
       kept_count += __syncthreads_count(c < k_blocks && a.keep[c] != 0);
   const bool only_kept = kept_count > a.top_k;
+  if (only_kept) kept_count = 0;
   __syncthreads();
   const float* km = a.k_mean +
                     ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * D * a.pitch;
-  for (int col = threadIdx.x; col < a.nk; col += kSelectThreads) {
-    double acc[ROWS] = {};
+  for (int col = threadIdx.x * S::kCols; col < k_blocks; col += S::kThreads * S::kCols) {
+    if constexpr (S::kCols == 2) {
+      // Columns col, col + 1 (the pitch is even; a column behind the last is scored and ignored).
+      float2 acc[ROWS] = {}, square = make_float2(0.f, 0.f);
 #pragma unroll 8
-    for (int d = 0; d < D; ++d) {
-      const double kd = (double)km[(int64_t)d * a.pitch + col];
+      for (int d = 0; d < D; ++d) {
+        const float2 k2 = __ldg(reinterpret_cast<const float2*>(km + (int64_t)d * a.pitch + col));
+        square = __ffma2_rn(k2, k2, square);
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) acc[r] = fma(q_tile[d * ROWS + r], kd, acc[r]);
+        for (int r = 0; r < ROWS; ++r) {
+          const float q = q_tile[d * ROWS + r];
+          acc[r] = __ffma2_rn(make_float2(q, q), k2, acc[r]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = col + i;
+        if (c >= k_blocks) continue;
+        const bool kept = a.keep != nullptr && a.keep[c] != 0;
+        if (kept || !only_kept) atomicMax(&k_square, __float_as_uint(i == 0 ? square.x : square.y));
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+          keys[r * a.pitch + c] = only_kept && !kept ? 0u
+                                  : kept && !only_kept ? kInKey
+                                                       : score_key(i == 0 ? acc[r].x : acc[r].y);
+      }
+    } else {
+      float acc[ROWS] = {}, square = 0.f;
+#pragma unroll 32
+      for (int d = 0; d < D; ++d) {
+        const float k1 = __ldg(km + (int64_t)d * a.pitch + col);
+        square = fmaf(k1, k1, square);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r] = fmaf(q_tile[d * ROWS + r], k1, acc[r]);
+      }
+      const bool kept = a.keep != nullptr && a.keep[col] != 0;
+      if (kept || !only_kept) atomicMax(&k_square, __float_as_uint(square));
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        keys[r * a.pitch + col] = only_kept && !kept ? 0u
+                                  : kept && !only_kept ? kInKey : score_key(acc[r]);
     }
-    const bool kept = a.keep != nullptr && a.keep[col] != 0;
-    const bool competes = col < k_blocks && (kept || !only_kept);
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      keys[(int64_t)r * a.nk + col] =
-          !competes ? 0ull : (kept && !only_kept ? kKeepKey : score_key(acc[r]));
   }
   __syncthreads();
 
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < ROWS; r += kSelectThreads / 32) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned below = (1u << lane) - 1u;
+  for (int r = warp; r < ROWS; r += S::kWarps) {
     if (row0 + r >= a.nq) break;
-    const unsigned long long* row = keys + (int64_t)r * a.nk;
+    uint32_t* row = keys + r * a.pitch;
     const int64_t list = bh * a.nq + row0 + r;
     int32_t* out = a.indices + list * a.top_k;
     const bool exists = (row0 + r) * a.block_q < q_rows;
     const int want = exists ? min(a.top_k, k_blocks) : 0;
-    int done = 0;
-    if (want > 0) {
-      // Largest threshold t with at least `want` keys >= t, found bit by bit from the top:
-      // `prefix` holds the bits decided, `above` the keys whose decided bits are larger.
-      unsigned long long prefix = 0;
-      int above = 0, equal = a.nk;
-      int bit = 63;
-      for (; bit >= 0 && above + equal > want; --bit) {
-        const unsigned long long probe = prefix | (1ull << bit);
-        int n = 0;
-        for (int c = lane; c < a.nk; c += 32) n += (row[c] >> bit) == (probe >> bit);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (above + n >= want) {
-          prefix = probe;
-          equal = n;
-        } else {
-          above += n;
-          equal -= n;
+    // Calls f(column) for every lane's columns, warp-uniformly: a column >= k_blocks has no key.
+    auto each = [&](auto f) {
+      for (int c = lane; c < k_blocks; c += 32) f(c);
+    };
+    uint32_t least_in = kInKey;  // keys from here on are in
+    if (want > kept_count) {
+      // Scores that compete differ from bit `bit` down.
+      uint32_t ones = 0, zeros = 0;
+      int n_keys = 0;
+      each([&](int c) {
+        const uint32_t k = row[c];
+        if (k != 0u && k != kInKey) {
+          ones |= k;
+          zeros |= ~k;
+          ++n_keys;
         }
-      }
-      // Keys above the decided prefix, then the lowest-index ones that equal it.
-      const int shift = bit + 1;
-      int ties = want - above;
-      for (int c0 = 0; c0 < a.nk && done < want; c0 += 32) {
+      });
+      ones = __reduce_or_sync(0xffffffffu, ones);
+      zeros = __reduce_or_sync(0xffffffffu, zeros);
+      n_keys = __reduce_add_sync(0xffffffffu, n_keys);
+      const uint32_t differ = ones & zeros;
+      const int bit = 31 - __clz((int)differ);  // -1: all equal
+      const uint32_t same = bit >= 31 ? 0u : ~((2u << bit) - 1u);
+      int above;
+      uint32_t decided;
+      const uint32_t prefix = kth_key<uint32_t>(
+          ones & (bit < 0 ? ~0u : same), bit, n_keys, want - kept_count, above, decided,
+          [&](uint32_t key, uint32_t mask) {
+            int n = 0;
+            each([&](int c) {
+              const uint32_t k = row[c];
+              n += k != kInKey && k != 0u && (k & mask) == key;
+            });
+            return (int)__reduce_add_sync(0xffffffffu, n);
+          });
+      // T: the least key among those from `prefix` up.
+      uint32_t kth = kInKey;
+      each([&](int c) {
+        const uint32_t k = row[c];
+        if (k != 0u && (k & decided) >= prefix) kth = min(kth, k);
+      });
+      kth = __reduce_min_sync(0xffffffffu, kth);
+      float q_square = 0.f;
+      for (int d = lane; d < D; d += 32) q_square += q_tile[d * ROWS + r] * q_tile[d * ROWS + r];
+      q_square = warp_sum(q_square);
+      // 2E, rounded up: D 2^-23 sqrt(|q|^2 |k|^2), 1% for the rounding of the norms, and the
+      // underflow of D products.
+      const float twice = 1.01f * D * 1.1920929e-7f * sqrtf(q_square) *
+                              sqrtf(__uint_as_float(k_square)) + 1.2e-38f;
+      const float t = key_score(kth);
+      const bool bounded = twice < INFINITY && fabsf(t) < INFINITY;
+      const uint32_t hi = bounded ? score_key(__fadd_ru(t, twice)) : kInKey - 1u;
+      const uint32_t lo = bounded ? score_key(__fadd_rd(t, -twice)) : 1u;
+      int n_in = 0, n_close = 0;
+      for (int c0 = 0; c0 < k_blocks; c0 += 32) {
         const int c = c0 + lane;
-        const unsigned long long key = c < a.nk ? row[c] : 0ull;
-        const unsigned long long top = shift < 64 ? key >> shift : 0ull;
-        const unsigned long long ref = shift < 64 ? prefix >> shift : 0ull;
-        const bool tie = c < a.nk && top == ref;
-        const unsigned tie_mask = __ballot_sync(0xffffffffu, tie);
-        const bool take = (c < a.nk && top > ref) ||
-                          (tie && __popc(tie_mask & ((1u << lane) - 1u)) < ties);
-        const unsigned mask = __ballot_sync(0xffffffffu, take);
-        if (take) out[done + __popc(mask & ((1u << lane) - 1u))] = c;
-        done += __popc(mask);
-        ties -= min(ties, __popc(tie_mask));
+        const uint32_t k = c < k_blocks ? row[c] : 0u;
+        const bool is_close = k >= lo && k <= hi;
+        const unsigned mask = __ballot_sync(0xffffffffu, is_close);
+        if (is_close) {
+          const int at = n_close + __popc(mask & below);
+          if (at < 32) close[warp][at] = c;
+        }
+        n_close += __popc(mask);
+        n_in += __popc(__ballot_sync(0xffffffffu, k > hi));
       }
+      __syncwarp();
+      const int open = want - n_in;  // places left for the close ones
+      least_in = hi == kInKey ? kInKey : hi + 1u;
+      if (n_close == open) {
+        least_in = lo;
+      } else {
+        // fp64 score of a column, the same sum in every lane.
+        auto score = [&](int c) -> unsigned long long {
+          double s = 0.0;
+          for (int d = lane; d < D; d += 32)
+            s = fma((double)q_tile[d * ROWS + r], (double)km[(int64_t)d * a.pitch + c], s);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          return score_key(s);
+        };
+        if (n_close <= 32) {
+          unsigned long long mine = 0ull;
+          for (int i = 0; i < n_close; ++i) {
+            const unsigned long long s = score(close[warp][i]);
+            if (i == lane) mine = s;
+          }
+          int rank = 0;  // close[] ascends: of equal scores the lower lane goes first
+          for (int i = 0; i < n_close; ++i) {
+            const unsigned long long s = __shfl_sync(0xffffffffu, mine, i);
+            rank += s > mine || (s == mine && i < lane);
+          }
+          if (lane < n_close) row[close[warp][lane]] = rank < open ? kInKey : 0u;
+        } else {
+          // Many scores within the bound (equal blocks, say): the same search on fp64 keys,
+          // which are computed again in every pass.
+          auto each_close = [&](auto f) {
+            for (int c0 = 0; c0 < k_blocks; c0 += 32) {
+              const uint32_t k = c0 + lane < k_blocks ? row[c0 + lane] : 0u;
+              unsigned mask = __ballot_sync(0xffffffffu, k >= lo && k <= hi);
+              for (; mask != 0u; mask &= mask - 1u) {
+                const int c = c0 + __ffs((int)mask) - 1;
+                f(c, score(c));
+              }
+            }
+          };
+          unsigned long long one = 0ull, zero = 0ull;
+          each_close([&](int, unsigned long long s) {
+            one |= s;
+            zero |= ~s;
+          });
+          const int top = 63 - __clzll((long long)(one & zero));  // -1: all equal
+          const unsigned long long same64 = top >= 63 ? 0ull : ~((2ull << top) - 1ull);
+          int above64;
+          unsigned long long decided64;
+          const unsigned long long prefix64 = kth_key<unsigned long long>(
+              one & (top < 0 ? ~0ull : same64), top, n_close, open, above64, decided64,
+              [&](unsigned long long key, unsigned long long mask) {
+                int n = 0;
+                each_close([&](int, unsigned long long s) { n += (s & mask) == key; });
+                return n;
+              });
+          int ties = open - above64;
+          each_close([&](int c, unsigned long long s) {
+            const unsigned long long high = s & decided64;
+            const bool in = high > prefix64 || (high == prefix64 && ties-- > 0);
+            if (lane == (c & 31)) row[c] = in ? kInKey : 0u;
+          });
+        }
+        __syncwarp();
+      }
+    }
+    int done = 0;
+    for (int c0 = 0; c0 < k_blocks && done < want; c0 += 32) {
+      const int c = c0 + lane;
+      const bool take = c < k_blocks && row[c] >= least_in;
+      const unsigned mask = __ballot_sync(0xffffffffu, take);
+      if (take) out[done + __popc(mask & below)] = c;
+      done += __popc(mask);
     }
     for (int c = done + lane; c < a.top_k; c += 32) out[c] = -1;
     if (lane == 0) a.counts[list] = done;
@@ -235,8 +414,8 @@ __global__ void __launch_bounds__(kSelectThreads) score_select(SelectArgs a) {
 
 constexpr int kMaxKeyBlocks = 24576;  // scores of one query block fit in shared memory
 
-size_t select_smem(int head_dim, int rows, int64_t nk) {
-  return sizeof(double) * (size_t)head_dim * rows + 8 * (size_t)nk * rows;
+size_t select_smem(int head_dim, int rows, int64_t pitch) {
+  return 4 * (size_t)rows * (head_dim + pitch);
 }
 
 template <int D, int ROWS>
@@ -245,7 +424,7 @@ int launch_select(const SelectArgs& a, int64_t batch, size_t smem, cudaStream_t 
   cudaError_t e = cudaErrorInvalidDevice;
   if (context_cached(slots, [&]() -> void* {
         e = cudaFuncSetAttribute(score_select<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 227 * 1024);
+                                 220 * 1024);
         return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
       }) == nullptr) {
     set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
@@ -254,7 +433,7 @@ int launch_select(const SelectArgs& a, int64_t batch, size_t smem, cudaStream_t 
   }
   const int64_t grid = batch * a.heads * a.row_groups;
   H3B_REQUIRE(grid <= 0x7fffffffLL, "select_key_blocks: shape exceeds launch limits");
-  score_select<D, ROWS><<<(unsigned)grid, kSelectThreads, smem, s>>>(a);
+  score_select<D, ROWS><<<(unsigned)grid, SelectShape<D, ROWS>::kThreads, smem, s>>>(a);
   return check_launch("h3b_select_key_blocks");
 }
 
@@ -268,9 +447,9 @@ int launch_all(const MeanArgs& m, SelectArgs a, int64_t batch, cudaStream_t s) {
   // Query blocks per CTA: as many as there are and as shared memory holds; each reads the
   // key means once.
   int rows = 16;
-  while (rows > 1 && (rows / 2 >= a.nq || select_smem(D, rows, a.nk) > 200 * 1024)) rows /= 4;
+  while (rows > 1 && (rows / 2 >= a.nq || select_smem(D, rows, a.pitch) > 200 * 1024)) rows /= 4;
   a.row_groups = (a.nq + rows - 1) / rows;
-  const size_t smem = select_smem(D, rows, a.nk);
+  const size_t smem = select_smem(D, rows, a.pitch);
   if (rows == 16) return launch_select<D, 16>(a, batch, smem, s);
   if (rows == 4) return launch_select<D, 4>(a, batch, smem, s);
   return launch_select<D, 1>(a, batch, smem, s);
