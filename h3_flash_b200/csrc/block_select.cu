@@ -144,18 +144,19 @@ __device__ __forceinline__ float key_score(uint32_t key) {
 // Besides scores: 0 for blocks that are out, kInKey for blocks that are in.
 constexpr uint32_t kInKey = 0xffffffffu;
 
-// Highest key t such that at least `want` of the warp's keys are >= t, and how many exceed
+// Highest fp64 key t such that at least `want` of n_keys keys are >= t, and how many exceed
 // it: bit by bit from the first bit in which keys differ. count(key, mask) gives the number
 // of keys that equal `key` in the bits of `mask`.
-template <class Key, class Count>
-__device__ __forceinline__ Key kth_key(Key common, int bit, int n_keys, int want, int& above,
-                                       Key& decided, Count count) {
-  Key prefix = common;
+template <class Count>
+__device__ __forceinline__ unsigned long long kth_key(unsigned long long common, int bit,
+                                                      int n_keys, int want, int& above,
+                                                      unsigned long long& decided, Count count) {
+  unsigned long long prefix = common;
   int equal = n_keys;
   above = 0;
   for (; bit >= 0 && above + equal > want; --bit) {
-    const Key probe = prefix | ((Key)1 << bit);
-    const int n = count(probe, ~(((Key)1 << bit) - 1));
+    const unsigned long long probe = prefix | (1ull << bit);
+    const int n = count(probe, ~((1ull << bit) - 1ull));
     if (above + n >= want) {
       prefix = probe;
       equal = n;
@@ -164,7 +165,7 @@ __device__ __forceinline__ Key kth_key(Key common, int bit, int n_keys, int want
       equal -= n;
     }
   }
-  decided = bit < 0 ? ~(Key)0 : ~((((Key)1 << bit) << 1) - 1);  // bits of prefix above `bit`
+  decided = bit < 0 ? ~0ull : ~(((1ull << bit) << 1) - 1ull);  // bits of prefix above `bit`
   return prefix;
 }
 
@@ -173,7 +174,10 @@ struct SelectShape {
   static constexpr int kThreads = ROWS == 1 ? 512 : 256;
   static constexpr int kCols = ROWS == 1 ? 1 : 2;  // columns per thread
   static constexpr int kWarps = kThreads / 32;
+  // CTAs per SM that registers should allow: three of 16 rows fit in shared memory at 800 columns.
+  static constexpr int kCtas = ROWS == 1 ? 2 : 3;
 };
+constexpr int kBins = 256;
 
 // ROWS query blocks of one (batch, head) per CTA. Scores are first taken in fp32, whose
 // rounding leaves at most E = D 2^-24 |q| max|k| (Cauchy-Schwarz). An order statistic moves
@@ -181,13 +185,15 @@ struct SelectShape {
 // are in and blocks below T - 2E are out whatever the rounding did; the few between are
 // scored again in fp64 and ranked. A bound that is not finite makes every block one of those.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(SelectArgs a) {
+__global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads, SelectShape<D, ROWS>::kCtas)
+    score_select(SelectArgs a) {
   using S = SelectShape<D, ROWS>;
   extern __shared__ __align__(16) unsigned char smem[];
   float* q_tile = reinterpret_cast<float*>(smem);                 // [D][ROWS]
   uint32_t* keys = reinterpret_cast<uint32_t*>(q_tile + D * ROWS);  // [ROWS][pitch]
   __shared__ unsigned int k_square;                               // bits of max |k|^2
   __shared__ int close[S::kWarps][32];                            // columns to score again
+  __shared__ uint32_t bins[S::kWarps][kBins];
   const int group = blockIdx.x % a.row_groups;
   const int64_t bh = blockIdx.x / a.row_groups;
   const int head = (int)(bh % a.heads);
@@ -215,16 +221,21 @@ __global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(S
                     ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * D * a.pitch;
   for (int col = threadIdx.x * S::kCols; col < k_blocks; col += S::kThreads * S::kCols) {
     if constexpr (S::kCols == 2) {
-      // Columns col, col + 1 (the pitch is even; a column behind the last is scored and ignored).
-      float2 acc[ROWS] = {}, square = make_float2(0.f, 0.f);
+      // Columns col, col + 1 (the pitch is even; a column behind the last is scored and
+      // ignored), rows in pairs: a pair of q comes as it lies in shared memory.
+      float2 acc[ROWS / 2][2] = {}, square = make_float2(0.f, 0.f);
 #pragma unroll 8
       for (int d = 0; d < D; ++d) {
         const float2 k2 = __ldg(reinterpret_cast<const float2*>(km + (int64_t)d * a.pitch + col));
         square = __ffma2_rn(k2, k2, square);
+        const float2 first = make_float2(k2.x, k2.x), second = make_float2(k2.y, k2.y);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-          const float q = q_tile[d * ROWS + r];
-          acc[r] = __ffma2_rn(make_float2(q, q), k2, acc[r]);
+        for (int r = 0; r < ROWS / 2; r += 2) {
+          const float4 q = *reinterpret_cast<const float4*>(q_tile + d * ROWS + 2 * r);
+          acc[r][0] = __ffma2_rn(make_float2(q.x, q.y), first, acc[r][0]);
+          acc[r][1] = __ffma2_rn(make_float2(q.x, q.y), second, acc[r][1]);
+          acc[r + 1][0] = __ffma2_rn(make_float2(q.z, q.w), first, acc[r + 1][0]);
+          acc[r + 1][1] = __ffma2_rn(make_float2(q.z, q.w), second, acc[r + 1][1]);
         }
       }
 #pragma unroll
@@ -235,9 +246,10 @@ __global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(S
         if (kept || !only_kept) atomicMax(&k_square, __float_as_uint(i == 0 ? square.x : square.y));
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
-          keys[r * a.pitch + c] = only_kept && !kept ? 0u
-                                  : kept && !only_kept ? kInKey
-                                                       : score_key(i == 0 ? acc[r].x : acc[r].y);
+          keys[r * a.pitch + c] =
+              only_kept && !kept ? 0u
+              : kept && !only_kept ? kInKey
+                                   : score_key(r % 2 == 0 ? acc[r / 2][i].x : acc[r / 2][i].y);
       }
     } else {
       float acc[ROWS] = {}, square = 0.f;
@@ -273,42 +285,116 @@ __global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(S
     };
     uint32_t least_in = kInKey;  // keys from here on are in
     if (want > kept_count) {
-      // Scores that compete differ from bit `bit` down.
-      uint32_t ones = 0, zeros = 0;
-      int n_keys = 0;
-      each([&](int c) {
-        const uint32_t k = row[c];
-        if (k != 0u && k != kInKey) {
-          ones |= k;
-          zeros |= ~k;
-          ++n_keys;
+      // T, the k-th largest score: count the scores in equal bins of their range, go on
+      // inside the bin that holds the k-th, rank what is left when a warp holds it. The bin
+      // of a score never decreases with it, whatever the rounding.
+      float low = -INFINITY, high = INFINITY;
+      int left = want - kept_count;  // the rank of T among the scores in [low, high]
+      uint32_t kth;
+      for (;;) {
+        uint32_t least = kInKey, most = 0u;
+        int n = 0;
+        const uint32_t low_key = score_key(low), high_key = score_key(high);
+        each([&](int c) {
+          const uint32_t k = row[c];
+          if (k >= low_key && k <= high_key) {
+            least = min(least, k);
+            most = max(most, k);
+            ++n;
+          }
+        });
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (least == most || left == n) {
+          kth = least;
+          break;
         }
-      });
-      ones = __reduce_or_sync(0xffffffffu, ones);
-      zeros = __reduce_or_sync(0xffffffffu, zeros);
-      n_keys = __reduce_add_sync(0xffffffffu, n_keys);
-      const uint32_t differ = ones & zeros;
-      const int bit = 31 - __clz((int)differ);  // -1: all equal
-      const uint32_t same = bit >= 31 ? 0u : ~((2u << bit) - 1u);
-      int above;
-      uint32_t decided;
-      const uint32_t prefix = kth_key<uint32_t>(
-          ones & (bit < 0 ? ~0u : same), bit, n_keys, want - kept_count, above, decided,
-          [&](uint32_t key, uint32_t mask) {
-            int n = 0;
-            each([&](int c) {
-              const uint32_t k = row[c];
-              n += k != kInKey && k != 0u && (k & mask) == key;
-            });
-            return (int)__reduce_add_sync(0xffffffffu, n);
-          });
-      // T: the least key among those from `prefix` up.
-      uint32_t kth = kInKey;
-      each([&](int c) {
-        const uint32_t k = row[c];
-        if (k != 0u && (k & decided) >= prefix) kth = min(kth, k);
-      });
-      kth = __reduce_min_sync(0xffffffffu, kth);
+        if (left == 1) {
+          kth = most;
+          break;
+        }
+        if (n <= 32) {
+          int at = 0;
+          for (int c0 = 0; c0 < k_blocks; c0 += 32) {
+            const uint32_t k = c0 + lane < k_blocks ? row[c0 + lane] : 0u;
+            const bool mine = k >= least && k <= most;
+            const unsigned mask = __ballot_sync(0xffffffffu, mine);
+            if (mine) bins[warp][at + __popc(mask & below)] = k;
+            at += __popc(mask);
+          }
+          __syncwarp();
+          const uint32_t mine = lane < n ? bins[warp][lane] : 0u;
+          int rank = 0;
+          for (int i = 0; i < n; ++i) {
+            const uint32_t k = __shfl_sync(0xffffffffu, mine, i);
+            rank += k > mine || (k == mine && i < lane);
+          }
+          const unsigned found = __ballot_sync(0xffffffffu, lane < n && rank == left - 1);
+          kth = __shfl_sync(0xffffffffu, mine, __ffs((int)found) - 1);
+          __syncwarp();
+          break;
+        }
+        low = key_score(least);
+        high = key_score(most);
+        const float span = high - low;
+        const float scale = (float)kBins / span;
+        // A range too wide or too narrow for fp32: every block is scored again in fp64.
+        if (!(span < INFINITY) || !(scale < INFINITY)) {
+          kth = 0u;
+          break;
+        }
+        auto bin_of = [&](uint32_t k) { return min((int)((key_score(k) - low) * scale), kBins - 1); };
+        for (int i = lane; i < kBins; i += 32) bins[warp][i] = 0u;
+        __syncwarp();
+        each([&](int c) {
+          const uint32_t k = row[c];
+          if (k >= least && k <= most) atomicAdd(&bins[warp][bin_of(k)], 1u);
+        });
+        __syncwarp();
+        // Lane l sums bins [8l, 8l + 8); from the top, the lane and then the bin that reach `left`.
+        uint32_t mine[kBins / 32];
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < kBins / 32; ++i) {
+          mine[i] = bins[warp][lane * (kBins / 32) + i];
+          sum += (int)mine[i];
+        }
+        int up = sum;  // scores in this lane's bins and above
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int other = __shfl_down_sync(0xffffffffu, up, o);
+          if (lane + o < 32) up += other;
+        }
+        const unsigned reach = __ballot_sync(0xffffffffu, up >= left);
+        const int owner = 31 - __clz((int)reach);
+        int bin = 0, over = up - sum;
+        if (lane == owner) {
+          bool done = false;
+#pragma unroll
+          for (int i = kBins / 32 - 1; i >= 0; --i) {
+            if (!done && over + (int)mine[i] >= left) {
+              bin = lane * (kBins / 32) + i;
+              done = true;
+            }
+            if (!done) over += (int)mine[i];
+          }
+        }
+        bin = __shfl_sync(0xffffffffu, bin, owner);
+        left -= __shfl_sync(0xffffffffu, over, owner);
+        // The bin's own range.
+        uint32_t bin_least = kInKey, bin_most = 0u;
+        each([&](int c) {
+          const uint32_t k = row[c];
+          if (k >= least && k <= most && bin_of(k) == bin) {
+            bin_least = min(bin_least, k);
+            bin_most = max(bin_most, k);
+          }
+        });
+        low = key_score(__reduce_min_sync(0xffffffffu, bin_least));
+        high = key_score(__reduce_max_sync(0xffffffffu, bin_most));
+        __syncwarp();
+      }
       float q_square = 0.f;
       for (int d = lane; d < D; d += 32) q_square += q_tile[d * ROWS + r] * q_tile[d * ROWS + r];
       q_square = warp_sum(q_square);
@@ -317,7 +403,7 @@ __global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(S
       const float twice = 1.01f * D * 1.1920929e-7f * sqrtf(q_square) *
                               sqrtf(__uint_as_float(k_square)) + 1.2e-38f;
       const float t = key_score(kth);
-      const bool bounded = twice < INFINITY && fabsf(t) < INFINITY;
+      const bool bounded = kth != 0u && twice < INFINITY && fabsf(t) < INFINITY;
       const uint32_t hi = bounded ? score_key(__fadd_ru(t, twice)) : kInKey - 1u;
       const uint32_t lo = bounded ? score_key(__fadd_rd(t, -twice)) : 1u;
       int n_in = 0, n_close = 0;
@@ -382,7 +468,7 @@ __global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads) score_select(S
           const unsigned long long same64 = top >= 63 ? 0ull : ~((2ull << top) - 1ull);
           int above64;
           unsigned long long decided64;
-          const unsigned long long prefix64 = kth_key<unsigned long long>(
+          const unsigned long long prefix64 = kth_key(
               one & (top < 0 ? ~0ull : same64), top, n_close, open, above64, decided64,
               [&](unsigned long long key, unsigned long long mask) {
                 int n = 0;
@@ -424,7 +510,7 @@ int launch_select(const SelectArgs& a, int64_t batch, size_t smem, cudaStream_t 
   cudaError_t e = cudaErrorInvalidDevice;
   if (context_cached(slots, [&]() -> void* {
         e = cudaFuncSetAttribute(score_select<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 220 * 1024);
+                                 200 * 1024);
         return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
       }) == nullptr) {
     set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
