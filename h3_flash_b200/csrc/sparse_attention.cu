@@ -5,28 +5,33 @@
 //   out[r] = sum_{j in list} sum_{c in block j} p_rc v_c / sum p_rc,
 //   p_rc = 2^(scale log2(e) q_r . k_c - m_r),   lse[r] = ln(2) (m_r + log2(sum p_rc))
 //
-// A step is 128 keys: one listed block of 128, or two of 64, each fetched by its own TMA
-// load from wherever its list entry points. A work item is a pair of neighbouring 128-row
-// query tiles of one (batch, head), or a range of steps of such a pair. CTAs are
-// persistent: item i runs on CTA i mod gridDim, and the loads of an item start while the
-// one before it ends.
+// The unit of work along a list is 64 keys: a listed block of 64, or half of one of 128. A
+// work item is a pair of neighbouring 128-row query tiles of one (batch, head), or a range
+// of units of such a pair. CTAs are persistent: item i runs on CTA i mod gridDim, and the
+// loads of an item start while the one before it ends.
 //
-//   warp 8      loads: the Q tiles of the item, then K and V tiles in the order the MMAs
-//               read them, into a ring of slots that hold one K or one V tile each. Where
-//               both tiles of the pair are at the same list entry the slot is filled once
-//               and read by both ("shared"); the list decides, so no entry needs sorting.
-//   warp 9      MMA issuer, one elected lane: S_t = Q_t K^T, O_t += P_t V, tiles t = 0, 1
-//               in turn, so that the tensor core works on one while the other's softmax runs.
+//   warp 8      loads: the Q tiles of the item, then a ring of slots. Slot u of a tile holds
+//               V of unit u and K of unit u + 2, which the MMA warp reads one after the
+//               other (a first slot holds K of units 0 and 1). Where both tiles of the pair
+//               are at the same entries the slot is filled once and read by both ("shared");
+//               the lists decide, so no entry needs sorting.
+//   warp 9      MMA issuer, one elected lane, tiles t = 0, 1 in turn: O_t += P_t(u) V(u), then
+//               S_t(u + 2) = Q_t K(u + 2)^T into the TMEM columns P_t(u) came from.
 //   warps 0-3   softmax of tile 0, warps 4-7 of tile 1, a thread per row: scores from TMEM,
 //               row max, p, row sum; P goes back over the S columns; O is rescaled in TMEM
 //               only when the running max grew by more than 2^8. P is rounded to the type
 //               of V (the MMA's operand type); sums, max and O stay fp32.
 //
-// TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512).
+// Why 64 keys: scores of a tile are double-buffered, two units of 64 fp32 columns beside
+// O, so the softmax of unit u + 1 has its scores while P V of unit u and the scores of u + 2
+// are computed; with units of 128 keys TMEM holds one buffer, and each tile's softmax and
+// MMAs wait for one another. The price is that an N = 64 score MMA reads its Q operand from
+// shared memory for half as many columns.
 //
-// What does not exist is never read into a result: list entries outside the sequence and
-// the upper half of an odd last step load zeros (a TMA box behind the end of the tensor),
-// and their scores are replaced by -inf. Keys behind k_lens inside a block may hold NaN:
+// TMEM (512 columns): S of tile t, buffer b at 128 t + 64 b; O of tile t at 256 + 128 t.
+//
+// What does not exist is never read into a result: list entries outside the sequence load
+// zeros (a TMA box behind the end of the tensor), and their scores are replaced by -inf. Keys behind k_lens inside a block may hold NaN:
 // their scores are replaced, and their V rows are overwritten with zeros in shared memory
 // before the tensor core sees them (0 * NaN is NaN).
 //
@@ -47,15 +52,17 @@ namespace h3b {
 namespace attn {
 namespace sparse {
 
-constexpr int kTile = 128;  // query rows per tile and keys per step
+constexpr int kTile = 128;  // query rows per tile
+constexpr int kUnit = 64;   // keys per unit
 constexpr int kTiles = 2;
 constexpr int kSoftmaxWarps = 4 * kTiles;
 constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
 constexpr int kLoadWarp = kSoftmaxWarps;
 constexpr int kMmaWarp = kSoftmaxWarps + 1;
-constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 columns, 128-byte swizzle
+constexpr uint32_t kQHalf = kTile * 128;   // 128 rows x 64 columns, 128-byte swizzle
+constexpr uint32_t kKvHalf = kUnit * 128;  // 64 rows x 64 columns
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kTmemS = 0;    // + t*128
+constexpr uint32_t kTmemS = 0;    // + t*128 + buffer*64
 constexpr uint32_t kTmemO = 256;  // + t*128
 // Rescale O only when the running row max (log2 units) grew by more than this; P then
 // stays within 2^8, exact in the fp32 accumulator and inside fp16's range.
@@ -64,14 +71,16 @@ constexpr float kRescaleThreshold = 8.0f;
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;
-  static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
+  static constexpr uint32_t kQBytes = kHalves * kQHalf;
+  static constexpr uint32_t kPartBytes = kHalves * kKvHalf;  // K or V rows of a unit
+  static constexpr uint32_t kSlotBytes = 2 * kPartBytes;
   // Slots: what fits beside the two Q tiles (five of 32 KB at D = 128).
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr uint32_t kSmemQ = 0;
-  static constexpr uint32_t kSmemRing = kTiles * kTileBytes;
-  static constexpr uint32_t kSmemBar = kSmemRing + kSlots * kTileBytes;
-  // qfull[2] qempty[2] full[slots] empty[slots] s[2] p[2][2] o[2] fix
-  static constexpr int kNumBars = 2 * kTiles + 2 * kSlots + 4 * kTiles + 1;
+  static constexpr uint32_t kSmemRing = kTiles * kQBytes;
+  static constexpr uint32_t kSmemBar = kSmemRing + kSlots * kSlotBytes;
+  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2] fix full[slots] empty[slots]
+  static constexpr int kNumBars = 15 + 2 * kSlots;
   static constexpr uint32_t kSmemShared = kSmemBar + kNumBars * 8;  // u32 per slot
   static constexpr uint32_t kSmemTail = kSmemShared + kSlots * 4;   // tmem slot, abort flag
   static constexpr uint32_t kSmemBytes = (kSmemTail + 16 + 127) / 128 * 128;
@@ -99,9 +108,9 @@ struct Params {
   int seq_q, seq_k, nk;
   float scale_log2;
   unsigned int* status;
-  // Items [0, n_full) are whole units; unit n_full + u is split into `splits` items of
-  // steps_per_split steps, which write unnormalised fp32 O and (max, sum) to ws.
-  int pairs, n_items, n_full, splits, steps_per_split;
+  // Items [0, n_full) are whole pairs of tiles; pair n_full + i is split into `splits` items
+  // of entries_per_split list entries, which write unnormalised fp32 O and (max, sum) to ws.
+  int pairs, n_items, n_full, splits, entries_per_split;
   float* ws;
 };
 
@@ -114,32 +123,28 @@ __device__ __forceinline__ int rows_of(const int32_t* lens, int b, int seq) {
   return n < 0 ? 0 : (n > seq ? seq : n);
 }
 
-// One item: which (batch, head, pair), which lists and which steps of them.
-template <int SUB>
+// One item: which (batch, head, pair), and which entries of which lists.
 struct Item {
-  int batch, head, pair, split;  // split < 0: a whole unit
+  int batch, head, pair, split;  // split < 0: whole lists
   int q_rows, k_rows;            // rows that exist
-  int step0;
-  int entries[kTiles];           // list entries of tile t from step0 on
-  int steps[kTiles];
-  const int32_t* list[kTiles];   // from step0 on
+  int entries[kTiles];
+  const int32_t* list[kTiles];
 
   __device__ __forceinline__ void load(const Params& p, int item) {
-    int unit = item, rank = 0;
+    int whole = item, rank = 0;
     split = -1;
     if (item >= p.n_full) {
-      const int r = item - p.n_full;
-      unit = p.n_full + r / p.splits;
-      rank = r % p.splits;
-      split = r;
+      split = item - p.n_full;
+      whole = p.n_full + split / p.splits;
+      rank = split % p.splits;
     }
-    pair = unit % p.pairs;
-    const int bh = unit / p.pairs;
+    pair = whole % p.pairs;
+    const int bh = whole / p.pairs;
     head = bh % p.heads;
     batch = bh / p.heads;
     q_rows = rows_of(p.q_lens, batch, p.seq_q);
     k_rows = rows_of(p.k_lens, batch, p.seq_k);
-    step0 = split < 0 ? 0 : rank * p.steps_per_split;
+    const int first = split < 0 ? 0 : rank * p.entries_per_split;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       const int tile = kTiles * pair + t;
@@ -148,19 +153,20 @@ struct Item {
       if (tile * kTile < q_rows) {
         const int64_t at = (int64_t)bh * p.nq + tile / p.tiles_per_list;
         int n = p.counts != nullptr ? p.counts[at] : p.list_len;
-        n = min(max(n, 0), p.list_len) - step0 * SUB;
-        if (split >= 0) n = min(n, p.steps_per_split * SUB);
+        n = min(max(n, 0), p.list_len) - first;
+        if (split >= 0) n = min(n, p.entries_per_split);
         entries[t] = max(n, 0);
-        list[t] = p.indices + at * p.list_len + step0 * SUB;
+        list[t] = p.indices + at * p.list_len + first;
       }
-      steps[t] = (entries[t] + SUB - 1) / SUB;
     }
   }
 };
 
-// Keys of a listed block that exist: 0 for an entry that names no block.
-__device__ __forceinline__ int block_keys(int entry, int block_k, int nk, int k_rows) {
-  return (unsigned)entry < (unsigned)nk ? max(0, min(block_k, k_rows - entry * block_k)) : 0;
+// The 64 keys of a unit: first row, and how many rows exist (0 for an entry that names no block).
+template <int BK>
+__device__ __forceinline__ int unit_keys(int entry, int unit, int nk, int k_rows, int& row) {
+  row = (unsigned)entry < (unsigned)nk ? entry * BK + (unit & (BK / kUnit - 1)) * kUnit : k_rows;
+  return max(0, min(kUnit, k_rows - row));
 }
 
 // Two fp32 values as a pair of the operand type.
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sparse_fwd(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map, const Params prm) {
   using L = Layout<D>;
-  constexpr int kSub = kTile / BK;  // list entries per step
+  constexpr int kPer = BK / kUnit;  // units per list entry
   constexpr int kSlots = L::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -186,15 +192,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bars = sbase + L::kSmemBar;
   auto bar_qfull = [&](int t) { return bars + 8u * t; };
-  auto bar_qempty = [&](int t) { return bars + 8u * (kTiles + t); };
-  auto bar_full = [&](int s) { return bars + 8u * (2 * kTiles + s); };
-  auto bar_empty = [&](int s) { return bars + 8u * (2 * kTiles + kSlots + s); };
-  auto bar_s = [&](int t) { return bars + 8u * (2 * kTiles + 2 * kSlots + t); };
-  auto bar_p = [&](int t, int h) {
-    return bars + 8u * (2 * kTiles + 2 * kSlots + kTiles + 2 * t + h);
-  };
-  auto bar_o = [&](int t) { return bars + 8u * (2 * kTiles + 2 * kSlots + 3 * kTiles + t); };
-  const uint32_t bar_fix = bars + 8u * (2 * kTiles + 2 * kSlots + 4 * kTiles);
+  auto bar_qempty = [&](int t) { return bars + 8u * (2 + t); };
+  auto bar_s = [&](int t, uint32_t buf) { return bars + 8u * (4 + 2 * t + buf); };
+  auto bar_p = [&](int t, uint32_t buf) { return bars + 8u * (8 + 2 * t + buf); };
+  auto bar_pv = [&](int t) { return bars + 8u * (12 + t); };
+  const uint32_t bar_fix = bars + 8u * 14;
+  auto bar_full = [&](int s) { return bars + 8u * (15 + s); };
+  auto bar_empty = [&](int s) { return bars + 8u * (15 + kSlots + s); };
   volatile uint32_t* shared_flag = reinterpret_cast<uint32_t*>(smem + L::kSmemShared);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSmemTail);
   volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -206,10 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(bar_qfull(t), 1);
       mbar_init(bar_qempty(t), 1);
-      mbar_init(bar_s(t), 1);
-      mbar_init(bar_p(t, 0), 4 * 32);
-      mbar_init(bar_p(t, 1), 4 * 32);
-      mbar_init(bar_o(t), 1);
+      for (int buf = 0; buf < 2; ++buf) {
+        mbar_init(bar_s(t, buf), 1);
+        mbar_init(bar_p(t, buf), 4 * 32);
+      }
+      mbar_init(bar_pv(t), 1);
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(bar_full(s), 1);
@@ -236,6 +241,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, prm.status));
+  };
   // Both sides of the ring walk it in the same order; a slot index and its phase parity.
   struct Ring {
     int slot = 0;
@@ -251,70 +259,86 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoadWarp) {
     // ---------------- loads: the whole warp walks, one lane issues ----------------
     Ring ring;
-    uint32_t q_phase[kTiles] = {0, 0};  // parity of the next qempty wait, minus one use
+    uint32_t q_phase[kTiles] = {0, 0};
     uint32_t fix_phase = 0;
     bool ok = true;
-    auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, prm.status));
+    // A tile's walk along its list: entries of units u, u + 1, u + 2 (-1 behind the end), and
+    // two chunks of 32 entries, a lane each, the second on its way while the first is used.
+    struct Walk {
+      const int32_t* list;
+      int entries, units, e[3], chunk, ahead, base;
     };
     for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item<kSub> it;
+      Item it;
       it.load(prm, item);
       const int kv_head = it.head / prm.group;
-      // List entries ahead: lane l holds entry base + l of tile t's list.
-      int chunk[kTiles], chunk_base[kTiles];
+      Walk walk[kTiles];
+      auto read = [&](Walk& w, int from) { return from + lane < w.entries ? w.list[from + lane] : -1; };
+      auto entry = [&](Walk& w, int unit) -> int {  // called with ascending units
+        const int i = unit / kPer;
+        if (i >= w.entries) return -1;
+        if (i >= w.base + 32) {
+          w.base += 32;
+          w.chunk = w.ahead;
+          w.ahead = read(w, w.base + 32);
+        }
+        return __shfl_sync(0xffffffffu, w.chunk, i & 31);
+      };
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        chunk_base[t] = 0;
-        chunk[t] = lane < it.entries[t] ? it.list[t][lane] : -1;
+        Walk& w = walk[t];
+        w.list = it.list[t];
+        w.entries = it.entries[t];
+        w.units = w.entries * kPer;
+        w.base = 0;
+        w.chunk = read(w, 0);
+        w.ahead = read(w, 32);
+        w.e[0] = entry(w, 0);
+        w.e[1] = entry(w, 1);
+        w.e[2] = entry(w, 2);
       }
-      auto entry = [&](int t, int e) -> int {  // e never decreases by more than a chunk
-        if (e >= it.entries[t]) return -1;
-        if (e < chunk_base[t] || e >= chunk_base[t] + 32) {
-          chunk_base[t] = e & ~31;
-          chunk[t] = chunk_base[t] + lane < it.entries[t] ? it.list[t][chunk_base[t] + lane] : -1;
-        }
-        return __shfl_sync(0xffffffffu, chunk[t], e & 31);
-      };
-      // K or V rows of step `step` of tile t into the next slot.
-      auto push = [&](const CUtensorMap* map, int t, int step, bool is_v, bool shared) -> bool {
+      // The next slot: V of `unit_v` (none below 0) and K of `unit_k` (none from the end on),
+      // or, before the first unit, K of units 0 and 1.
+      auto push = [&](const Walk& w, int unit, bool shared) -> bool {
+        const bool first = unit < 0;
+        const bool two = first ? w.units > 1 : unit + 2 < w.units;  // both parts are there
+        int row0, row1;
+        const int keys0 = unit_keys<BK>(w.e[0], first ? 0 : unit, prm.nk, it.k_rows, row0);
+        const int keys1 = first ? unit_keys<BK>(w.e[1], 1, prm.nk, it.k_rows, row1)
+                                : unit_keys<BK>(w.e[2], unit + 2, prm.nk, it.k_rows, row1);
+        if (keys0 == 0) row0 = prm.seq_k;  // behind the end: zeros
+        if (keys1 == 0) row1 = prm.seq_k;
+        const bool cut = !first && keys0 > 0 && keys0 < kUnit && it.k_rows < prm.seq_k;
         if (!wait_all(bar_empty(ring.slot), ring.phase ^ 1)) return false;
-        const uint32_t dst = sbase + L::kSmemRing + ring.slot * L::kTileBytes;
+        const uint32_t dst = sbase + L::kSmemRing + ring.slot * L::kSlotBytes;
         const uint32_t full = bar_full(ring.slot);
-        int row[kSub], keys[kSub];
-        bool cut = false;
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          const int e = entry(t, step * kSub + s);
-          keys[s] = block_keys(e, BK, prm.nk, it.k_rows);
-          row[s] = keys[s] > 0 ? e * BK : prm.seq_k;  // behind the end: zeros
-          cut = cut || (is_v && keys[s] > 0 && keys[s] < BK && it.k_rows < prm.seq_k);
-        }
         if (elect_one()) {
           shared_flag[ring.slot] = shared ? 1u : 0u;
           const uint32_t bar = cut ? bar_fix : full;
-          mbar_expect_tx(bar, L::kTileBytes);
+          mbar_expect_tx(bar, two ? L::kSlotBytes : L::kPartBytes);
+          const CUtensorMap* map0 = first ? &k_map : &v_map;
 #pragma unroll
-          for (int s = 0; s < kSub; ++s)
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_4d(dst + h * kKvHalf, map0, bar, 64 * h, kv_head, row0, it.batch);
+          if (two) {
 #pragma unroll
             for (int h = 0; h < L::kHalves; ++h)
-              tma_load_4d(dst + h * kHalfBytes + s * BK * 128, map, bar, 64 * h, kv_head, row[s],
+              tma_load_4d(dst + L::kPartBytes + h * kKvHalf, &k_map, bar, 64 * h, kv_head, row1,
                           it.batch);
+          }
         }
         __syncwarp();
         if (cut) {
           // V rows behind the last key: zeros, then hand the slot over.
           if (!wait_all(bar_fix, fix_phase)) return false;
           fix_phase ^= 1;
-#pragma unroll
-          for (int s = 0; s < kSub; ++s)
-            for (int i = lane; i < (BK - keys[s]) * 8 * L::kHalves; i += 32) {
-              const int r = keys[s] + i / (8 * L::kHalves), c = i % (8 * L::kHalves);
-              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(
-                               dst + (c >> 3) * kHalfBytes + (s * BK + r) * 128 + (c & 7) * 16),
-                           "r"(0)
-                           : "memory");
-            }
+          for (int i = lane; i < (kUnit - keys0) * 8 * L::kHalves; i += 32) {
+            const int r = keys0 + i / (8 * L::kHalves), c = i % (8 * L::kHalves);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(
+                             dst + (c >> 3) * kKvHalf + r * 128 + (c & 7) * 16),
+                         "r"(0)
+                         : "memory");
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (elect_one()) mbar_arrive(full);
@@ -323,147 +347,135 @@ __global__ void __launch_bounds__(kThreads, 1)
         ring.next();
         return true;
       };
-      auto same = [&](int step) -> bool {  // both tiles at the same entries
-        if (step >= it.steps[0] || step >= it.steps[1]) return false;
-        bool eq = true;
-#pragma unroll
-        for (int s = 0; s < kSub; ++s)
-          eq = (entry(0, step * kSub + s) == entry(1, step * kSub + s)) && eq;
-        return eq;
-      };
-      bool share = same(0);
+      // Both tiles need the same slot: the same parts of the same blocks.
+      auto same_end = [&](int unit) { return (unit < walk[0].units) == (unit < walk[1].units); };
+      bool share = walk[0].units > 0 && walk[1].units > 0 && same_end(1) &&
+                   walk[0].e[0] == walk[1].e[0] && walk[0].e[1] == walk[1].e[1];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        if (it.steps[t] == 0 || !ok) continue;
+        if (walk[t].units == 0 || !ok) continue;
         ok = wait_all(bar_qempty(t), q_phase[t] ^ 1);
         if (!ok) break;
         q_phase[t] ^= 1;
         if (elect_one()) {
-          const uint32_t dst = sbase + L::kSmemQ + t * L::kTileBytes;
-          mbar_expect_tx(bar_qfull(t), L::kTileBytes);
+          const uint32_t dst = sbase + L::kSmemQ + t * L::kQBytes;
+          mbar_expect_tx(bar_qfull(t), L::kQBytes);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
-            tma_load_4d(dst + h * kHalfBytes, &q_map, bar_qfull(t), 64 * h, it.head,
+            tma_load_4d(dst + h * kQHalf, &q_map, bar_qfull(t), 64 * h, it.head,
                         (kTiles * it.pair + t) * kTile, it.batch);
         }
         __syncwarp();
-        if (t == 0 || !share) ok = push(&k_map, t, 0, false, share);
+        if (t == 0 || !share) ok = push(walk[t], -1, share);
       }
-      const int steps = max(it.steps[0], it.steps[1]);
-      for (int j = 0; j < steps && ok; ++j) {
-        const bool share_next = same(j + 1);
+      const int units = max(walk[0].units, walk[1].units);
+      for (int u = 0; u < units && ok; ++u) {
+        share = u < walk[0].units && u < walk[1].units && same_end(u + 2) &&
+                walk[0].e[0] == walk[1].e[0] && walk[0].e[2] == walk[1].e[2];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          if (j >= it.steps[t] || !ok) continue;
-          if (t == 0 || !share) ok = push(&v_map, t, j, true, share);
-          if (ok && j + 1 < it.steps[t] && (t == 0 || !share_next))
-            ok = push(&k_map, t, j + 1, false, share_next);
+          Walk& w = walk[t];
+          if (u < w.units && ok && (t == 0 || !share)) ok = push(w, u, share);
+          w.e[0] = w.e[1];
+          w.e[1] = w.e[2];
+          w.e[2] = entry(w, u + 3);
         }
-        share = share_next;
       }
     }
   } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
-    constexpr uint32_t idesc_qk = instr_desc(FP16, kTile, false);
+    constexpr uint32_t idesc_qk = instr_desc(FP16, kUnit, false);
     constexpr uint32_t idesc_pv = instr_desc(FP16, D, true);
-    auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, prm.status));
-    };
     const uint64_t q_desc0 = smem_desc(sbase + L::kSmemQ, 16, 1024);
     const uint64_t k_desc0 = smem_desc(sbase + L::kSmemRing, 16, 1024);
-    const uint64_t v_desc0 = smem_desc(sbase + L::kSmemRing, kHalfBytes, 1024);
+    const uint64_t v_desc0 = smem_desc(sbase + L::kSmemRing, kKvHalf, 1024);
     Ring ring;
-    uint32_t q_phase[kTiles] = {0, 0}, p_phase[kTiles] = {0, 0};
-    int k_held = 0;  // K slot tile 0 left for tile 1
-    bool ok = true;
-    // Takes the next slot of the ring and says whether both tiles read it.
-    auto take = [&](bool& shared) -> int {
+    uint32_t q_phase[kTiles] = {0, 0};
+    uint32_t n_s[kTiles] = {0, 0}, n_pv[kTiles] = {0, 0};  // units issued so far
+    bool ok = true, shared = false;
+    int slot = 0;
+    // The slot tile t reads next: the ring's next, or the one tile 0 left for tile 1.
+    auto take = [&](int t) {
+      if (t == 1 && shared) return;
       if (!wait_all(bar_full(ring.slot), ring.phase)) {
         ok = false;
-        return 0;
+        return;
       }
       tc_fence_after();
-      const int slot = ring.slot;
+      slot = ring.slot;
       shared = shared_flag[slot] != 0;
       ring.next();
-      return slot;
     };
-    auto commit = [&](uint32_t bar) {
-      if (elect_one()) mma_commit(bar);
-      __syncwarp();
+    // One lane: S_t = Q_t K^T, K being part `part` of the slot.
+    auto issue_s = [&](int t, int part) {
+      const uint64_t qd = q_desc0 + (uint64_t)((t * L::kQBytes) >> 4);
+      const uint64_t kd =
+          k_desc0 + (uint64_t)((slot * L::kSlotBytes + part * L::kPartBytes) >> 4);
+      const uint32_t d = tmem + kTmemS + t * 128 + (n_s[t] & 1) * 64;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t in = (kk & 3) * 32;
+        mma_ss(d, qd + (uint64_t)(((kk >> 2) * kQHalf + in) >> 4),
+               kd + (uint64_t)(((kk >> 2) * kKvHalf + in) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
+      }
+      mma_commit(bar_s(t, n_s[t] & 1));
     };
     for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item<kSub> it;
+      Item it;
       it.load(prm, item);
-      bool share = false, share_next = false;
-      auto issue_s = [&](int t, int step, bool& shared) {
-        const int slot = t == 1 && shared ? k_held : take(shared);
-        if (!ok) return;
-        if (t == 0) k_held = slot;
-        const uint64_t qd = q_desc0 + (uint64_t)((t * L::kTileBytes) >> 4);
-        const uint64_t kd = k_desc0 + (uint64_t)((slot * L::kTileBytes) >> 4);
-        const uint32_t d = tmem + kTmemS + t * 128;
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = (uint64_t)(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4);
-            mma_ss(d, qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(bar_s(t));
-          if (t == 1 || !shared) mma_commit(bar_empty(slot));
-          if (step + 1 == it.steps[t]) mma_commit(bar_qempty(t));
-        }
-        __syncwarp();
-      };
+      const int units[kTiles] = {it.entries[0] * kPer, it.entries[1] * kPer};
+      shared = false;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        if (it.steps[t] == 0 || !ok) continue;
+        if (units[t] == 0 || !ok) continue;
         ok = wait_all(bar_qfull(t), q_phase[t]);
         if (!ok) break;
         q_phase[t] ^= 1;
         tc_fence_after();
-        issue_s(t, 0, share);
+        take(t);
+        if (!ok) break;
+        if (elect_one()) issue_s(t, 0);
+        __syncwarp();
+        ++n_s[t];
+        if (units[t] > 1) {
+          if (elect_one()) issue_s(t, 1);
+          __syncwarp();
+          ++n_s[t];
+        }
+        if (elect_one()) {
+          if (t == 1 || !shared) mma_commit(bar_empty(slot));
+          if (units[t] <= 2) mma_commit(bar_qempty(t));
+        }
+        __syncwarp();
       }
-      const int steps = max(it.steps[0], it.steps[1]);
-      int v_slot = 0;
-      for (int j = 0; j < steps && ok; ++j) {
-        share_next = false;
+      const int most = max(units[0], units[1]);
+      for (int u = 0; u < most && ok; ++u) {
+        // A slot left for tile 1 is read in the same unit, or both tiles end there.
+        if (u >= units[0]) shared = false;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          if (j >= it.steps[t] || !ok) continue;
-          // O_t += P_t V in two 64-key halves as the softmax hands them over.
-          if (t == 0 || !share) {
-            bool v_shared = false;
-            v_slot = take(v_shared);
-            if (!ok) break;
-          }
-          const uint64_t vd = v_desc0 + (uint64_t)((v_slot * L::kTileBytes) >> 4);
-          const uint32_t d = tmem + kTmemO + t * 128;
-#pragma unroll
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = wait_all(bar_p(t, h), p_phase[t]);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int k4 = 0; k4 < 4; ++k4) {
-                const int kk = h * 4 + k4;
-                mma_ts(d, tmem + kTmemS + t * 128 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4),
-                       idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-              }
-            }
-            __syncwarp();
-          }
+          if (u >= units[t] || !ok) continue;
+          take(t);
           if (!ok) break;
-          p_phase[t] ^= 1;
-          if (t == 1 || !share) commit(bar_empty(v_slot));
-          if (j + 1 < it.steps[t]) {
-            issue_s(t, j + 1, share_next);
-          } else {
-            commit(bar_o(t));
+          ok = wait_all(bar_p(t, n_pv[t] & 1), (n_pv[t] >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = v_desc0 + (uint64_t)((slot * L::kSlotBytes) >> 4);
+            const uint32_t p = tmem + kTmemS + t * 128 + (n_pv[t] & 1) * 64;
+#pragma unroll
+            for (int kk = 0; kk < kUnit / 16; ++kk)
+              mma_ts(tmem + kTmemO + t * 128, p + kk * 8, vd + (uint64_t)((kk * 2048) >> 4),
+                     idesc_pv, (u > 0 || kk > 0) ? 1u : 0u);
+            mma_commit(bar_pv(t));
+            if (u + 2 < units[t]) issue_s(t, 1);
+            if (t == 1 || !shared) mma_commit(bar_empty(slot));
+            if (u + 3 == units[t]) mma_commit(bar_qempty(t));
           }
+          __syncwarp();
+          ++n_pv[t];
+          if (u + 2 < units[t]) ++n_s[t];
         }
-        share = share_next;
       }
     }
   } else {
@@ -472,84 +484,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3;
     const int row_in_tile = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t t_s = tmem + lanes + kTmemS + t * 128;
     const uint32_t t_o = tmem + lanes + kTmemO + t * 128;
     const float c = prm.scale_log2;
     const float2 c2 = make_float2(c, c);
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t n = 0;  // units so far: buffer n & 1, phase n >> 1
     bool ok = true;
     for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item<kSub> it;
+      Item it;
       it.load(prm, item);
-      const int n_steps = it.steps[t];
-      const int32_t* list = it.list[t];
+      const int32_t* list = t == 0 ? it.list[0] : it.list[1];
+      const int entries = t == 0 ? it.entries[0] : it.entries[1];
+      const int units = entries * kPer;
       float m_use = -INFINITY;  // running row max, log2 units, that P is taken against
       float l_sum = 0.f;
-      int e_next[kSub];
-      auto fetch = [&](int step) {
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          const int e = step * kSub + s;
-          e_next[s] = e < it.entries[t] ? __ldg(list + e) : -1;
-        }
-      };
-      fetch(0);
-      for (int j = 0; j < n_steps && ok; ++j) {
-        int keys[kSub];
-        bool whole = true;
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          keys[s] = block_keys(e_next[s], BK, prm.nk, it.k_rows);
-          whole = whole && keys[s] == BK;
-        }
-        fetch(j + 1);
-        ok = wait_bar(bar_s(t), s_phase, abort_flag, prm.status);
+      int e_next = entries > 0 ? __ldg(list) : -1;
+      for (int u = 0; u < units; ++u, ++n) {
+        int row;
+        const int keys = unit_keys<BK>(e_next, u, prm.nk, it.k_rows, row);
+        if ((u + 1) % kPer == 0 && u + 1 < units) e_next = __ldg(list + (u + 1) / kPer);
+        const uint32_t t_s = tmem + lanes + kTmemS + t * 128 + (n & 1) * 64;
         // tcgen05.ld/st below are warp-collective.
-        ok = __all_sync(0xffffffffu, ok);
+        ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
         if (!ok) break;
-        s_phase ^= 1;
         tc_fence_after();
-        uint32_t sv[4][32];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32(t_s + 32 * q4, sv[q4]);
+        uint32_t sv[2][32];
+        tmem_ld32(t_s, sv[0]);
+        tmem_ld32(t_s + 32, sv[1]);
         tmem_ld_wait(sv[0]);
         tmem_pin(sv[1]);
-        tmem_pin(sv[2]);
-        tmem_pin(sv[3]);
-        // Column 32*q4 + i exists if it is below the keys of its block.
-        auto mask = [&](int q4) {
-          const int limit = (kSub == 1 || q4 < 2) ? keys[0] : BK + keys[kSub - 1];
+        if (keys < kUnit) {  // columns from `keys` on do not exist
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * q4 + i >= limit) sv[q4][i] = __float_as_uint(-INFINITY);
-        };
-        if (!whole) {
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) mask(q4);
+          for (int i = 0; i < 64; ++i)
+            if (i >= keys) sv[i >> 5][i & 31] = __float_as_uint(-INFINITY);
         }
-        float2 acc[2];
-        uint32_t pk[32];
-        auto exponentiate = [&](int h, float m) {
-          const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: all p are 0
-          const float2 nm2 = make_float2(-base, -base);
+        float mx[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int key = 64 * h + 2 * i;
-            const uint32_t* src = sv[key >> 5] + (key & 31);
-            const float2 x = __ffma2_rn(
-                make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, nm2);
-            float2 p;
-            p.x = ex2(x.x);
-            p.y = ex2(x.y);
-            acc[i & 1] = __fadd2_rn(acc[i & 1], p);
-            pk[i] = pack_pair<FP16>(p.x, p.y);
-          }
-        };
-        // The row max and, independent of it, the first half of P against the running
-        // max; that half is redone when the max moved by more than the threshold.
-        float mx[8];
-#pragma unroll
-        for (int a = 0; a < 8; ++a) {
+        for (int a = 0; a < 4; ++a) {
           const uint32_t* r = sv[a >> 1] + (a & 1) * 16;
           float m = max3(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[2]));
 #pragma unroll
@@ -557,16 +527,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             m = max3(m, __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
           mx[a] = fmaxf(m, __uint_as_float(r[15]));
         }
-        acc[0] = acc[1] = make_float2(0.f, 0.f);
-        exponentiate(0, m_use);
-        const float row_max =
-            fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], max3(mx[4], mx[5], mx[6]), mx[7]));
-        const float m_new = row_max * c;
+        const float m_new = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
         const bool need = m_new > m_use + kRescaleThreshold;
         if (__any_sync(0xffffffffu, need)) {
           const float m_next = need ? m_new : m_use;
-          if (j > 0) {
-            // The PV of the step before is complete: the commit of this S covers it.
+          if (u > 0) {
+            // O is at rest once P V of the unit before is complete; these scores certify the
+            // one before that, so the parity names the phase.
+            ok = wait_all(bar_pv(t), (n - 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
             const float alpha = need ? ex2(m_use - m_next) : 1.f;
 #pragma unroll 1
             for (int q8 = 0; q8 < D / 16; ++q8) {
@@ -580,43 +550,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             l_sum *= alpha;
           }
           m_use = m_next;
-          // S columns [0, 64) are still intact.
-          tmem_ld32(t_s, sv[0]);
-          tmem_ld32(t_s + 32, sv[1]);
-          tmem_ld_wait(sv[0]);
-          tmem_pin(sv[1]);
-          if (!whole) {
-            mask(0);
-            mask(1);
-          }
-          acc[0] = acc[1] = make_float2(0.f, 0.f);
-          exponentiate(0, m_use);
         }
-        // P of keys [64h, 64h+64) -> S columns [32h, 32h+32), already read.
+        const float base = m_use == -INFINITY ? 0.f : m_use;  // no key yet: all p are 0
+        const float2 nm2 = make_float2(-base, -base);
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint32_t* src = sv[i >> 4] + 2 * (i & 15);
+          const float2 x = __ffma2_rn(
+              make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, nm2);
+          float2 p;
+          p.x = ex2(x.x);
+          p.y = ex2(x.y);
+          acc[i & 1] = __fadd2_rn(acc[i & 1], p);
+          pk[i] = pack_pair<FP16>(p.x, p.y);
+        }
+        // P over the first 32 of the unit's S columns, all of them read.
         tmem_st32(t_s, pk);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(bar_p(t, 0));
-        exponentiate(1, m_use);
-        tmem_st32(t_s + 32, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(bar_p(t, 1));
+        mbar_arrive(bar_p(t, n & 1));
         l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       }
       // ---------------- epilogue ----------------
-      if (ok && n_steps > 0) {
-        ok = wait_bar(bar_o(t), o_phase, abort_flag, prm.status);
-        ok = __all_sync(0xffffffffu, ok);
-        o_phase ^= 1;
-      }
+      // The last scores seen certify P V up to two units back only, so both phases that can
+      // still be open are waited for (a parity tells neighbouring phases apart, no others).
+      if (ok && units > 1) ok = wait_all(bar_pv(t), (n - 2) & 1);
+      if (ok && units > 0) ok = wait_all(bar_pv(t), (n - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       const int row = (kTiles * it.pair + t) * kTile + row_in_tile;
       const bool live = row < it.q_rows;
       if (it.split >= 0) {
         float* ws = prm.ws + ((int64_t)it.split * kTiles + t) * kWsTileFloats<D>;
-        if (n_steps > 0) {
+        if (units > 0) {
 #pragma unroll 1
           for (int q4 = 0; q4 < D / 32; ++q4) {
             uint32_t o[32];
@@ -636,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float2*>(ws + kTile * D + 2 * row_in_tile) = make_float2(m_use, l_sum);
         continue;
       }
-      const float inv_l = live && l_sum != 0.f ? 1.f / l_sum : 0.f;
+      const bool some = live && l_sum != 0.f;  // the row has a key
+      const float inv_l = some ? 1.f / l_sum : 0.f;
       uint16_t* dst = row < prm.seq_q
                           ? reinterpret_cast<uint16_t*>(prm.out) +
                                 (int64_t)it.batch * prm.o_batch_stride +
@@ -646,33 +615,33 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int q4 = 0; q4 < D / 32; ++q4) {
         uint32_t o[32];
-        if (n_steps > 0) {
+        if (units > 0) {
           tmem_ld32(t_o + 32 * q4, o);
           tmem_ld_wait(o);
         }
-        if (n_steps == 0 || !live || l_sum == 0.f) {
+        if (units == 0 || !some) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
         if (dst != nullptr) {
 #pragma unroll
           for (int v8 = 0; v8 < 4; ++v8) {
-            uint4 u;
-            u.x = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 0]) * inv_l,
+            uint4 w;
+            w.x = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 0]) * inv_l,
                                   __uint_as_float(o[v8 * 8 + 1]) * inv_l);
-            u.y = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 2]) * inv_l,
+            w.y = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 2]) * inv_l,
                                   __uint_as_float(o[v8 * 8 + 3]) * inv_l);
-            u.z = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 4]) * inv_l,
+            w.z = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 4]) * inv_l,
                                   __uint_as_float(o[v8 * 8 + 5]) * inv_l);
-            u.w = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 6]) * inv_l,
+            w.w = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 6]) * inv_l,
                                   __uint_as_float(o[v8 * 8 + 7]) * inv_l);
-            *reinterpret_cast<uint4*>(dst + 32 * q4 + v8 * 8) = u;
+            *reinterpret_cast<uint4*>(dst + 32 * q4 + v8 * 8) = w;
           }
         }
       }
       if (dst != nullptr && prm.lse != nullptr)
         prm.lse[((int64_t)it.batch * prm.heads + it.head) * prm.seq_q + row] =
-            live && l_sum != 0.f ? (m_use + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
+            some ? (m_use + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
     }
   }
 
@@ -691,24 +660,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of the split units: one warp per query row, D/32 columns per lane.
+// Joins the parts of the split pairs: one warp per query row, D/32 columns per lane.
 // O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.
 template <bool FP16, int D>
-__global__ void __launch_bounds__(256) sparse_combine(const Params prm, int split_units) {
+__global__ void __launch_bounds__(256) sparse_combine(const Params prm, int split_pairs) {
   const int gw = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  constexpr int kUnitRows = kTiles * kTile;
-  const int unit_rows = min(kUnitRows, prm.seq_q);
-  if (gw >= split_units * unit_rows) return;
-  const int ui = gw / unit_rows;
-  const int rr = gw - ui * unit_rows;
+  constexpr int kPairRows = kTiles * kTile;
+  const int pair_rows = min(kPairRows, prm.seq_q);
+  if (gw >= split_pairs * pair_rows) return;
+  const int ui = gw / pair_rows;
+  const int rr = gw - ui * pair_rows;
   const int t = rr / kTile;
   const int r_in_tile = rr - t * kTile;
-  const int unit = prm.n_full + ui;
-  const int bh = unit / prm.pairs;
+  const int whole = prm.n_full + ui;
+  const int bh = whole / prm.pairs;
   const int head = bh % prm.heads;
   const int batch = bh / prm.heads;
-  const int row = unit % prm.pairs * kUnitRows + rr;
+  const int row = whole % prm.pairs * kPairRows + rr;
   if (row >= prm.seq_q) return;
   const bool live = row < rows_of(prm.q_lens, batch, prm.seq_q);
   auto part = [&](int s) {
@@ -748,37 +717,37 @@ __global__ void __launch_bounds__(256) sparse_combine(const Params prm, int spli
 // ---------------------------------------------------------------------------
 
 struct Plan {
-  int pairs, units, n_full, splits, steps_per_split, items, split_units;
+  int pairs, total, n_full, splits, entries_per_split, items, split_pairs;
   int64_t ws_bytes;
 };
 
-// Whole units fill waves of SMs; when the last wave would leave at least half of them
-// idle, its units are split along their lists.
+// Whole pairs of tiles fill waves of SMs; when the last wave would leave at least half of
+// them idle, its pairs are split along their lists, down to 128 keys per part.
 Plan make_plan(int64_t batch, int64_t seq_q, int64_t heads, int64_t head_dim, int64_t block_k,
                int64_t list_len) {
   Plan pl{};
   pl.pairs = (int)((seq_q + kTiles * kTile - 1) / (kTiles * kTile));
-  pl.units = (int)(pl.pairs * heads * batch);
-  const int sub = (int)(kTile / block_k);
-  const int steps = (int)((list_len + sub - 1) / sub);
+  pl.total = (int)(pl.pairs * heads * batch);
+  const int least = (int)(2 * kUnit / block_k);  // entries of 128 keys
+  const int parts = (int)((list_len + least - 1) / least);
   const int sms = num_sms();
-  const int rem = pl.units % sms;
+  const int rem = pl.total % sms;
   pl.splits = 1;
-  pl.steps_per_split = steps;
-  pl.n_full = pl.items = pl.units;
-  if (rem > 0 && 2 * rem <= sms && steps >= 2) {
-    const int want = std::min(std::min(sms / rem, 32), steps);
-    pl.steps_per_split = (steps + want - 1) / want;
-    pl.splits = (steps + pl.steps_per_split - 1) / pl.steps_per_split;
+  pl.entries_per_split = (int)list_len;
+  pl.n_full = pl.items = pl.total;
+  if (rem > 0 && 2 * rem <= sms && parts >= 2) {
+    const int want = std::min(std::min(sms / rem, 32), parts);
+    pl.entries_per_split = (parts + want - 1) / want * least;
+    pl.splits = (int)((list_len + pl.entries_per_split - 1) / pl.entries_per_split);
   }
   if (pl.splits >= 2) {
-    pl.split_units = rem;
-    pl.n_full = pl.units - rem;
+    pl.split_pairs = rem;
+    pl.n_full = pl.total - rem;
     pl.items = pl.n_full + rem * pl.splits;
     pl.ws_bytes = (int64_t)rem * pl.splits * kTiles * (kTile * head_dim + 2 * kTile) * 4;
   } else {
     pl.splits = 1;
-    pl.steps_per_split = steps;
+    pl.entries_per_split = (int)list_len;
   }
   return pl;
 }
@@ -817,7 +786,7 @@ int make_map(CUtensorMap* map, const void* base, int64_t batch, int64_t seq, int
 
 template <bool FP16, int D, int BK>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p,
-           int split_units, cudaStream_t stream) {
+           int split_pairs, cudaStream_t stream) {
   static ContextSlot slots[kMaxDevices];
   cudaError_t e = cudaErrorInvalidDevice;
   if (context_cached(slots, [&]() -> void* {
@@ -833,20 +802,20 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   const unsigned grid = (unsigned)std::min(p.n_items, num_sms());
   sparse_fwd<FP16, D, BK><<<grid, kThreads, Layout<D>::kSmemAlloc, stream>>>(qm, km, vm, p);
   int rc = check_launch("h3b_block_sparse_attention");
-  if (rc != H3B_OK || split_units == 0) return rc;
-  const int rows = split_units * std::min(kTiles * kTile, p.seq_q);
-  sparse_combine<FP16, D><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p, split_units);
+  if (rc != H3B_OK || split_pairs == 0) return rc;
+  const int rows = split_pairs * std::min(kTiles * kTile, p.seq_q);
+  sparse_combine<FP16, D><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p, split_pairs);
   return check_launch("h3b_block_sparse_attention");
 }
 
 template <bool FP16>
 int launch_dims(int64_t head_dim, int64_t block_k, const CUtensorMap& qm, const CUtensorMap& km,
-                const CUtensorMap& vm, const Params& p, int split_units, cudaStream_t s) {
+                const CUtensorMap& vm, const Params& p, int split_pairs, cudaStream_t s) {
   if (head_dim == 128)
-    return block_k == 128 ? launch<FP16, 128, 128>(qm, km, vm, p, split_units, s)
-                          : launch<FP16, 128, 64>(qm, km, vm, p, split_units, s);
-  return block_k == 128 ? launch<FP16, 64, 128>(qm, km, vm, p, split_units, s)
-                        : launch<FP16, 64, 64>(qm, km, vm, p, split_units, s);
+    return block_k == 128 ? launch<FP16, 128, 128>(qm, km, vm, p, split_pairs, s)
+                          : launch<FP16, 128, 64>(qm, km, vm, p, split_pairs, s);
+  return block_k == 128 ? launch<FP16, 64, 128>(qm, km, vm, p, split_pairs, s)
+                        : launch<FP16, 64, 64>(qm, km, vm, p, split_pairs, s);
 }
 
 }  // namespace sparse
@@ -921,18 +890,18 @@ extern "C" int h3b_block_sparse_attention(
                      q_head_stride, kTile, fp16, "q")) != H3B_OK)
     return rc;
   if ((rc = make_map(&km, k, batch, seq_k, kv_heads, head_dim, k_batch_stride, k_row_stride,
-                     k_head_stride, (int)block_k, fp16, "k")) != H3B_OK)
+                     k_head_stride, kUnit, fp16, "k")) != H3B_OK)
     return rc;
   if ((rc = make_map(&vm, v, batch, seq_k, kv_heads, head_dim, v_batch_stride, v_row_stride,
-                     v_head_stride, (int)block_k, fp16, "v")) != H3B_OK)
+                     v_head_stride, kUnit, fp16, "v")) != H3B_OK)
     return rc;
   Plan pl = make_plan(batch, seq_q, heads, head_dim, block_k, list_len);
   if (pl.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < pl.ws_bytes ||
                           !h3b::aligned16(workspace))) {
-    // No (or too small a) workspace: run every unit whole.
+    // No (or too small a) workspace: run every pair whole.
     pl.splits = 1;
-    pl.split_units = 0;
-    pl.n_full = pl.items = pl.units;
+    pl.split_pairs = 0;
+    pl.n_full = pl.items = pl.total;
   }
   Params p{};
   p.out = out;
@@ -958,8 +927,8 @@ extern "C" int h3b_block_sparse_attention(
   p.n_items = pl.items;
   p.n_full = pl.n_full;
   p.splits = pl.splits;
-  p.steps_per_split = pl.steps_per_split;
+  p.entries_per_split = pl.entries_per_split;
   p.ws = reinterpret_cast<float*>(workspace);
-  return fp16 ? launch_dims<true>(head_dim, block_k, qm, km, vm, p, pl.split_units, stream)
-              : launch_dims<false>(head_dim, block_k, qm, km, vm, p, pl.split_units, stream);
+  return fp16 ? launch_dims<true>(head_dim, block_k, qm, km, vm, p, pl.split_pairs, stream)
+              : launch_dims<false>(head_dim, block_k, qm, km, vm, p, pl.split_pairs, stream);
 }
