@@ -11,12 +11,15 @@
 // loads of an item start while the one before it ends.
 //
 //   warp 8      loads: the Q tiles of the item, then a ring of slots. Slot u of a tile holds
-//               V of unit u and K of unit u + 2, which the MMA warp reads one after the
-//               other (a first slot holds K of units 0 and 1). Where both tiles of the pair
-//               are at the same entries the slot is filled once and read by both ("shared");
-//               the lists decide, so no entry needs sorting.
-//   warp 9      MMA issuer, one elected lane, tiles t = 0, 1 in turn: O_t += P_t(u) V(u), then
-//               S_t(u + 2) = Q_t K(u + 2)^T into the TMEM columns P_t(u) came from.
+//               V of unit u and K of unit u + 2, which the tile's MMA warp reads one after
+//               the other (a first slot holds K of units 0 and 1). Where the tiles of a pair
+//               have one list (block_q = 256) one slot serves both; with lists of their own
+//               slots of tile 0 and tile 1 alternate.
+//   warps 9, 10 MMA issuers of tile 0 and 1, one elected lane each: O_t += P_t(u) V(u), then
+//               S_t(u + 2) = Q_t K(u + 2)^T into the TMEM columns P_t(u) came from. The
+//               tensor core takes only an MMA or two ahead, so issuing a unit lasts as long
+//               as its MMAs (about 690 clocks) and the waits before it (about 420) would
+//               leave it idle: with a warp per tile the other's MMAs fill them.
 //   warps 0-3   softmax of tile 0, warps 4-7 of tile 1, a thread per row: scores from TMEM,
 //               row max, p, row sum; P goes back over the S columns; O is rescaled in TMEM
 //               only when the running max grew by more than 2^8. P is rounded to the type
@@ -56,9 +59,9 @@ constexpr int kTile = 128;  // query rows per tile
 constexpr int kUnit = 64;   // keys per unit
 constexpr int kTiles = 2;
 constexpr int kSoftmaxWarps = 4 * kTiles;
-constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kThreads = (kSoftmaxWarps + 1 + kTiles) * 32;
 constexpr int kLoadWarp = kSoftmaxWarps;
-constexpr int kMmaWarp = kSoftmaxWarps + 1;
+constexpr int kMmaWarp = kSoftmaxWarps + 1;  // + tile
 constexpr uint32_t kQHalf = kTile * 128;   // 128 rows x 64 columns, 128-byte swizzle
 constexpr uint32_t kKvHalf = kUnit * 128;  // 64 rows x 64 columns
 constexpr uint32_t kTmemCols = 512;
@@ -79,10 +82,9 @@ struct Layout {
   static constexpr uint32_t kSmemQ = 0;
   static constexpr uint32_t kSmemRing = kTiles * kQBytes;
   static constexpr uint32_t kSmemBar = kSmemRing + kSlots * kSlotBytes;
-  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2] fix full[slots] empty[slots]
-  static constexpr int kNumBars = 15 + 2 * kSlots;
-  static constexpr uint32_t kSmemShared = kSmemBar + kNumBars * 8;  // u32 per slot
-  static constexpr uint32_t kSmemTail = kSmemShared + kSlots * 4;   // tmem slot, abort flag
+  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2][2] fix full[slots] empty[slots]
+  static constexpr int kNumBars = 17 + 2 * kSlots;
+  static constexpr uint32_t kSmemTail = kSmemBar + kNumBars * 8;  // tmem slot, abort flag
   static constexpr uint32_t kSmemBytes = (kSmemTail + 16 + 127) / 128 * 128;
   static constexpr uint32_t kSmemAlloc = kSmemBytes + 1024;
   static_assert(kSmemAlloc <= 232448, "shared memory per CTA");
@@ -195,11 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar_qempty = [&](int t) { return bars + 8u * (2 + t); };
   auto bar_s = [&](int t, uint32_t buf) { return bars + 8u * (4 + 2 * t + buf); };
   auto bar_p = [&](int t, uint32_t buf) { return bars + 8u * (8 + 2 * t + buf); };
-  auto bar_pv = [&](int t) { return bars + 8u * (12 + t); };
-  const uint32_t bar_fix = bars + 8u * 14;
-  auto bar_full = [&](int s) { return bars + 8u * (15 + s); };
-  auto bar_empty = [&](int s) { return bars + 8u * (15 + kSlots + s); };
-  volatile uint32_t* shared_flag = reinterpret_cast<uint32_t*>(smem + L::kSmemShared);
+  auto bar_pv = [&](int t, uint32_t buf) { return bars + 8u * (12 + 2 * t + buf); };
+  const uint32_t bar_fix = bars + 8u * 16;
+  auto bar_full = [&](int s) { return bars + 8u * (17 + s); };
+  auto bar_empty = [&](int s) { return bars + 8u * (17 + kSlots + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSmemTail);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
@@ -213,12 +214,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int buf = 0; buf < 2; ++buf) {
         mbar_init(bar_s(t, buf), 1);
         mbar_init(bar_p(t, buf), 4 * 32);
+        mbar_init(bar_pv(t, buf), 1);
       }
-      mbar_init(bar_pv(t), 1);
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(bar_full(s), 1);
-      mbar_init(bar_empty(s), 1);
+      mbar_init(bar_empty(s), prm.tiles_per_list);  // the tiles that read a slot
     }
     mbar_init(bar_fix, 1);
     *abort_flag = 0u;
@@ -244,21 +245,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, prm.status));
   };
-  // Both sides of the ring walk it in the same order; a slot index and its phase parity.
-  struct Ring {
-    int slot = 0;
-    uint32_t phase = 0;
-    __device__ __forceinline__ void next() {
-      if (++slot == kSlots) {
-        slot = 0;
-        phase ^= 1;
-      }
-    }
-  };
+  // Slots are filled and read in one order; `pos` counts them since the start.
+  auto slot_of = [](uint32_t pos) { return (int)(pos % kSlots); };
+  auto phase_of = [](uint32_t pos) { return (pos / kSlots) & 1u; };
+  const bool shared = prm.tiles_per_list == kTiles;  // one slot serves both tiles
 
   if (warp == kLoadWarp) {
     // ---------------- loads: the whole warp walks, one lane issues ----------------
-    Ring ring;
+    uint32_t pos = 0;
     uint32_t q_phase[kTiles] = {0, 0};
     uint32_t fix_phase = 0;
     bool ok = true;
@@ -299,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // The next slot: V of `unit_v` (none below 0) and K of `unit_k` (none from the end on),
       // or, before the first unit, K of units 0 and 1.
-      auto push = [&](const Walk& w, int unit, bool shared) -> bool {
+      auto push = [&](const Walk& w, int unit) -> bool {
         const bool first = unit < 0;
         const bool two = first ? w.units > 1 : unit + 2 < w.units;  // both parts are there
         int row0, row1;
@@ -309,11 +303,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (keys0 == 0) row0 = prm.seq_k;  // behind the end: zeros
         if (keys1 == 0) row1 = prm.seq_k;
         const bool cut = !first && keys0 > 0 && keys0 < kUnit && it.k_rows < prm.seq_k;
-        if (!wait_all(bar_empty(ring.slot), ring.phase ^ 1)) return false;
-        const uint32_t dst = sbase + L::kSmemRing + ring.slot * L::kSlotBytes;
-        const uint32_t full = bar_full(ring.slot);
+        const int slot = slot_of(pos);
+        if (!wait_all(bar_empty(slot), phase_of(pos) ^ 1)) return false;
+        const uint32_t dst = sbase + L::kSmemRing + slot * L::kSlotBytes;
+        const uint32_t full = bar_full(slot);
         if (elect_one()) {
-          shared_flag[ring.slot] = shared ? 1u : 0u;
           const uint32_t bar = cut ? bar_fix : full;
           mbar_expect_tx(bar, two ? L::kSlotBytes : L::kPartBytes);
           const CUtensorMap* map0 = first ? &k_map : &v_map;
@@ -344,13 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) mbar_arrive(full);
           __syncwarp();
         }
-        ring.next();
+        ++pos;
         return true;
       };
-      // Both tiles need the same slot: the same parts of the same blocks.
-      auto same_end = [&](int unit) { return (unit < walk[0].units) == (unit < walk[1].units); };
-      bool share = walk[0].units > 0 && walk[1].units > 0 && same_end(1) &&
-                   walk[0].e[0] == walk[1].e[0] && walk[0].e[1] == walk[1].e[1];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         if (walk[t].units == 0 || !ok) continue;
@@ -366,117 +356,112 @@ __global__ void __launch_bounds__(kThreads, 1)
                         (kTiles * it.pair + t) * kTile, it.batch);
         }
         __syncwarp();
-        if (t == 0 || !share) ok = push(walk[t], -1, share);
+        if (t == 0 || !shared) ok = push(walk[t], -1);
       }
       const int units = max(walk[0].units, walk[1].units);
       for (int u = 0; u < units && ok; ++u) {
-        share = u < walk[0].units && u < walk[1].units && same_end(u + 2) &&
-                walk[0].e[0] == walk[1].e[0] && walk[0].e[2] == walk[1].e[2];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           Walk& w = walk[t];
-          if (u < w.units && ok && (t == 0 || !share)) ok = push(w, u, share);
+          if (u < w.units && ok && (t == 0 || !shared)) ok = push(w, u);
           w.e[0] = w.e[1];
           w.e[1] = w.e[2];
           w.e[2] = entry(w, u + 3);
         }
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
+  } else if (warp >= kMmaWarp) {
+    // ---------------- MMA issuer of tile t ----------------
+    const int t = warp - kMmaWarp;
     constexpr uint32_t idesc_qk = instr_desc(FP16, kUnit, false);
     constexpr uint32_t idesc_pv = instr_desc(FP16, D, true);
-    const uint64_t q_desc0 = smem_desc(sbase + L::kSmemQ, 16, 1024);
+    const uint64_t q_desc = smem_desc(sbase + L::kSmemQ + t * L::kQBytes, 16, 1024);
     const uint64_t k_desc0 = smem_desc(sbase + L::kSmemRing, 16, 1024);
     const uint64_t v_desc0 = smem_desc(sbase + L::kSmemRing, kKvHalf, 1024);
-    Ring ring;
-    uint32_t q_phase[kTiles] = {0, 0};
-    uint32_t n_s[kTiles] = {0, 0}, n_pv[kTiles] = {0, 0};  // units issued so far
-    bool ok = true, shared = false;
-    int slot = 0;
-    // The slot tile t reads next: the ring's next, or the one tile 0 left for tile 1.
-    auto take = [&](int t) {
-      if (t == 1 && shared) return;
-      if (!wait_all(bar_full(ring.slot), ring.phase)) {
-        ok = false;
-        return;
-      }
-      tc_fence_after();
-      slot = ring.slot;
-      shared = shared_flag[slot] != 0;
-      ring.next();
-    };
-    // One lane: S_t = Q_t K^T, K being part `part` of the slot.
-    auto issue_s = [&](int t, int part) {
-      const uint64_t qd = q_desc0 + (uint64_t)((t * L::kQBytes) >> 4);
+    const uint32_t t_s = tmem + kTmemS + t * 128;
+    const uint32_t t_o = tmem + kTmemO + t * 128;
+    uint32_t base = 0;           // slots of the items before
+    uint32_t n_s = 0, n_pv = 0;  // units issued so far
+    uint32_t q_phase = 0;
+    bool ok = true;
+    // One lane: S = Q K^T, K being part `part` of the slot.
+    auto issue_s = [&](int slot, int part) {
       const uint64_t kd =
           k_desc0 + (uint64_t)((slot * L::kSlotBytes + part * L::kPartBytes) >> 4);
-      const uint32_t d = tmem + kTmemS + t * 128 + (n_s[t] & 1) * 64;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t in = (kk & 3) * 32;
-        mma_ss(d, qd + (uint64_t)(((kk >> 2) * kQHalf + in) >> 4),
+        mma_ss(t_s + (n_s & 1) * 64, q_desc + (uint64_t)(((kk >> 2) * kQHalf + in) >> 4),
                kd + (uint64_t)(((kk >> 2) * kKvHalf + in) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
       }
-      mma_commit(bar_s(t, n_s[t] & 1));
+      mma_commit(bar_s(t, n_s & 1));
     };
     for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
       Item it;
       it.load(prm, item);
-      const int units[kTiles] = {it.entries[0] * kPer, it.entries[1] * kPer};
-      shared = false;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        if (units[t] == 0 || !ok) continue;
-        ok = wait_all(bar_qfull(t), q_phase[t]);
+      const int units0 = it.entries[0] * kPer, units1 = it.entries[1] * kPer;
+      const int units = t == 0 ? units0 : units1;
+      // Where this tile's slots are: its first at base + lead, slot u at `next`, which steps
+      // over the other tile's while that has units left.
+      const int other = t == 0 ? units1 : units0;
+      const uint32_t lead = t == 1 && !shared && units0 > 0 ? 1u : 0u;
+      const uint32_t firsts = shared ? 1u : (units0 > 0) + (units1 > 0);
+      uint32_t next = base + firsts + (t == 1 && !shared && units0 > 0 ? 1u : 0u);
+      const uint32_t slots = units0 == 0 && units1 == 0 ? 0u
+                             : firsts + (shared ? max(units0, units1) : units0 + units1);
+      auto release = [&](int slot) {  // one lane
+        mma_commit(bar_empty(slot));
+        if (shared && other == 0) mma_commit(bar_empty(slot));  // nobody else reads it
+      };
+      if (units > 0) {
+        const uint32_t first = base + lead;
+        const int slot = slot_of(first);
+        ok = wait_all(bar_qfull(t), q_phase) && wait_all(bar_full(slot), phase_of(first));
         if (!ok) break;
-        q_phase[t] ^= 1;
+        q_phase ^= 1;
         tc_fence_after();
-        take(t);
-        if (!ok) break;
-        if (elect_one()) issue_s(t, 0);
+        if (elect_one()) issue_s(slot, 0);
         __syncwarp();
-        ++n_s[t];
-        if (units[t] > 1) {
-          if (elect_one()) issue_s(t, 1);
+        ++n_s;
+        if (units > 1) {
+          if (elect_one()) issue_s(slot, 1);
           __syncwarp();
-          ++n_s[t];
+          ++n_s;
         }
         if (elect_one()) {
-          if (t == 1 || !shared) mma_commit(bar_empty(slot));
-          if (units[t] <= 2) mma_commit(bar_qempty(t));
+          release(slot);
+          if (units <= 2) mma_commit(bar_qempty(t));
         }
         __syncwarp();
       }
-      const int most = max(units[0], units[1]);
-      for (int u = 0; u < most && ok; ++u) {
-        // A slot left for tile 1 is read in the same unit, or both tiles end there.
-        if (u >= units[0]) shared = false;
+      for (int u = 0; u < units; ++u) {
+        const int slot = slot_of(next);
+        ok = wait_all(bar_full(slot), phase_of(next)) &&
+             wait_all(bar_p(t, n_pv & 1), (n_pv >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = v_desc0 + (uint64_t)((slot * L::kSlotBytes) >> 4);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          if (u >= units[t] || !ok) continue;
-          take(t);
-          if (!ok) break;
-          ok = wait_all(bar_p(t, n_pv[t] & 1), (n_pv[t] >> 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t vd = v_desc0 + (uint64_t)((slot * L::kSlotBytes) >> 4);
-            const uint32_t p = tmem + kTmemS + t * 128 + (n_pv[t] & 1) * 64;
-#pragma unroll
-            for (int kk = 0; kk < kUnit / 16; ++kk)
-              mma_ts(tmem + kTmemO + t * 128, p + kk * 8, vd + (uint64_t)((kk * 2048) >> 4),
-                     idesc_pv, (u > 0 || kk > 0) ? 1u : 0u);
-            mma_commit(bar_pv(t));
-            if (u + 2 < units[t]) issue_s(t, 1);
-            if (t == 1 || !shared) mma_commit(bar_empty(slot));
-            if (u + 3 == units[t]) mma_commit(bar_qempty(t));
-          }
-          __syncwarp();
-          ++n_pv[t];
-          if (u + 2 < units[t]) ++n_s[t];
+          for (int kk = 0; kk < kUnit / 16; ++kk)
+            mma_ts(t_o, t_s + (n_pv & 1) * 64 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4),
+                   idesc_pv, (u > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(bar_pv(t, n_pv & 1));
+          if (u + 2 < units) issue_s(slot, 1);
+          release(slot);
+          if (u + 3 == units) mma_commit(bar_qempty(t));
+        }
+        __syncwarp();
+        ++n_pv;
+        if (u + 2 < units) ++n_s;
+        // Slots in order: unit u of tile 0, of tile 1, unit u + 1 of tile 0, ...
+        if (shared) {
+          next += 1;
+        } else {
+          next += 1u + (t == 0 ? u < other : u + 1 < other);
         }
       }
+      base += slots;
     }
   } else {
     // ---------------- softmax: warp -> (tile, lane quadrant), thread -> query row ----------------
@@ -532,9 +517,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, need)) {
           const float m_next = need ? m_new : m_use;
           if (u > 0) {
-            // O is at rest once P V of the unit before is complete; these scores certify the
-            // one before that, so the parity names the phase.
-            ok = wait_all(bar_pv(t), (n - 1) & 1);
+            // O is at rest once P V of the unit before is complete. That one's buffer was last
+            // used two units before it, which these scores certify: the parity names the phase.
+            ok = wait_all(bar_pv(t, (n - 1) & 1), ((n - 1) >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
             const float alpha = need ? ex2(m_use - m_next) : 1.f;
@@ -574,10 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       }
       // ---------------- epilogue ----------------
-      // The last scores seen certify P V up to two units back only, so both phases that can
-      // still be open are waited for (a parity tells neighbouring phases apart, no others).
-      if (ok && units > 1) ok = wait_all(bar_pv(t), (n - 2) & 1);
-      if (ok && units > 0) ok = wait_all(bar_pv(t), (n - 1) & 1);
+      if (ok && units > 0) ok = wait_all(bar_pv(t, (n - 1) & 1), ((n - 1) >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
       const int row = (kTiles * it.pair + t) * kTile + row_in_tile;

@@ -109,6 +109,31 @@ def test_many_items_per_cta():
     _check(block_sparse_attention(q, k, v, shifted, n), None, q, k, v, shifted, n)
 
 
+@pytest.mark.parametrize("block_q", [128, 256])
+@pytest.mark.parametrize("block_k", [64, 128])
+def test_short_lists_over_and_over(block_q, block_k):
+    """Items of one to three units, many per CTA, many calls: every wait ends, the bits repeat."""
+
+    from h3_flash_b200 import _lib
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
+
+    s, h = 148 * 256, 2
+    q, k, v = (_randn((1, s, h, 128), i) for i in (1, 2, 3))
+    nq, nk = s // block_q, s // block_k
+    for n in (1, 2, 3):
+        indices = torch.randint(0, nk, (1, h, nq, n), device="cuda", generator=torch.Generator("cuda").manual_seed(n)).int()
+        for counts in (None, torch.randint(0, n + 1, (1, h, nq), device="cuda").int()):
+            first = block_sparse_attention(q, k, v, indices, counts, block_q=block_q, block_k=block_k)
+            for _ in range(40):
+                again = block_sparse_attention(q, k, v, indices, counts, block_q=block_q, block_k=block_k)
+            assert torch.equal(first, again)
+            assert _lib.device_status() == 0
+            rows = slice(0, 512)
+            part = indices[:, :, : 512 // block_q].contiguous()
+            n_part = None if counts is None else counts[:, :, : 512 // block_q].contiguous()
+            _check(first[:, rows], None, q[:, rows], k, v, part, n_part, block_q=block_q, block_k=block_k)
+
+
 @pytest.mark.parametrize("block_k", [64, 128])
 @pytest.mark.parametrize("d", [64, 128])
 def test_padded_batch_with_nan(d, block_k):
