@@ -7,10 +7,12 @@
 //
 // The unit of work along a list is 64 keys: a listed block of 64, or half of one of 128. A
 // work item is a pair of neighbouring 128-row query tiles of one (batch, head), or a range
-// of units of such a pair. CTAs are persistent: item i runs on CTA i mod gridDim, and the
-// loads of an item start while the one before it ends.
+// of units of such a pair; where the queries are one tile (a few rows against a long list)
+// the two tiles of an item are that tile with two ranges of its list. CTAs are persistent:
+// item i runs on CTA i mod gridDim, and the loads of an item start while the one before ends.
 //
-//   warp 8      loads: the Q tiles of the item, then a ring of slots. Slot u of a tile holds
+//   warp 8      loads: what an item is, read from global memory one item ahead and handed to
+//               the other warps through shared memory; its Q tiles; then a ring of slots. Slot u of a tile holds
 //               V of unit u and K of unit u + 2, which the tile's MMA warp reads one after
 //               the other (a first slot holds K of units 0 and 1). Where the tiles of a pair
 //               have one list (block_q = 256) one slot serves both; with lists of their own
@@ -44,6 +46,7 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -71,6 +74,17 @@ constexpr uint32_t kTmemO = 256;  // + t*128
 // stays within 2^8, exact in the fp32 accumulator and inside fp16's range.
 constexpr float kRescaleThreshold = 8.0f;
 
+// What the MMA and softmax warps know of an item.
+struct Info {
+  int batch, head, row0[kTiles];  // first query row of the tiles
+  int q_rows;                     // rows of the batch entry that exist
+  int units[kTiles];
+  int part;  // workspace part of tile 0 (tile 1: the next), or -1: rows are final
+};
+// Keys of the units ahead, per tile: more than the slots of the ring and the scores in TMEM
+// can be ahead of the softmax (10 + 2 units).
+constexpr int kKeyRing = 16;
+
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;
@@ -82,9 +96,12 @@ struct Layout {
   static constexpr uint32_t kSmemQ = 0;
   static constexpr uint32_t kSmemRing = kTiles * kQBytes;
   static constexpr uint32_t kSmemBar = kSmemRing + kSlots * kSlotBytes;
-  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2][2] fix full[slots] empty[slots]
-  static constexpr int kNumBars = 17 + 2 * kSlots;
-  static constexpr uint32_t kSmemTail = kSmemBar + kNumBars * 8;  // tmem slot, abort flag
+  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2][2] fix ifull[2] iempty[2] full[slots] empty[slots]
+  static constexpr int kNumBars = 21 + 2 * kSlots;
+  static constexpr uint32_t kSmemInfo = kSmemBar + kNumBars * 8;           // Info[2]
+  static constexpr uint32_t kSmemKeys = kSmemInfo + 2 * sizeof(Info);      // u8 [2][kKeyRing]
+  static constexpr uint32_t kSmemTag = kSmemKeys + kTiles * kKeyRing;      // u32 [slots]
+  static constexpr uint32_t kSmemTail = kSmemTag + 4 * kSlots;             // tmem slot, abort flag
   static constexpr uint32_t kSmemBytes = (kSmemTail + 16 + 127) / 128 * 128;
   static constexpr uint32_t kSmemAlloc = kSmemBytes + 1024;
   static_assert(kSmemAlloc <= 232448, "shared memory per CTA");
@@ -111,13 +128,13 @@ struct Params {
   float scale_log2;
   unsigned int* status;
   // Items [0, n_full) are whole pairs of tiles; pair n_full + i is split into `splits` items
-  // of entries_per_split list entries, which write unnormalised fp32 O and (max, sum) to ws.
-  int pairs, n_items, n_full, splits, entries_per_split;
+  // of entries_per_split list entries. With `duo` (one query tile) both tiles of an item are
+  // that tile, with entries_per_split entries each. Split items write unnormalised fp32 O
+  // and (max, sum) of `ws_rows` rows per tile to ws: ws_rows * D, then ws_rows * 4 floats of
+  // which two are used (a part starts on 16 bytes).
+  int pairs, n_items, n_full, splits, entries_per_split, duo, ws_rows, wide_out;
   float* ws;
 };
-
-template <int D>
-constexpr int kWsTileFloats = kTile * D + 2 * kTile;
 
 __device__ __forceinline__ int rows_of(const int32_t* lens, int b, int seq) {
   if (lens == nullptr) return seq;
@@ -125,42 +142,51 @@ __device__ __forceinline__ int rows_of(const int32_t* lens, int b, int seq) {
   return n < 0 ? 0 : (n > seq ? seq : n);
 }
 
-// One item: which (batch, head, pair), and which entries of which lists.
+// One item as the load warp reads it: everything that comes from global memory is asked for
+// at once, list entries a lane each (entries lane and 32 + lane of both lists).
 struct Item {
-  int batch, head, pair, split;  // split < 0: whole lists
-  int q_rows, k_rows;            // rows that exist
-  int entries[kTiles];
-  const int32_t* list[kTiles];
+  int batch, head, row0[kTiles], q_len, k_len, part;
+  int count[kTiles];            // as it stands in memory
+  int first[kTiles], most[kTiles];  // the item's first entry, and how many it may use
+  const int32_t* list[kTiles];  // from the first entry on
+  int chunk[kTiles], ahead[kTiles];
 
-  __device__ __forceinline__ void load(const Params& p, int item) {
+  __device__ __forceinline__ void load(const Params& p, int item, int lane) {
     int whole = item, rank = 0;
-    split = -1;
-    if (item >= p.n_full) {
-      split = item - p.n_full;
-      whole = p.n_full + split / p.splits;
-      rank = split % p.splits;
+    const bool split = item >= p.n_full;
+    part = -1;
+    if (split) {
+      const int i = item - p.n_full;
+      whole = p.n_full + i / p.splits;
+      rank = i % p.splits;
+      part = i * kTiles;
     }
-    pair = whole % p.pairs;
+    const int pair = whole % p.pairs;
     const int bh = whole / p.pairs;
     head = bh % p.heads;
     batch = bh / p.heads;
-    q_rows = rows_of(p.q_lens, batch, p.seq_q);
-    k_rows = rows_of(p.k_lens, batch, p.seq_k);
-    const int first = split < 0 ? 0 : rank * p.entries_per_split;
+    q_len = p.q_lens != nullptr ? p.q_lens[batch] : p.seq_q;
+    k_len = p.k_lens != nullptr ? p.k_lens[batch] : p.seq_k;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-      const int tile = kTiles * pair + t;
-      entries[t] = 0;
-      list[t] = p.indices;
-      if (tile * kTile < q_rows) {
-        const int64_t at = (int64_t)bh * p.nq + tile / p.tiles_per_list;
-        int n = p.counts != nullptr ? p.counts[at] : p.list_len;
-        n = min(max(n, 0), p.list_len) - first;
-        if (split >= 0) n = min(n, p.entries_per_split);
-        entries[t] = max(n, 0);
-        list[t] = p.indices + at * p.list_len + first;
-      }
+      const int tile = p.duo ? 0 : kTiles * pair + t;
+      row0[t] = tile * kTile;
+      first[t] = split ? (p.duo ? kTiles * rank + t : rank) * p.entries_per_split : 0;
+      // A tile behind the last row has no list of its own; it gets no entries either.
+      const int64_t at = (int64_t)bh * p.nq + min(tile / p.tiles_per_list, p.nq - 1);
+      count[t] = p.counts != nullptr ? p.counts[at] : p.list_len;
+      most[t] = split ? min(p.entries_per_split, p.list_len - first[t]) : p.list_len;
+      list[t] = p.indices + at * p.list_len + first[t];
+      chunk[t] = lane < most[t] ? list[t][lane] : -1;
+      ahead[t] = 32 + lane < most[t] ? list[t][32 + lane] : -1;
     }
+  }
+  __device__ __forceinline__ int q_rows(const Params& p) const { return min(max(q_len, 0), p.seq_q); }
+  __device__ __forceinline__ int k_rows(const Params& p) const { return min(max(k_len, 0), p.seq_k); }
+  __device__ __forceinline__ int entries(const Params& p, int t) const {
+    return row0[t] < q_rows(p)
+               ? max(0, min(min(max(count[t], 0), p.list_len) - first[t], most[t]))
+               : 0;
   }
 };
 
@@ -199,8 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar_p = [&](int t, uint32_t buf) { return bars + 8u * (8 + 2 * t + buf); };
   auto bar_pv = [&](int t, uint32_t buf) { return bars + 8u * (12 + 2 * t + buf); };
   const uint32_t bar_fix = bars + 8u * 16;
-  auto bar_full = [&](int s) { return bars + 8u * (17 + s); };
-  auto bar_empty = [&](int s) { return bars + 8u * (17 + kSlots + s); };
+  auto bar_ifull = [&](uint32_t i) { return bars + 8u * (17 + (i & 1)); };
+  auto bar_iempty = [&](uint32_t i) { return bars + 8u * (19 + (i & 1)); };
+  auto bar_full = [&](int s) { return bars + 8u * (21 + s); };
+  auto bar_empty = [&](int s) { return bars + 8u * (21 + kSlots + s); };
+  volatile Info* info = reinterpret_cast<volatile Info*>(smem + L::kSmemInfo);
+  volatile uint8_t* key_ring = smem + L::kSmemKeys;  // [tile][unit % kKeyRing]
+  volatile uint32_t* slot_tag = reinterpret_cast<uint32_t*>(smem + L::kSmemTag);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSmemTail);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
@@ -219,9 +250,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(bar_full(s), 1);
-      mbar_init(bar_empty(s), prm.tiles_per_list);  // the tiles that read a slot
+      slot_tag[s] = 0xffffffffu;
+      mbar_init(bar_empty(s), prm.duo ? 1 : prm.tiles_per_list);  // the tiles that read a slot
     }
     mbar_init(bar_fix, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_ifull(i), 1);
+      mbar_init(bar_iempty(i), kSoftmaxWarps + kTiles);
+    }
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -248,7 +284,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Slots are filled and read in one order; `pos` counts them since the start.
   auto slot_of = [](uint32_t pos) { return (int)(pos % kSlots); };
   auto phase_of = [](uint32_t pos) { return (pos / kSlots) & 1u; };
-  const bool shared = prm.tiles_per_list == kTiles;  // one slot serves both tiles
+  const bool shared = prm.tiles_per_list == kTiles && !prm.duo;  // one slot serves both tiles
+  // The next item of this warp, `i` counting them: read from shared memory, then released.
+  auto take_info = [&](uint32_t i, Info& it) -> bool {
+    if (!wait_all(bar_ifull(i), (i >> 1) & 1)) return false;
+    const volatile Info& src = info[i & 1];
+    it.batch = src.batch;
+    it.head = src.head;
+    it.row0[0] = src.row0[0];
+    it.row0[1] = src.row0[1];
+    it.q_rows = src.q_rows;
+    it.units[0] = src.units[0];
+    it.units[1] = src.units[1];
+    it.part = src.part;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_iempty(i));
+    return true;
+  };
 
   if (warp == kLoadWarp) {
     // ---------------- loads: the whole warp walks, one lane issues ----------------
@@ -261,20 +313,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     struct Walk {
       const int32_t* list;
       int entries, units, e[3], chunk, ahead, base;
+      uint32_t keys_at;  // units handed to the softmax so far
     };
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item it;
-      it.load(prm, item);
+    Walk walk[kTiles];
+    walk[0].keys_at = walk[1].keys_at = 0;
+    Item following;
+    if ((int)blockIdx.x < prm.n_items) following.load(prm, blockIdx.x, lane);
+    uint32_t n_items = 0;
+    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
+      const Item it = following;
+      if (item + (int)gridDim.x < prm.n_items) following.load(prm, item + gridDim.x, lane);
       const int kv_head = it.head / prm.group;
-      Walk walk[kTiles];
-      auto read = [&](Walk& w, int from) { return from + lane < w.entries ? w.list[from + lane] : -1; };
+      const int k_rows = it.k_rows(prm);
       auto entry = [&](Walk& w, int unit) -> int {  // called with ascending units
         const int i = unit / kPer;
         if (i >= w.entries) return -1;
         if (i >= w.base + 32) {
           w.base += 32;
           w.chunk = w.ahead;
-          w.ahead = read(w, w.base + 32);
+          w.ahead = w.base + 32 + lane < w.entries ? w.list[w.base + 32 + lane] : -1;
         }
         return __shfl_sync(0xffffffffu, w.chunk, i & 31);
       };
@@ -282,32 +339,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < kTiles; ++t) {
         Walk& w = walk[t];
         w.list = it.list[t];
-        w.entries = it.entries[t];
+        w.entries = it.entries(prm, t);
         w.units = w.entries * kPer;
         w.base = 0;
-        w.chunk = read(w, 0);
-        w.ahead = read(w, 32);
+        w.chunk = it.chunk[t];
+        w.ahead = it.ahead[t];
         w.e[0] = entry(w, 0);
         w.e[1] = entry(w, 1);
         w.e[2] = entry(w, 2);
       }
-      // The next slot: V of `unit_v` (none below 0) and K of `unit_k` (none from the end on),
-      // or, before the first unit, K of units 0 and 1.
-      auto push = [&](const Walk& w, int unit) -> bool {
+      if (!wait_all(bar_iempty(n_items), ((n_items >> 1) & 1) ^ 1)) break;
+      if (lane == 0) {
+        volatile Info& dst = info[n_items & 1];
+        dst.batch = it.batch;
+        dst.head = it.head;
+        dst.row0[0] = it.row0[0];
+        dst.row0[1] = it.row0[1];
+        dst.q_rows = it.q_rows(prm);
+        dst.units[0] = walk[0].units;
+        dst.units[1] = walk[1].units;
+        dst.part = it.part;
+        mbar_arrive(bar_ifull(n_items));
+      }
+      __syncwarp();
+      // The next slot: V of `unit` and K of unit + 2 (none from the end on), or, with unit -1,
+      // K of units 0 and 1. The keys of the K units go to the softmax of the tiles that read it.
+      auto push = [&](int t, int unit) -> bool {
+        Walk& w = walk[t];
         const bool first = unit < 0;
         const bool two = first ? w.units > 1 : unit + 2 < w.units;  // both parts are there
         int row0, row1;
-        const int keys0 = unit_keys<BK>(w.e[0], first ? 0 : unit, prm.nk, it.k_rows, row0);
-        const int keys1 = first ? unit_keys<BK>(w.e[1], 1, prm.nk, it.k_rows, row1)
-                                : unit_keys<BK>(w.e[2], unit + 2, prm.nk, it.k_rows, row1);
+        const int keys0 = unit_keys<BK>(w.e[0], first ? 0 : unit, prm.nk, k_rows, row0);
+        const int keys1 = first ? unit_keys<BK>(w.e[1], 1, prm.nk, k_rows, row1)
+                                : unit_keys<BK>(w.e[2], unit + 2, prm.nk, k_rows, row1);
         if (keys0 == 0) row0 = prm.seq_k;  // behind the end: zeros
         if (keys1 == 0) row1 = prm.seq_k;
-        const bool cut = !first && keys0 > 0 && keys0 < kUnit && it.k_rows < prm.seq_k;
+        const bool cut = !first && keys0 > 0 && keys0 < kUnit && k_rows < prm.seq_k;
         const int slot = slot_of(pos);
         if (!wait_all(bar_empty(slot), phase_of(pos) ^ 1)) return false;
         const uint32_t dst = sbase + L::kSmemRing + slot * L::kSlotBytes;
         const uint32_t full = bar_full(slot);
+        // Visible to the softmax through this slot's barrier, the MMA warp and its commit.
+        auto hand_keys = [&](Walk& reader, int tile) {
+          if (lane == 0) {
+            if (first) key_ring[tile * kKeyRing + reader.keys_at % kKeyRing] = (uint8_t)keys0;
+            if (two) key_ring[tile * kKeyRing + (reader.keys_at + (first ? 1 : 0)) % kKeyRing] = (uint8_t)keys1;
+          }
+          reader.keys_at += (first ? 1u : 0u) + (two ? 1u : 0u);
+        };
+        hand_keys(w, t);
+        if (shared && walk[1].units > 0) hand_keys(walk[1], 1);
         if (elect_one()) {
+          slot_tag[slot] = pos;
           const uint32_t bar = cut ? bar_fix : full;
           mbar_expect_tx(bar, two ? L::kSlotBytes : L::kPartBytes);
           const CUtensorMap* map0 = first ? &k_map : &v_map;
@@ -353,17 +436,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
             tma_load_4d(dst + h * kQHalf, &q_map, bar_qfull(t), 64 * h, it.head,
-                        (kTiles * it.pair + t) * kTile, it.batch);
+                        it.row0[t], it.batch);
         }
         __syncwarp();
-        if (t == 0 || !shared) ok = push(walk[t], -1);
+        if (t == 0 || !shared) ok = push(t, -1);
       }
       const int units = max(walk[0].units, walk[1].units);
       for (int u = 0; u < units && ok; ++u) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           Walk& w = walk[t];
-          if (u < w.units && ok && (t == 0 || !shared)) ok = push(w, u);
+          if (u < w.units && ok && (t == 0 || !shared)) ok = push(t, u);
           w.e[0] = w.e[1];
           w.e[1] = w.e[2];
           w.e[2] = entry(w, u + 3);
@@ -384,6 +467,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n_s = 0, n_pv = 0;  // units issued so far
     uint32_t q_phase = 0;
     bool ok = true;
+    // Waits for the slot at `at`. With slots of its own a tile never looks at the other's, so
+    // it can be here before the slot's use before this one (the other's) has landed, and the
+    // parity of that phase is the one it would take for its own: the tag comes first.
+    auto wait_slot = [&](uint32_t at) -> bool {
+      const int slot = slot_of(at);
+      if (!shared) {
+        const unsigned long long t0 = globaltimer();
+        while (__any_sync(0xffffffffu, slot_tag[slot] != at)) {
+          const bool late = globaltimer() - t0 > kWaitLimitNs;
+          if (late && lane == 0) {
+            *abort_flag = 1u;
+            if (prm.status) atomicOr(prm.status, kStatusAttentionTimeout);
+          }
+          if (__any_sync(0xffffffffu, late || *abort_flag != 0u)) return false;
+        }
+      }
+      return wait_all(bar_full(slot), phase_of(at));
+    };
     // One lane: S = Q K^T, K being part `part` of the slot.
     auto issue_s = [&](int slot, int part) {
       const uint64_t kd =
@@ -396,10 +497,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mma_commit(bar_s(t, n_s & 1));
     };
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item it;
-      it.load(prm, item);
-      const int units0 = it.entries[0] * kPer, units1 = it.entries[1] * kPer;
+    uint32_t n_items = 0;
+    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
+      Info it;
+      if (!take_info(n_items, it)) break;
+      const int units0 = it.units[0], units1 = it.units[1];
       const int units = t == 0 ? units0 : units1;
       // Where this tile's slots are: its first at base + lead, slot u at `next`, which steps
       // over the other tile's while that has units left.
@@ -416,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (units > 0) {
         const uint32_t first = base + lead;
         const int slot = slot_of(first);
-        ok = wait_all(bar_qfull(t), q_phase) && wait_all(bar_full(slot), phase_of(first));
+        ok = wait_all(bar_qfull(t), q_phase) && wait_slot(first);
         if (!ok) break;
         q_phase ^= 1;
         tc_fence_after();
@@ -436,8 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int u = 0; u < units; ++u) {
         const int slot = slot_of(next);
-        ok = wait_all(bar_full(slot), phase_of(next)) &&
-             wait_all(bar_p(t, n_pv & 1), (n_pv >> 1) & 1);
+        ok = wait_slot(next) && wait_all(bar_p(t, n_pv & 1), (n_pv >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -474,24 +575,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 c2 = make_float2(c, c);
     uint32_t n = 0;  // units so far: buffer n & 1, phase n >> 1
     bool ok = true;
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x) {
-      Item it;
-      it.load(prm, item);
-      const int32_t* list = t == 0 ? it.list[0] : it.list[1];
-      const int entries = t == 0 ? it.entries[0] : it.entries[1];
-      const int units = entries * kPer;
+    uint32_t n_items = 0;
+    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
+      Info it;
+      if (!take_info(n_items, it)) break;
+      const int units = t == 0 ? it.units[0] : it.units[1];
+      const int row = (t == 0 ? it.row0[0] : it.row0[1]) + row_in_tile;
+      const bool live = row < it.q_rows;
+      const bool idle = !__any_sync(0xffffffffu, live);  // no row of this warp exists
       float m_use = -INFINITY;  // running row max, log2 units, that P is taken against
       float l_sum = 0.f;
-      int e_next = entries > 0 ? __ldg(list) : -1;
       for (int u = 0; u < units; ++u, ++n) {
-        int row;
-        const int keys = unit_keys<BK>(e_next, u, prm.nk, it.k_rows, row);
-        if ((u + 1) % kPer == 0 && u + 1 < units) e_next = __ldg(list + (u + 1) / kPer);
         const uint32_t t_s = tmem + lanes + kTmemS + t * 128 + (n & 1) * 64;
         // tcgen05.ld/st below are warp-collective.
         ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
+        if (idle) {
+          // Nobody reads these rows of P V: whatever stands in TMEM will do for P.
+          tc_fence_before();
+          mbar_arrive(bar_p(t, n & 1));
+          continue;
+        }
+        const int keys = key_ring[t * kKeyRing + n % kKeyRing];
         uint32_t sv[2][32];
         tmem_ld32(t_s, sv[0]);
         tmem_ld32(t_s + 32, sv[1]);
@@ -562,11 +668,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && units > 0) ok = wait_all(bar_pv(t, (n - 1) & 1), ((n - 1) >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
-      const int row = (kTiles * it.pair + t) * kTile + row_in_tile;
-      const bool live = row < it.q_rows;
-      if (it.split >= 0) {
-        float* ws = prm.ws + ((int64_t)it.split * kTiles + t) * kWsTileFloats<D>;
-        if (units > 0) {
+      if (it.part >= 0) {
+        float* ws = prm.ws + (int64_t)(it.part + t) * prm.ws_rows * (D + 4);
+        if (units > 0 && !idle) {
 #pragma unroll 1
           for (int q4 = 0; q4 < D / 32; ++q4) {
             uint32_t o[32];
@@ -583,7 +687,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (live)
-          *reinterpret_cast<float2*>(ws + kTile * D + 2 * row_in_tile) = make_float2(m_use, l_sum);
+          *reinterpret_cast<float2*>(ws + prm.ws_rows * D + 2 * row_in_tile) =
+              make_float2(m_use, l_sum);
         continue;
       }
       const bool some = live && l_sum != 0.f;  // the row has a key
@@ -606,18 +711,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
         if (dst != nullptr) {
+          Chunk32 w[2];
+          uint32_t* words = reinterpret_cast<uint32_t*>(w);
 #pragma unroll
-          for (int v8 = 0; v8 < 4; ++v8) {
-            uint4 w;
-            w.x = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 0]) * inv_l,
-                                  __uint_as_float(o[v8 * 8 + 1]) * inv_l);
-            w.y = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 2]) * inv_l,
-                                  __uint_as_float(o[v8 * 8 + 3]) * inv_l);
-            w.z = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 4]) * inv_l,
-                                  __uint_as_float(o[v8 * 8 + 5]) * inv_l);
-            w.w = pack_pair<FP16>(__uint_as_float(o[v8 * 8 + 6]) * inv_l,
-                                  __uint_as_float(o[v8 * 8 + 7]) * inv_l);
-            *reinterpret_cast<uint4*>(dst + 32 * q4 + v8 * 8) = w;
+          for (int i = 0; i < 16; ++i)
+            words[i] = pack_pair<FP16>(__uint_as_float(o[2 * i]) * inv_l,
+                                       __uint_as_float(o[2 * i + 1]) * inv_l);
+          // A thread per row: 32-byte stores are whole sectors, half as many as 16-byte ones.
+          if (prm.wide_out) {
+            st32(dst + 32 * q4, w[0]);
+            st32(dst + 32 * q4 + 16, w[1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              *reinterpret_cast<uint4*>(dst + 32 * q4 + 16 * i) = w[i].lo;
+              *reinterpret_cast<uint4*>(dst + 32 * q4 + 16 * i + 8) = w[i].hi;
+            }
           }
         }
       }
@@ -643,13 +752,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the split pairs: one warp per query row, D/32 columns per lane.
-// O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.
+// O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. Up to kMaxParts parts: lane s holds the
+// max and sum of part s, and the O of four parts is on its way at a time.
+constexpr int kMaxParts = 32;
 template <bool FP16, int D>
 __global__ void __launch_bounds__(256) sparse_combine(const Params prm, int split_pairs) {
   const int gw = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  constexpr int kPairRows = kTiles * kTile;
-  const int pair_rows = min(kPairRows, prm.seq_q);
+  const int pair_rows = min(prm.duo ? kTile : kTiles * kTile, prm.seq_q);
   if (gw >= split_pairs * pair_rows) return;
   const int ui = gw / pair_rows;
   const int rr = gw - ui * pair_rows;
@@ -659,27 +769,39 @@ __global__ void __launch_bounds__(256) sparse_combine(const Params prm, int spli
   const int bh = whole / prm.pairs;
   const int head = bh % prm.heads;
   const int batch = bh / prm.heads;
-  const int row = whole % prm.pairs * kPairRows + rr;
+  const int row = whole % prm.pairs * (kTiles * kTile) + rr;
   if (row >= prm.seq_q) return;
   const bool live = row < rows_of(prm.q_lens, batch, prm.seq_q);
-  auto part = [&](int s) {
-    return prm.ws + ((int64_t)(ui * prm.splits + s) * kTiles + t) * kWsTileFloats<D>;
-  };
+  const int parts = prm.duo ? prm.splits * kTiles : prm.splits;
+  const int64_t part_floats = (int64_t)prm.ws_rows * (D + 4);
+  const int64_t step = prm.duo ? part_floats : part_floats * kTiles;
+  const float* first = prm.ws + (int64_t)ui * prm.splits * kTiles * part_floats + t * part_floats;
   constexpr int kCols = D / 32;
-  float m_max = -INFINITY, l_tot = 0.f, acc[kCols] = {};
-  if (live) {
-    for (int s = 0; s < prm.splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(part(s) + kTile * D + 2 * r_in_tile);
-      m_max = fmaxf(m_max, ml.x);
-    }
-    for (int s = 0; s < prm.splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(part(s) + kTile * D + 2 * r_in_tile);
-      if (ml.y == 0.f) continue;  // a part without keys wrote no O
-      const float w = ex2(ml.x - m_max);
-      l_tot += w * ml.y;
-      const float* o = part(s) + r_in_tile * D + lane * kCols;
+  float acc[kCols] = {};
+  float m = -INFINITY, l = 0.f;
+  if (live && lane < parts) {
+    const float2 ml =
+        *reinterpret_cast<const float2*>(first + lane * step + prm.ws_rows * D + 2 * r_in_tile);
+    m = ml.x;
+    l = ml.y;
+  }
+  float m_max = m;
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) acc[i] += w * o[i];
+  for (int o = 16; o > 0; o >>= 1) m_max = fmaxf(m_max, __shfl_xor_sync(0xffffffffu, m_max, o));
+  // A part without keys wrote no O and has no weight.
+  const float weight = l == 0.f ? 0.f : ex2(m - m_max);
+  const float l_tot = warp_sum(l == 0.f ? 0.f : weight * l);
+  const unsigned with_keys = __ballot_sync(0xffffffffu, l != 0.f);
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float w = __shfl_sync(0xffffffffu, weight, s);
+    if ((with_keys >> s & 1u) == 0u) continue;
+    const float* o = first + s * step + r_in_tile * D + lane * kCols;
+#pragma unroll
+    for (int i = 0; i < kCols; i += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(o + i);
+      acc[i] += w * v.x;
+      acc[i + 1] += w * v.y;
     }
   }
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;
@@ -699,34 +821,41 @@ __global__ void __launch_bounds__(256) sparse_combine(const Params prm, int spli
 // ---------------------------------------------------------------------------
 
 struct Plan {
-  int pairs, total, n_full, splits, entries_per_split, items, split_pairs;
+  int pairs, total, n_full, splits, entries_per_split, items, split_pairs, duo, ws_rows;
   int64_t ws_bytes;
 };
 
 // Whole pairs of tiles fill waves of SMs; when the last wave would leave at least half of
-// them idle, its pairs are split along their lists, down to 128 keys per part.
+// them idle, its pairs are split along their lists, down to 128 keys per part. A query of
+// one tile is split in any case: half a list for each of the two tiles of an item.
 Plan make_plan(int64_t batch, int64_t seq_q, int64_t heads, int64_t head_dim, int64_t block_k,
-               int64_t list_len) {
+               int64_t list_len, bool can_split) {
   Plan pl{};
   pl.pairs = (int)((seq_q + kTiles * kTile - 1) / (kTiles * kTile));
   pl.total = (int)(pl.pairs * heads * batch);
   const int least = (int)(2 * kUnit / block_k);  // entries of 128 keys
   const int parts = (int)((list_len + least - 1) / least);
   const int sms = num_sms();
-  const int rem = pl.total % sms;
+  pl.ws_rows = (int)std::min<int64_t>(kTile, seq_q);
+  // (While the workspace stays within 256 MB; more items than that fill the GPU anyway.)
+  pl.duo = can_split && seq_q <= kTile && parts >= 2 &&
+           (int64_t)pl.total * kTiles * pl.ws_rows * (head_dim + 4) * 4 <= (256ll << 20);
+  const int rem = pl.duo ? pl.total : pl.total % sms;
+  const int each = pl.duo ? kTiles : 1;  // ranges per item
   pl.splits = 1;
   pl.entries_per_split = (int)list_len;
   pl.n_full = pl.items = pl.total;
-  if (rem > 0 && 2 * rem <= sms && parts >= 2) {
-    const int want = std::min(std::min(sms / rem, 32), parts);
+  if (can_split && rem > 0 && parts >= 2 && (pl.duo || 2 * rem <= sms)) {
+    int want = std::min(std::min(std::max(sms / rem, 1) * each, kMaxParts), parts);
     pl.entries_per_split = (parts + want - 1) / want * least;
-    pl.splits = (int)((list_len + pl.entries_per_split - 1) / pl.entries_per_split);
+    want = (int)((list_len + pl.entries_per_split - 1) / pl.entries_per_split);
+    pl.splits = (want + each - 1) / each;
   }
-  if (pl.splits >= 2) {
+  if (pl.duo || pl.splits >= 2) {
     pl.split_pairs = rem;
     pl.n_full = pl.total - rem;
     pl.items = pl.n_full + rem * pl.splits;
-    pl.ws_bytes = (int64_t)rem * pl.splits * kTiles * (kTile * head_dim + 2 * kTile) * 4;
+    pl.ws_bytes = (int64_t)rem * pl.splits * kTiles * pl.ws_rows * (head_dim + 4) * 4;
   } else {
     pl.splits = 1;
     pl.entries_per_split = (int)list_len;
@@ -785,7 +914,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   sparse_fwd<FP16, D, BK><<<grid, kThreads, Layout<D>::kSmemAlloc, stream>>>(qm, km, vm, p);
   int rc = check_launch("h3b_block_sparse_attention");
   if (rc != H3B_OK || split_pairs == 0) return rc;
-  const int rows = split_pairs * std::min(kTiles * kTile, p.seq_q);
+  const int rows = split_pairs * std::min(p.duo ? kTile : kTiles * kTile, p.seq_q);
   sparse_combine<FP16, D><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p, split_pairs);
   return check_launch("h3b_block_sparse_attention");
 }
@@ -816,7 +945,7 @@ extern "C" int h3b_block_sparse_attention_workspace_size(int64_t batch, int64_t 
   if (batch == 0 || seq_q == 0 || heads == 0 || list_len == 0 ||
       !(head_dim == 64 || head_dim == 128) || !(block_k == 64 || block_k == 128))
     return H3B_OK;
-  *bytes_out = h3b::attn::sparse::make_plan(batch, seq_q, heads, head_dim, block_k, list_len).ws_bytes;
+  *bytes_out = h3b::attn::sparse::make_plan(batch, seq_q, heads, head_dim, block_k, list_len, true).ws_bytes;
   return H3B_OK;
 }
 
@@ -877,14 +1006,11 @@ extern "C" int h3b_block_sparse_attention(
   if ((rc = make_map(&vm, v, batch, seq_k, kv_heads, head_dim, v_batch_stride, v_row_stride,
                      v_head_stride, kUnit, fp16, "v")) != H3B_OK)
     return rc;
-  Plan pl = make_plan(batch, seq_q, heads, head_dim, block_k, list_len);
+  Plan pl = make_plan(batch, seq_q, heads, head_dim, block_k, list_len, true);
   if (pl.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < pl.ws_bytes ||
-                          !h3b::aligned16(workspace))) {
+                          !h3b::aligned16(workspace)))
     // No (or too small a) workspace: run every pair whole.
-    pl.splits = 1;
-    pl.split_pairs = 0;
-    pl.n_full = pl.items = pl.total;
-  }
+    pl = make_plan(batch, seq_q, heads, head_dim, block_k, list_len, false);
   Params p{};
   p.out = out;
   p.lse = lse;
@@ -910,6 +1036,10 @@ extern "C" int h3b_block_sparse_attention(
   p.n_full = pl.n_full;
   p.splits = pl.splits;
   p.entries_per_split = pl.entries_per_split;
+  p.duo = pl.duo;
+  p.ws_rows = pl.ws_rows;
+  p.wide_out = h3b::aligned32(out) && (batch == 1 || o_batch_stride % 16 == 0) &&
+               (seq_q == 1 || o_row_stride % 16 == 0) && (heads == 1 || o_head_stride % 16 == 0);
   p.ws = reinterpret_cast<float*>(workspace);
   return fp16 ? launch_dims<true>(head_dim, block_k, qm, km, vm, p, pl.split_pairs, stream)
               : launch_dims<false>(head_dim, block_k, qm, km, vm, p, pl.split_pairs, stream);

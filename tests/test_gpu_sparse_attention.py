@@ -72,7 +72,7 @@ def test_attend(dtype, d, block_q, block_k):
     _check(out, lse, q, k, v, indices, counts, block_q=block_q, block_k=block_k)
 
 
-@pytest.mark.parametrize("sq,sk", [(1, 1), (1, 5000), (2, 64), (128, 127), (129, 129), (255, 65), (257, 1025), (1000, 3)])
+@pytest.mark.parametrize("sq,sk", [(1, 1), (1, 5000), (2, 64), (3, 1300), (33, 3000), (128, 127), (128, 2500), (129, 129), (255, 65), (257, 1025), (1000, 3)])
 @pytest.mark.parametrize("block_k", [64, 128])
 def test_lengths(sq, sk, block_k):
     """From one row and one key; a single query block is split along its list and joined."""
@@ -132,6 +132,26 @@ def test_short_lists_over_and_over(block_q, block_k):
             part = indices[:, :, : 512 // block_q].contiguous()
             n_part = None if counts is None else counts[:, :, : 512 // block_q].contiguous()
             _check(first[:, rows], None, q[:, rows], k, v, part, n_part, block_q=block_q, block_k=block_k)
+
+
+@pytest.mark.parametrize("sq,block_k", [(1, 128), (1, 64), (40, 128), (300, 64)])
+def test_long_lists_over_cold_keys(sq, block_k):
+    """Lists of many units over keys that come from HBM: loads land out of order, and a tile
+    may reach a slot before the other tile's rows in it have landed."""
+
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
+
+    s, h = 60000, 24
+    k, v = _randn((1, s, h, 128), 2), _randn((1, s, h, 128), 3)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    nq, nk = -(-sq // 128), -(-s // block_k)
+    for seed in range(3):
+        q = _randn((1, sq, h, 128), 10 + seed)
+        indices, counts = _lists(1, h, nq, nk, 100, seed)
+        flush.zero_()
+        out, lse = block_sparse_attention(q, k, v, indices, counts, block_k=block_k, return_lse=True)
+        few = slice(0, 3)
+        _check(out[:, :, few], lse[:, few], q[:, :, few], k[:, :, few], v[:, :, few], indices[:, few], counts[:, few], block_k=block_k)
 
 
 @pytest.mark.parametrize("block_k", [64, 128])
