@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // parity of that phase is the one it would take for its own: the tag comes first.
     auto wait_slot = [&](uint32_t at) -> bool {
       const int slot = slot_of(at);
-      if (!shared) {
+      if (!shared && __any_sync(0xffffffffu, slot_tag[slot] != at)) {
         const unsigned long long t0 = globaltimer();
         while (__any_sync(0xffffffffu, slot_tag[slot] != at)) {
           const bool late = globaltimer() - t0 > kWaitLimitNs;
@@ -585,18 +585,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool idle = !__any_sync(0xffffffffu, live);  // no row of this warp exists
       float m_use = -INFINITY;  // running row max, log2 units, that P is taken against
       float l_sum = 0.f;
-      for (int u = 0; u < units; ++u, ++n) {
+      // Nobody reads the rows of a warp without rows: whatever stands in TMEM will do for P.
+      for (int u = 0; idle && u < units; ++u, ++n) {
+        ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
+        if (!ok) break;
+        mbar_arrive(bar_p(t, n & 1));
+      }
+      for (int u = 0; !idle && u < units; ++u, ++n) {
         const uint32_t t_s = tmem + lanes + kTmemS + t * 128 + (n & 1) * 64;
         // tcgen05.ld/st below are warp-collective.
         ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (idle) {
-          // Nobody reads these rows of P V: whatever stands in TMEM will do for P.
-          tc_fence_before();
-          mbar_arrive(bar_p(t, n & 1));
-          continue;
-        }
         const int keys = key_ring[t * kKeyRing + n % kKeyRing];
         uint32_t sv[2][32];
         tmem_ld32(t_s, sv[0]);
