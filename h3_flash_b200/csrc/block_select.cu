@@ -10,12 +10,19 @@
 // of at most 256 16-bit values is summed in fp64 and the products of two fp32 means are
 // exact in fp64, which leaves 2^-52 relative in a score. Two devices, two batch layouts
 // or another summation order then choose alike. Most of it is done in fp32 all the same:
-// only scores too close to the border for fp32 to tell are taken in fp64 (score_select).
+// only scores too close to the border for fp32 to tell are taken in fp64 (block_choose).
 //
-// Two kernels. block_means reads q and k once (bound by HBM: everything else is small);
-// one warp per (block, head), heads of one block in neighbouring warps so that whole rows
-// are read together. score_select holds the scores of up to 16 query blocks in shared
-// memory as order-preserving keys and selects with one warp per row.
+// Three kernels:
+//   block_means   reads q and k once; bound by HBM, and nearly all of the time at long
+//                 sequences. Heads of one block lie next to each other in
+//                 the grid, so that whole rows are read together. Leaves each mean in fp32, its norm, and
+//                 the mean as a sum of two bf16.
+//   block_scores  s in fp32 from the bf16 parts, hi hi + hi mid + mid hi, on the tensor cores
+//                 (mma.sync: a product of a few GFLOP, not worth a tcgen05 pipeline). The
+//                 query heads that share a key head are rows of one product.
+//   block_choose  a warp per query block, its scores in registers: counts them in bins, ranks
+//                 those next to the border. Rows that this does not settle, or of more than
+//                 4096 key blocks, go through the workspace (choose_any).
 #include <cuda_fp16.h>
 
 #include <cstdio>
@@ -27,19 +34,25 @@ namespace select {
 
 constexpr int kMeanWarps = 4;
 
+// Where the means of one side (queries or keys) go: per row, D values each.
+struct Means {
+  float* mean;
+  __nv_bfloat16* hi;
+  __nv_bfloat16* mid;
+  float* norm;
+};
+
 struct MeanSide {
   const void* x;
-  float* mean;  // q: [batch, heads, blocks, D]; k: [batch, heads, D, pitch]
+  Means out;
   int64_t batch_stride, row_stride, head_stride;
   const int32_t* lens;
-  int seq, heads, block, blocks, pitch;
-  bool transposed;
-  int64_t warps;  // batch * blocks * heads
+  int seq, heads, block, blocks;
+  int64_t blocks_total;  // batch * blocks * heads
 };
 
 struct MeanArgs {
   MeanSide side[2];
-  int64_t total;
 };
 
 __device__ __forceinline__ int rows_of(const int32_t* lens, int b, int seq) {
@@ -64,20 +77,24 @@ __device__ __forceinline__ void add8(double (&acc)[8], uint4 u) {
   }
 }
 
-// One warp per (batch, block, head): D/8 lanes hold the columns of a row, the others further rows.
-template <bool FP16, int D>
-__global__ void __launch_bounds__(kMeanWarps * 32) block_means(MeanArgs a) {
-  int64_t w = (int64_t)blockIdx.x * kMeanWarps + (threadIdx.x >> 5);
-  if (w >= a.total) return;
-  const int lane = threadIdx.x & 31;
-  const bool is_k = w >= a.side[0].warps;
+// WARPS warps per (batch, block, head) take turns at its rows: D/8 lanes hold the columns of a
+// row, the others further rows. One warp where there are blocks enough to fill the GPU (24
+// heads of 51,200 rows, 64-key blocks: 105 us, with four 155 us), four for short sequences
+// (4352 rows, three heads: 4.6 us, with one 9.3 us).
+template <bool FP16, int D, int WARPS>
+__global__ void __launch_bounds__(kMeanWarps * 32) block_means(const MeanArgs a) {
+  __shared__ double part[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
+  const int warp = threadIdx.x >> 5 & (WARPS - 1), lane = threadIdx.x & 31;
+  int64_t w = (int64_t)blockIdx.x * (kMeanWarps / WARPS) + (threadIdx.x >> 5) / WARPS;
+  if (w >= a.side[0].blocks_total + a.side[1].blocks_total) return;
+  const bool is_k = w >= a.side[0].blocks_total;
   const MeanSide& s = a.side[is_k ? 1 : 0];
-  if (is_k) w -= a.side[0].warps;
+  if (is_k) w -= a.side[0].blocks_total;
   const int head = (int)(w % s.heads);
   const int block = (int)(w / s.heads % s.blocks);
   const int b = (int)(w / s.heads / s.blocks);
-  constexpr int kLanes = D / 8;          // lanes per row
-  constexpr int kRows = 32 / kLanes;     // rows per load
+  constexpr int kLanes = D / 8;                     // lanes per row
+  constexpr int kRows = 32 / kLanes * WARPS;       // rows per load of these warps
   constexpr int kUnroll = 8;
   const int col = (lane % kLanes) * 8;
   const int row0 = block * s.block;
@@ -86,7 +103,7 @@ __global__ void __launch_bounds__(kMeanWarps * 32) block_means(MeanArgs a) {
   const char* base = (const char*)s.x + 2 * ((int64_t)b * s.batch_stride +
                                              (int64_t)row0 * s.row_stride +
                                              (int64_t)head * s.head_stride + col);
-  for (int r0 = lane / kLanes; r0 < count; r0 += kRows * kUnroll) {
+  for (int r0 = warp * (32 / kLanes) + lane / kLanes; r0 < count; r0 += kRows * kUnroll) {
     uint4 u[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
@@ -100,29 +117,150 @@ __global__ void __launch_bounds__(kMeanWarps * 32) block_means(MeanArgs a) {
   for (int o = 16; o >= kLanes; o >>= 1)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-  if (lane >= kLanes) return;
-  const double n = count > 0 ? (double)count : 1.0;
-  if (s.transposed) {
-    float* out = s.mean + (((int64_t)b * s.heads + head) * D + col) * s.pitch + block;
+  if (WARPS > 1) {
+    if (lane < kLanes) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[(int64_t)j * s.pitch] = (float)(acc[j] / n);
-  } else {
-    float* out = s.mean + (((int64_t)b * s.heads + head) * s.blocks + block) * D + col;
+      for (int j = 0; j < 8; ++j) part[warp][col + j] = acc[j];
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    if (lane < kLanes) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = (float)(acc[j] / n);
+      for (int i = 1; i < WARPS; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += part[i][col + j];
+    }
   }
+  const int64_t out = ((int64_t)b * s.heads + head) * s.blocks + block;
+  double square = 0.0;
+  if (lane < kLanes) {
+    const double n = count > 0 ? (double)count : 1.0;
+    float m[8], hi[8], mid[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = (float)(acc[j] / n);
+      hi[j] = __bfloat162float(__float2bfloat16_rn(m[j]));
+      mid[j] = m[j] - hi[j];
+      square += (double)m[j] * (double)m[j];
+    }
+    float4* mean = reinterpret_cast<float4*>(s.out.mean + out * D + col);
+    mean[0] = make_float4(m[0], m[1], m[2], m[3]);
+    mean[1] = make_float4(m[4], m[5], m[6], m[7]);
+    *reinterpret_cast<uint4*>(s.out.hi + out * D + col) = pack8(hi);
+    *reinterpret_cast<uint4*>(s.out.mid + out * D + col) = pack8(mid);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+  if (lane == 0) s.out.norm[out] = (float)sqrt(square);
 }
 
-struct SelectArgs {
+// ---- scores ---------------------------------------------------------------
+
+constexpr int kScoreM = 64, kScoreN = 128, kScoreThreads = 256;
+
+struct ScoreArgs {
+  Means q, k;
+  float* scores;  // [products][m][pitch]
+  int m, nk, pitch;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes into shared memory, or zeros where the row does not exist.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+
+// A 64 x 128 tile of scores per CTA, eight warps of 32 x 32; the whole depth D of both bf16
+// parts of both operands in shared memory, 16-byte chunks xor-swizzled by row.
+template <int D>
+__global__ void __launch_bounds__(kScoreThreads) block_scores(const ScoreArgs a) {
+  extern __shared__ __align__(128) uint8_t tiles[];
+  constexpr int kRowBytes = 2 * D, kChunks = D / 8;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(tiles);
+  const uint32_t part_a = kScoreM * kRowBytes, part_b = kScoreN * kRowBytes;
+  const uint32_t tile_b = base + 2 * part_a;
+  const int m0 = blockIdx.y * kScoreM, n0 = blockIdx.x * kScoreN;
+  const int64_t product = blockIdx.z;
+  auto at = [&](int row, int chunk) { return row * kRowBytes + ((chunk ^ (row & 7)) << 4); };
+  for (int i = threadIdx.x; i < (kScoreM + kScoreN) * kChunks; i += kScoreThreads) {
+    const int row = i / kChunks, chunk = i % kChunks;
+    const bool is_a = row < kScoreM;
+    const int r = is_a ? m0 + row : n0 + row - kScoreM;
+    const bool there = r < (is_a ? a.m : a.nk);
+    const Means& side = is_a ? a.q : a.k;
+    const int64_t off = there ? (product * (is_a ? a.m : a.nk) + r) * D + chunk * 8 : 0;
+    const uint32_t dst = is_a ? base + at(row, chunk) : tile_b + at(row - kScoreM, chunk);
+    copy16(dst, side.hi + off, there);
+    copy16(dst + (is_a ? part_a : part_b), side.mid + off, there);
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
+  float acc[2][4][4] = {};
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    uint32_t ah[2][4], am[2][4], bh[2][4], bm[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // A: rows 0-15 by two chunks; B: rows (columns of the scores) 0-15 by two chunks.
+      const uint32_t oa = at(wm + 16 * i + (lane & 15), 2 * kk + (lane >> 4));
+      const uint32_t ob = at(wn + 16 * i + (lane & 7) + ((lane >> 4) << 3), 2 * kk + (lane >> 3 & 1));
+      ldmatrix4(base + oa, ah[i]);
+      ldmatrix4(base + part_a + oa, am[i]);
+      ldmatrix4(tile_b + ob, bh[i]);
+      ldmatrix4(tile_b + part_b + ob, bm[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = j >> 1, q = (j & 1) * 2;
+        mma_bf16(acc[i][j], am[i], bh[p][q], bh[p][q + 1]);
+        mma_bf16(acc[i][j], ah[i], bm[p][q], bm[p][q + 1]);
+        mma_bf16(acc[i][j], ah[i], bh[p][q], bh[p][q + 1]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = m0 + wm + 16 * i + 8 * half + lane / 4;
+        if (row < a.m)
+          *reinterpret_cast<float2*>(a.scores + (product * a.m + row) * a.pitch + n0 + wn + 8 * j +
+                                     (lane & 3) * 2) =
+              make_float2(acc[i][j][2 * half], acc[i][j][2 * half + 1]);
+      }
+}
+
+// ---- choice ---------------------------------------------------------------
+
+struct ChooseArgs {
   int32_t* indices;
   int32_t* counts;
-  const float* q_mean;
-  const float* k_mean;
+  Means q, k;
+  uint32_t* scores;  // [rows][pitch]: fp32 scores, overwritten with keys where these do not fit registers
   const int32_t* q_lens;
   const int32_t* k_lens;
   const uint8_t* keep;
-  int heads, kv_heads, seq_q, seq_k, block_q, block_k, nq, nk, pitch, top_k;
-  int row_groups;  // CTAs per (batch, head)
+  int heads, kv_heads, seq_q, seq_k, head_dim, block_q, block_k, nq, nk, pitch, top_k;
+  int64_t rows;  // batch * heads * nq
 };
 
 // Order-preserving keys of a score. -0 and +0 are the same score, NaN ranks as -inf.
@@ -169,376 +307,529 @@ __device__ __forceinline__ unsigned long long kth_key(unsigned long long common,
   return prefix;
 }
 
-template <int D, int ROWS>
-struct SelectShape {
-  static constexpr int kThreads = ROWS == 1 ? 512 : 256;
-  static constexpr int kCols = ROWS == 1 ? 1 : 2;  // columns per thread
-  static constexpr int kWarps = kThreads / 32;
-  // CTAs per SM that registers should allow: three of 16 rows fit in shared memory at 800 columns.
-  static constexpr int kCtas = ROWS == 1 ? 2 : 3;
-};
 constexpr int kBins = 256;
+constexpr int kChooseWarps = 8;
 
-// ROWS query blocks of one (batch, head) per CTA. Scores are first taken in fp32, whose
-// rounding leaves at most E = D 2^-24 |q| max|k| (Cauchy-Schwarz). An order statistic moves
-// by no more than the values do, so with T the k-th largest fp32 score, blocks above T + 2E
-// are in and blocks below T - 2E are out whatever the rounding did; the few between are
-// scored again in fp64 and ranked. A bound that is not finite makes every block one of those.
-template <int D, int ROWS>
-__global__ void __launch_bounds__(SelectShape<D, ROWS>::kThreads, SelectShape<D, ROWS>::kCtas)
-    score_select(SelectArgs a) {
-  using S = SelectShape<D, ROWS>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  float* q_tile = reinterpret_cast<float*>(smem);                 // [D][ROWS]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(q_tile + D * ROWS);  // [ROWS][pitch]
-  __shared__ unsigned int k_square;                               // bits of max |k|^2
-  __shared__ int close[S::kWarps][32];                            // columns to score again
-  __shared__ uint32_t bins[S::kWarps][kBins];
-  const int group = blockIdx.x % a.row_groups;
-  const int64_t bh = blockIdx.x / a.row_groups;
-  const int head = (int)(bh % a.heads);
-  const int b = (int)(bh / a.heads);
-  const int row0 = group * ROWS;
-  const int q_rows = rows_of(a.q_lens, b, a.seq_q);
-  const int k_rows = rows_of(a.k_lens, b, a.seq_k);
-  const int k_blocks = (k_rows + a.block_k - 1) / a.block_k;  // blocks that exist
+// What a warp's row of scores is about.
+struct Row {
+  int64_t list, k_row0;  // which query block, and the first key block of its head
+  int k_blocks, want, kept;  // blocks that exist, places in the list, kept blocks
+  float q_norm, k_norm;      // k_norm: the largest of the blocks that exist
+};
 
-  if (threadIdx.x == 0) k_square = 0u;
-  for (int i = threadIdx.x; i < D * ROWS; i += S::kThreads) {
-    const int r = i / D, d = i % D;
-    q_tile[d * ROWS + r] = row0 + r < a.nq ? a.q_mean[(bh * a.nq + row0 + r) * D + d] : 0.f;
-  }
-  // More kept blocks than a list holds: only they compete, by score.
-  int kept_count = 0;
-  if (a.keep != nullptr)
-    for (int c = threadIdx.x; c < (k_blocks + S::kThreads - 1) / S::kThreads * S::kThreads;
-         c += S::kThreads)
-      kept_count += __syncthreads_count(c < k_blocks && a.keep[c] != 0);
-  const bool only_kept = kept_count > a.top_k;
-  if (only_kept) kept_count = 0;
-  __syncthreads();
-  const float* km = a.k_mean +
-                    ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * D * a.pitch;
-  for (int col = threadIdx.x * S::kCols; col < k_blocks; col += S::kThreads * S::kCols) {
-    if constexpr (S::kCols == 2) {
-      // Columns col, col + 1 (the pitch is even; a column behind the last is scored and
-      // ignored), rows in pairs: a pair of q comes as it lies in shared memory.
-      float2 acc[ROWS / 2][2] = {}, square = make_float2(0.f, 0.f);
-#pragma unroll 8
-      for (int d = 0; d < D; ++d) {
-        const float2 k2 = __ldg(reinterpret_cast<const float2*>(km + (int64_t)d * a.pitch + col));
-        square = __ffma2_rn(k2, k2, square);
-        const float2 first = make_float2(k2.x, k2.x), second = make_float2(k2.y, k2.y);
+// fp64 score of a column as an order-preserving key, the same sum in every lane.
+__device__ __forceinline__ unsigned long long exact_key(const ChooseArgs& a, const Row& r, int c,
+                                                        int lane) {
+  const float* q = a.q.mean + r.list * a.head_dim;
+  const float* k = a.k.mean + (r.k_row0 + c) * a.head_dim;
+  double s = 0.0;
+  for (int d = lane; d < a.head_dim; d += 32) s = fma((double)q[d], (double)k[d], s);
 #pragma unroll
-        for (int r = 0; r < ROWS / 2; r += 2) {
-          const float4 q = *reinterpret_cast<const float4*>(q_tile + d * ROWS + 2 * r);
-          acc[r][0] = __ffma2_rn(make_float2(q.x, q.y), first, acc[r][0]);
-          acc[r][1] = __ffma2_rn(make_float2(q.x, q.y), second, acc[r][1]);
-          acc[r + 1][0] = __ffma2_rn(make_float2(q.z, q.w), first, acc[r + 1][0]);
-          acc[r + 1][1] = __ffma2_rn(make_float2(q.z, q.w), second, acc[r + 1][1]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = col + i;
-        if (c >= k_blocks) continue;
-        const bool kept = a.keep != nullptr && a.keep[c] != 0;
-        if (kept || !only_kept) atomicMax(&k_square, __float_as_uint(i == 0 ? square.x : square.y));
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-          keys[r * a.pitch + c] =
-              only_kept && !kept ? 0u
-              : kept && !only_kept ? kInKey
-                                   : score_key(r % 2 == 0 ? acc[r / 2][i].x : acc[r / 2][i].y);
-      }
-    } else {
-      float acc[ROWS] = {}, square = 0.f;
-#pragma unroll 32
-      for (int d = 0; d < D; ++d) {
-        const float k1 = __ldg(km + (int64_t)d * a.pitch + col);
-        square = fmaf(k1, k1, square);
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[r] = fmaf(q_tile[d * ROWS + r], k1, acc[r]);
-      }
-      const bool kept = a.keep != nullptr && a.keep[col] != 0;
-      if (kept || !only_kept) atomicMax(&k_square, __float_as_uint(square));
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r)
-        keys[r * a.pitch + col] = only_kept && !kept ? 0u
-                                  : kept && !only_kept ? kInKey : score_key(acc[r]);
-    }
-  }
-  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return score_key(s);
+}
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The bound on the difference of two scores from their fp32 values, 2E with
+//   E = 1e-4 |q| max|k| + 1e-35:
+// dropping mid mid and what two bf16 leave of a mean, 3 2^-18 of |q| |k| (Cauchy-Schwarz);
+// 384 products summed in fp32, 2^-23 each if every addition truncates; products below fp32's
+// range. Infinite where it does not hold: norms beyond fp32, and means too small for two bf16
+// to hold their digits.
+__device__ __forceinline__ float twice_error(const Row& r) {
+  const bool sound = (r.q_norm >= 1e-30f || r.q_norm == 0.f) && (r.k_norm >= 1e-30f || r.k_norm == 0.f);
+  return sound ? 2.02e-4f * r.q_norm * r.k_norm + 2e-35f : INFINITY;
+}
+
+// Any row: keys of the scores in the workspace, where each lane reads and writes columns
+// lane, lane + 32, ... only. Returns how many blocks it listed.
+__device__ __noinline__ int choose_any(const ChooseArgs& a, const Row& r, uint32_t* bins,
+                                       int* close, int lane) {
   const unsigned below = (1u << lane) - 1u;
-  for (int r = warp; r < ROWS; r += S::kWarps) {
-    if (row0 + r >= a.nq) break;
-    uint32_t* row = keys + r * a.pitch;
-    const int64_t list = bh * a.nq + row0 + r;
-    int32_t* out = a.indices + list * a.top_k;
-    const bool exists = (row0 + r) * a.block_q < q_rows;
-    const int want = exists ? min(a.top_k, k_blocks) : 0;
-    // Calls f(column) for every lane's columns, warp-uniformly: a column >= k_blocks has no key.
-    auto each = [&](auto f) {
-      for (int c = lane; c < k_blocks; c += 32) f(c);
-    };
-    uint32_t least_in = kInKey;  // keys from here on are in
-    if (want > kept_count) {
-      // T, the k-th largest score: count the scores in equal bins of their range, go on
-      // inside the bin that holds the k-th, rank what is left when a warp holds it. The bin
-      // of a score never decreases with it, whatever the rounding.
-      float low = -INFINITY, high = INFINITY;
-      int left = want - kept_count;  // the rank of T among the scores in [low, high]
-      uint32_t kth;
-      for (;;) {
-        uint32_t least = kInKey, most = 0u;
-        int n = 0;
-        const uint32_t low_key = score_key(low), high_key = score_key(high);
-        each([&](int c) {
-          const uint32_t k = row[c];
-          if (k >= low_key && k <= high_key) {
-            least = min(least, k);
-            most = max(most, k);
-            ++n;
-          }
-        });
-        least = __reduce_min_sync(0xffffffffu, least);
-        most = __reduce_max_sync(0xffffffffu, most);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (least == most || left == n) {
-          kth = least;
-          break;
-        }
-        if (left == 1) {
-          kth = most;
-          break;
-        }
-        if (n <= 32) {
-          int at = 0;
-          for (int c0 = 0; c0 < k_blocks; c0 += 32) {
-            const uint32_t k = c0 + lane < k_blocks ? row[c0 + lane] : 0u;
-            const bool mine = k >= least && k <= most;
-            const unsigned mask = __ballot_sync(0xffffffffu, mine);
-            if (mine) bins[warp][at + __popc(mask & below)] = k;
-            at += __popc(mask);
-          }
-          __syncwarp();
-          const uint32_t mine = lane < n ? bins[warp][lane] : 0u;
-          int rank = 0;
-          for (int i = 0; i < n; ++i) {
-            const uint32_t k = __shfl_sync(0xffffffffu, mine, i);
-            rank += k > mine || (k == mine && i < lane);
-          }
-          const unsigned found = __ballot_sync(0xffffffffu, lane < n && rank == left - 1);
-          kth = __shfl_sync(0xffffffffu, mine, __ffs((int)found) - 1);
-          __syncwarp();
-          break;
-        }
-        low = key_score(least);
-        high = key_score(most);
-        const float span = high - low;
-        const float scale = (float)kBins / span;
-        // A range too wide or too narrow for fp32: every block is scored again in fp64.
-        if (!(span < INFINITY) || !(scale < INFINITY)) {
-          kth = 0u;
-          break;
-        }
-        auto bin_of = [&](uint32_t k) { return min((int)((key_score(k) - low) * scale), kBins - 1); };
-        for (int i = lane; i < kBins; i += 32) bins[warp][i] = 0u;
-        __syncwarp();
-        each([&](int c) {
-          const uint32_t k = row[c];
-          if (k >= least && k <= most) atomicAdd(&bins[warp][bin_of(k)], 1u);
-        });
-        __syncwarp();
-        // Lane l sums bins [8l, 8l + 8); from the top, the lane and then the bin that reach `left`.
-        uint32_t mine[kBins / 32];
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBins / 32; ++i) {
-          mine[i] = bins[warp][lane * (kBins / 32) + i];
-          sum += (int)mine[i];
-        }
-        int up = sum;  // scores in this lane's bins and above
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int other = __shfl_down_sync(0xffffffffu, up, o);
-          if (lane + o < 32) up += other;
-        }
-        const unsigned reach = __ballot_sync(0xffffffffu, up >= left);
-        const int owner = 31 - __clz((int)reach);
-        int bin = 0, over = up - sum;
-        if (lane == owner) {
-          bool done = false;
-#pragma unroll
-          for (int i = kBins / 32 - 1; i >= 0; --i) {
-            if (!done && over + (int)mine[i] >= left) {
-              bin = lane * (kBins / 32) + i;
-              done = true;
-            }
-            if (!done) over += (int)mine[i];
-          }
-        }
-        bin = __shfl_sync(0xffffffffu, bin, owner);
-        left -= __shfl_sync(0xffffffffu, over, owner);
-        // The bin's own range.
-        uint32_t bin_least = kInKey, bin_most = 0u;
-        each([&](int c) {
-          const uint32_t k = row[c];
-          if (k >= least && k <= most && bin_of(k) == bin) {
-            bin_least = min(bin_least, k);
-            bin_most = max(bin_most, k);
-          }
-        });
-        low = key_score(__reduce_min_sync(0xffffffffu, bin_least));
-        high = key_score(__reduce_max_sync(0xffffffffu, bin_most));
-        __syncwarp();
-      }
-      float q_square = 0.f;
-      for (int d = lane; d < D; d += 32) q_square += q_tile[d * ROWS + r] * q_tile[d * ROWS + r];
-      q_square = warp_sum(q_square);
-      // 2E, rounded up: D 2^-23 sqrt(|q|^2 |k|^2), 1% for the rounding of the norms, and the
-      // underflow of D products.
-      const float twice = 1.01f * D * 1.1920929e-7f * sqrtf(q_square) *
-                              sqrtf(__uint_as_float(k_square)) + 1.2e-38f;
-      const float t = key_score(kth);
-      const bool bounded = kth != 0u && twice < INFINITY && fabsf(t) < INFINITY;
-      const uint32_t hi = bounded ? score_key(__fadd_ru(t, twice)) : kInKey - 1u;
-      const uint32_t lo = bounded ? score_key(__fadd_rd(t, -twice)) : 1u;
-      int n_in = 0, n_close = 0;
-      for (int c0 = 0; c0 < k_blocks; c0 += 32) {
-        const int c = c0 + lane;
-        const uint32_t k = c < k_blocks ? row[c] : 0u;
-        const bool is_close = k >= lo && k <= hi;
-        const unsigned mask = __ballot_sync(0xffffffffu, is_close);
-        if (is_close) {
-          const int at = n_close + __popc(mask & below);
-          if (at < 32) close[warp][at] = c;
-        }
-        n_close += __popc(mask);
-        n_in += __popc(__ballot_sync(0xffffffffu, k > hi));
-      }
-      __syncwarp();
-      const int open = want - n_in;  // places left for the close ones
-      least_in = hi == kInKey ? kInKey : hi + 1u;
-      if (n_close == open) {
-        least_in = lo;
-      } else {
-        // fp64 score of a column, the same sum in every lane.
-        auto score = [&](int c) -> unsigned long long {
-          double s = 0.0;
-          for (int d = lane; d < D; d += 32)
-            s = fma((double)q_tile[d * ROWS + r], (double)km[(int64_t)d * a.pitch + c], s);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          return score_key(s);
-        };
-        if (n_close <= 32) {
-          unsigned long long mine = 0ull;
-          for (int i = 0; i < n_close; ++i) {
-            const unsigned long long s = score(close[warp][i]);
-            if (i == lane) mine = s;
-          }
-          int rank = 0;  // close[] ascends: of equal scores the lower lane goes first
-          for (int i = 0; i < n_close; ++i) {
-            const unsigned long long s = __shfl_sync(0xffffffffu, mine, i);
-            rank += s > mine || (s == mine && i < lane);
-          }
-          if (lane < n_close) row[close[warp][lane]] = rank < open ? kInKey : 0u;
-        } else {
-          // Many scores within the bound (equal blocks, say): the same search on fp64 keys,
-          // which are computed again in every pass.
-          auto each_close = [&](auto f) {
-            for (int c0 = 0; c0 < k_blocks; c0 += 32) {
-              const uint32_t k = c0 + lane < k_blocks ? row[c0 + lane] : 0u;
-              unsigned mask = __ballot_sync(0xffffffffu, k >= lo && k <= hi);
-              for (; mask != 0u; mask &= mask - 1u) {
-                const int c = c0 + __ffs((int)mask) - 1;
-                f(c, score(c));
-              }
-            }
-          };
-          unsigned long long one = 0ull, zero = 0ull;
-          each_close([&](int, unsigned long long s) {
-            one |= s;
-            zero |= ~s;
-          });
-          const int top = 63 - __clzll((long long)(one & zero));  // -1: all equal
-          const unsigned long long same64 = top >= 63 ? 0ull : ~((2ull << top) - 1ull);
-          int above64;
-          unsigned long long decided64;
-          const unsigned long long prefix64 = kth_key(
-              one & (top < 0 ? ~0ull : same64), top, n_close, open, above64, decided64,
-              [&](unsigned long long key, unsigned long long mask) {
-                int n = 0;
-                each_close([&](int, unsigned long long s) { n += (s & mask) == key; });
-                return n;
-              });
-          int ties = open - above64;
-          each_close([&](int c, unsigned long long s) {
-            const unsigned long long high = s & decided64;
-            const bool in = high > prefix64 || (high == prefix64 && ties-- > 0);
-            if (lane == (c & 31)) row[c] = in ? kInKey : 0u;
-          });
-        }
-        __syncwarp();
-      }
-    }
-    int done = 0;
-    for (int c0 = 0; c0 < k_blocks && done < want; c0 += 32) {
-      const int c = c0 + lane;
-      const bool take = c < k_blocks && row[c] >= least_in;
-      const unsigned mask = __ballot_sync(0xffffffffu, take);
-      if (take) out[done + __popc(mask & below)] = c;
-      done += __popc(mask);
-    }
-    for (int c = done + lane; c < a.top_k; c += 32) out[c] = -1;
-    if (lane == 0) a.counts[list] = done;
+  const int k_blocks = r.k_blocks, want = r.want;
+  int32_t* out = a.indices + r.list * a.top_k;
+  uint32_t* row = a.scores + r.list * a.pitch;
+  // More kept blocks than a list holds: only they compete, by score.
+  const bool only_kept = r.kept > a.top_k;
+  const int kept = only_kept ? 0 : r.kept;
+  for (int c = lane; c < k_blocks; c += 32) {
+    const bool keep = a.keep != nullptr && a.keep[c] != 0;
+    row[c] = only_kept && !keep ? 0u
+             : keep && !only_kept ? kInKey : score_key(__uint_as_float(row[c]));
   }
+  // f(column, key) for all columns; a column behind the last block has key 0.
+  auto each_column = [&](auto f) {
+#pragma unroll 4
+    for (int c0 = 0; c0 < k_blocks; c0 += 32) f(c0 + lane, c0 + lane < k_blocks ? row[c0 + lane] : 0u);
+  };
+  auto each = [&](auto f) { each_column([&](int, uint32_t k) { f(k); }); };
+  uint32_t least_in = kInKey;  // keys from here on are in
+  int done = 0;
+  if (want > kept) {
+    // T, the k-th largest score: count the scores in equal bins of their range, go on
+    // inside the bin that holds the k-th, rank what is left when a warp holds it. The bin
+    // of a score never decreases with it, whatever the rounding.
+    float low = -INFINITY, high = INFINITY;
+    int left = want - kept;  // the rank of T among the scores in [low, high]
+    uint32_t kth;
+    for (;;) {
+      uint32_t least = kInKey, most = 0u;
+      int n = 0;
+      const uint32_t low_key = score_key(low), high_key = score_key(high);
+      each([&](uint32_t k) {
+        if (k >= low_key && k <= high_key) {
+          least = min(least, k);
+          most = max(most, k);
+          ++n;
+        }
+      });
+      least = __reduce_min_sync(0xffffffffu, least);
+      most = __reduce_max_sync(0xffffffffu, most);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (least == most || left == n) {
+        kth = least;
+        break;
+      }
+      if (left == 1) {
+        kth = most;
+        break;
+      }
+      if (n <= 32) {
+        int at = 0;
+        each([&](uint32_t k) {
+          const bool mine = k >= least && k <= most;
+          const unsigned mask = __ballot_sync(0xffffffffu, mine);
+          if (mine) bins[at + __popc(mask & below)] = k;
+          at += __popc(mask);
+        });
+        __syncwarp();
+        const uint32_t mine = lane < n ? bins[lane] : 0u;
+        int rank = 0;
+        for (int i = 0; i < n; ++i) {
+          const uint32_t k = __shfl_sync(0xffffffffu, mine, i);
+          rank += k > mine || (k == mine && i < lane);
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, lane < n && rank == left - 1);
+        kth = __shfl_sync(0xffffffffu, mine, __ffs((int)found) - 1);
+        __syncwarp();
+        break;
+      }
+      low = key_score(least);
+      high = key_score(most);
+      const float span = high - low;
+      const float scale = (float)kBins / span;
+      // A range too wide or too narrow for fp32: every block is scored again in fp64.
+      if (!(span < INFINITY) || !(scale < INFINITY)) {
+        kth = 0u;
+        break;
+      }
+      auto bin_of = [&](uint32_t k) { return min((int)((key_score(k) - low) * scale), kBins - 1); };
+      for (int i = lane; i < kBins; i += 32) bins[i] = 0u;
+      __syncwarp();
+      each([&](uint32_t k) {
+        if (k >= least && k <= most) atomicAdd(&bins[bin_of(k)], 1u);
+      });
+      __syncwarp();
+      // Lane l sums bins [8l, 8l + 8); from the top, the lane and then the bin that reach `left`.
+      uint32_t mine[kBins / 32];
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < kBins / 32; ++i) {
+        mine[i] = bins[lane * (kBins / 32) + i];
+        sum += (int)mine[i];
+      }
+      int up = sum;  // scores in this lane's bins and above
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_down_sync(0xffffffffu, up, o);
+        if (lane + o < 32) up += other;
+      }
+      const unsigned reach = __ballot_sync(0xffffffffu, up >= left);
+      const int owner = 31 - __clz((int)reach);
+      int bin = 0, over = up - sum;
+      if (lane == owner) {
+        bool done = false;
+#pragma unroll
+        for (int i = kBins / 32 - 1; i >= 0; --i) {
+          if (!done && over + (int)mine[i] >= left) {
+            bin = lane * (kBins / 32) + i;
+            done = true;
+          }
+          if (!done) over += (int)mine[i];
+        }
+      }
+      bin = __shfl_sync(0xffffffffu, bin, owner);
+      left -= __shfl_sync(0xffffffffu, over, owner);
+      // The bin's own range.
+      uint32_t bin_least = kInKey, bin_most = 0u;
+      each([&](uint32_t k) {
+        if (k >= least && k <= most && bin_of(k) == bin) {
+          bin_least = min(bin_least, k);
+          bin_most = max(bin_most, k);
+        }
+      });
+      low = key_score(__reduce_min_sync(0xffffffffu, bin_least));
+      high = key_score(__reduce_max_sync(0xffffffffu, bin_most));
+      __syncwarp();
+    }
+    const float twice = twice_error(r);
+    const float t = key_score(kth);
+    const bool bounded = kth != 0u && twice < INFINITY && fabsf(t) < INFINITY;
+    const uint32_t hi = bounded ? score_key(__fadd_ru(t, twice)) : kInKey - 1u;
+    const uint32_t lo = bounded ? score_key(__fadd_rd(t, -twice)) : 1u;
+    int n_in = 0, n_close = 0;
+    each_column([&](int c, uint32_t k) {
+      const bool is_close = k >= lo && k <= hi;
+      const unsigned mask = __ballot_sync(0xffffffffu, is_close);
+      if (is_close) {
+        const int at = n_close + __popc(mask & below);
+        if (at < 32) close[at] = c;
+      }
+      n_close += __popc(mask);
+      n_in += __popc(__ballot_sync(0xffffffffu, k > hi));
+    });
+    __syncwarp();
+    const int open = want - n_in;  // places left for the close ones
+    least_in = hi + 1u;
+    if (n_close == open) {
+      least_in = lo;
+    } else {
+      auto score = [&](int c) { return exact_key(a, r, c, lane); };
+      if (n_close <= 32) {
+        unsigned long long mine = 0ull;
+        for (int i = 0; i < n_close; ++i) {
+          const unsigned long long s = score(close[i]);
+          if (i == lane) mine = s;
+        }
+        int rank = 0;  // close[] ascends: of equal scores the lower lane goes first
+        for (int i = 0; i < n_close; ++i) {
+          const unsigned long long s = __shfl_sync(0xffffffffu, mine, i);
+          rank += s > mine || (s == mine && i < lane);
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, lane < n_close && rank < open);
+        for (int i = 0; i < n_close; ++i) {
+          const int c = close[i];
+          if (lane == (c & 31)) row[c] = (in >> i & 1u) ? kInKey : 0u;
+        }
+      } else {
+        // Many scores within the bound (equal blocks, say): a search on fp64 keys, which are
+        // computed again in every pass.
+        auto each_close = [&](auto f) {
+          each_column([&](int c0, uint32_t k) {
+            unsigned mask = __ballot_sync(0xffffffffu, k >= lo && k <= hi);
+            for (; mask != 0u; mask &= mask - 1u) {
+              const int c = c0 - lane + __ffs((int)mask) - 1;
+              f(c, score(c));
+            }
+          });
+        };
+        unsigned long long one = 0ull, zero = 0ull;
+        each_close([&](int, unsigned long long s) {
+          one |= s;
+          zero |= ~s;
+        });
+        const int top = 63 - __clzll((long long)(one & zero));  // -1: all equal
+        const unsigned long long same64 = top >= 63 ? 0ull : ~((2ull << top) - 1ull);
+        int above64;
+        unsigned long long decided64;
+        const unsigned long long prefix64 = kth_key(
+            one & (top < 0 ? ~0ull : same64), top, n_close, open, above64, decided64,
+            [&](unsigned long long key, unsigned long long mask) {
+              int n = 0;
+              each_close([&](int, unsigned long long s) { n += (s & mask) == key; });
+              return n;
+            });
+        int ties = open - above64;
+        each_close([&](int c, unsigned long long s) {
+          const unsigned long long high = s & decided64;
+          const bool in = high > prefix64 || (high == prefix64 && ties-- > 0);
+          if (lane == (c & 31)) row[c] = in ? kInKey : 0u;
+        });
+      }
+    }
+  }
+  each_column([&](int c, uint32_t k) {
+    const bool take = k >= least_in;
+    const unsigned mask = __ballot_sync(0xffffffffu, take);
+    if (take) out[done + __popc(mask & below)] = c;
+    done += __popc(mask);
+  });
+  return done;
 }
 
-constexpr int kMaxKeyBlocks = 24576;  // scores of one query block fit in shared memory
-
-size_t select_smem(int head_dim, int rows, int64_t pitch) {
-  return 4 * (size_t)rows * (head_dim + pitch);
+// A row of at most 32 KEYS finite scores, KEYS columns in the registers of each lane: counts
+// them in bins of their range, gathers the bin that holds the k-th and its neighbours, and
+// ranks these, one a lane. Returns -1 where that does not settle it (scores bunched in a bin,
+// all alike, a border wider than a bin): choose_any does.
+template <int KEYS>
+__device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, uint32_t* bins,
+                                           int* columns, float* values, int* gathered, int lane) {
+  constexpr float kBig = 3.4028235e38f;  // above every score: in; -kBig: out
+  const float* row = reinterpret_cast<const float*>(a.scores) + r.list * a.pitch;
+  const int c0 = lane * KEYS;
+  const float twice = twice_error(r);
+  float v[KEYS];
+  float low = kBig, high = -kBig;
+#pragma unroll
+  for (int i = 0; i < KEYS; i += 4) {
+    const float4 s = c0 + i < a.pitch ? __ldcg(reinterpret_cast<const float4*>(row + c0 + i))
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[i] = s.x;
+    v[i + 1] = s.y;
+    v[i + 2] = s.z;
+    v[i + 3] = s.w;
+  }
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) {
+    const int c = c0 + i;
+    if (c >= r.k_blocks) {
+      v[i] = -kBig;
+    } else if (r.kept > 0 && a.keep[c] != 0) {
+      v[i] = kBig;
+    } else {
+      low = fminf(low, v[i]);
+      high = fmaxf(high, v[i]);
+    }
+  }
+  float cut = 0.f;  // scores above are in
+  if (r.want == r.kept || r.want == r.k_blocks) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      v[i] = v[i] == kBig || (r.want == r.k_blocks && c0 + i < r.k_blocks) ? kBig : -kBig;
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    const float scale = 255.8f / (high - low);
+    // (An error below 1e30 keeps every score well below the marks.)
+    if (!(twice < 1e30f) || !(scale < 1e30f) || !(scale > 1e-30f)) return -1;
+    const float shift = 0.1f - low * scale;
+    // Never decreases with the score; the marks fall outside.
+    auto bin_of = [&](float s) { return __float2int_rd(fmaf(s, scale, shift)); };
+#pragma unroll
+    for (int i = 0; i < kBins / 32; ++i) bins[32 * i + lane] = 0u;
+    if (lane == 0) *gathered = 0;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int bin = bin_of(v[i]);
+      if ((unsigned)bin < (unsigned)kBins) atomicAdd(&bins[bin], 1u);
+    }
+    __syncwarp();
+    // From the top, the bin that reaches the k-th: lane l looks at bins [8l, 8l + 8).
+    const int left = r.want - r.kept;
+    int mine[kBins / 32], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kBins / 32; ++i) {
+      mine[i] = (int)bins[lane * (kBins / 32) + i];
+      sum += mine[i];
+    }
+    int up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_down_sync(0xffffffffu, up, o);
+      if (lane + o < 32) up += other;
+    }
+    const int total = __shfl_sync(0xffffffffu, up, 0);
+    if (total != r.k_blocks - r.kept) return -1;  // (a score that rounded out of the bins)
+    const unsigned reach = __ballot_sync(0xffffffffu, up >= left);
+    const int owner = 31 - __clz((int)reach);
+    int bin = 0, over = up - sum;
+    if (lane == owner) {
+      bool found = false;
+#pragma unroll
+      for (int i = kBins / 32 - 1; i >= 0; --i) {
+        if (!found && over + mine[i] >= left) {
+          bin = lane * (kBins / 32) + i;
+          found = true;
+        }
+        if (!found) over += mine[i];
+      }
+    }
+    bin = __shfl_sync(0xffffffffu, bin, owner);
+    over = __shfl_sync(0xffffffffu, over, owner);  // scores in the bins above
+    const int next = bin + 1 < kBins ? (int)bins[bin + 1] : 0;
+    const int n = next + (int)bins[bin] + (bin > 0 ? (int)bins[bin - 1] : 0);
+    if (n > 32) return -1;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      if ((unsigned)bin_of(v[i]) - (unsigned)bin + 1u < 3u) {
+        const int at = atomicAdd(gathered, 1);
+        columns[at] = c0 + i;
+        values[at] = v[i];
+      }
+    }
+    __syncwarp();
+    const int my_column = lane < n ? columns[lane] : 0x7fffffff;
+    const float my_value = lane < n ? values[lane] : -kBig;
+    int rank = 0;
+    for (int i = 0; i < n; ++i) {
+      const float s = values[i];
+      rank += s > my_value || (s == my_value && columns[i] < my_column);
+    }
+    const int first = over - next;  // scores above all that were gathered
+    const unsigned kth = __ballot_sync(0xffffffffu, lane < n && rank == left - first - 1);
+    const float t = __shfl_sync(0xffffffffu, my_value, __ffs((int)kth) - 1);
+    const float hi = __fadd_ru(t, twice), lo = __fadd_rd(t, -twice);
+    // All that is close has to be among the gathered.
+    if ((bin > 0 && bin_of(lo) < bin - 1) || (bin + 1 < kBins && bin_of(hi) > bin + 1)) return -1;
+    const unsigned near = __ballot_sync(0xffffffffu, lane < n && my_value >= lo && my_value <= hi);
+    const int open = left - first - __popc(__ballot_sync(0xffffffffu, lane < n && my_value > hi));
+    if (__popc(near) == open) {
+      cut = lo;
+      // (>= lo below: take the next value down as the cut.)
+      cut = __int_as_float(__float_as_int(cut) + (cut > 0.f ? -1 : 1));
+      if (lo == 0.f) cut = -1e-45f;
+    } else {
+      unsigned long long exact = 0ull;
+      for (unsigned m = near; m != 0u; m &= m - 1u) {
+        const int i = __ffs((int)m) - 1;
+        const unsigned long long s = exact_key(a, r, columns[i], lane);
+        if (lane == i) exact = s;
+      }
+      int exact_rank = 0;
+      for (unsigned m = near; m != 0u; m &= m - 1u) {
+        const int i = __ffs((int)m) - 1;
+        const unsigned long long s = __shfl_sync(0xffffffffu, exact, i);
+        exact_rank += s > exact || (s == exact && columns[i] < my_column);
+      }
+      const unsigned in = __ballot_sync(0xffffffffu, (near >> lane & 1u) && exact_rank < open);
+      for (unsigned m = near; m != 0u; m &= m - 1u) {
+        const int i = __ffs((int)m) - 1;
+        const int at = columns[i] - c0;
+        const float mark = (in >> i & 1u) ? kBig : -kBig;
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j)
+          if (j == at) v[j] = mark;
+      }
+      cut = hi;
+    }
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) count += v[i] > cut;
+  int before = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += other;
+  }
+  const int done = __shfl_sync(0xffffffffu, before, 31);
+  int32_t* out = a.indices + r.list * a.top_k + (before - count);
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i)
+    if (v[i] > cut) *out++ = c0 + i;
+  return done;
 }
 
-template <int D, int ROWS>
-int launch_select(const SelectArgs& a, int64_t batch, size_t smem, cudaStream_t s) {
+// A warp per query block. An order statistic moves by no more than the values do: with T the
+// k-th largest fp32 score and E its error (twice_error), blocks above T + 2E are in and blocks
+// below T - 2E are out whatever the rounding did; the few between are scored again in fp64 and
+// ranked.
+template <int KEYS>
+__global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseArgs a) {
+  __shared__ uint32_t bins[kChooseWarps][kBins];
+  __shared__ int columns[kChooseWarps][32];
+  __shared__ float values[kChooseWarps][32];
+  __shared__ int gathered[kChooseWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Row r;
+  r.list = (int64_t)blockIdx.x * kChooseWarps + warp;
+  if (r.list >= a.rows) return;
+  const int block = (int)(r.list % a.nq);
+  const int head = (int)(r.list / a.nq % a.heads);
+  const int b = (int)(r.list / a.nq / a.heads);
+  r.k_row0 = ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * a.nk;
+  r.k_blocks = (rows_of(a.k_lens, b, a.seq_k) + a.block_k - 1) / a.block_k;
+  r.want = block * a.block_q < rows_of(a.q_lens, b, a.seq_q) ? min(a.top_k, r.k_blocks) : 0;
+  r.kept = 0;
+  int done = 0;
+  if (r.want > 0) {
+    uint32_t norm = 0u;  // bits of max |k|: they order like the values, NaN above all
+    for (int c = lane; c < r.k_blocks; c += 32)
+      norm = max(norm, __float_as_uint(a.k.norm[r.k_row0 + c]));
+    if (a.keep != nullptr) {
+      for (int c = lane; c < r.k_blocks; c += 32) r.kept += a.keep[c] != 0;
+      r.kept = __reduce_add_sync(0xffffffffu, r.kept);
+    }
+    r.k_norm = __uint_as_float(__reduce_max_sync(0xffffffffu, norm));
+    r.q_norm = a.q.norm[r.list];
+    done = -1;
+    if constexpr (KEYS > 0) {
+      if (r.kept <= r.want)
+        done = choose_fast<KEYS>(a, r, bins[warp], columns[warp], values[warp], &gathered[warp], lane);
+    }
+    if (done < 0) {
+      __syncwarp();
+      done = choose_any(a, r, bins[warp], columns[warp], lane);
+    }
+  }
+  int32_t* out = a.indices + r.list * a.top_k;
+  for (int c = done + lane; c < a.top_k; c += 32) out[c] = -1;
+  if (lane == 0) a.counts[r.list] = done;
+}
+
+// ---- host side --------------------------------------------------------------
+
+struct Sizes {
+  int64_t q_rows, k_rows, pitch, scores_at, bytes;
+};
+Sizes sizes_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t nq,
+               int64_t nk) {
+  Sizes s;
+  s.q_rows = batch * heads * nq;
+  s.k_rows = batch * kv_heads * nk;
+  s.pitch = (nk + kScoreN - 1) / kScoreN * kScoreN;
+  // Per row: D fp32, D + D bf16, a norm (rounded up so that every part starts on 16 bytes).
+  s.scores_at = (s.q_rows + s.k_rows) * head_dim * 8 + ((s.q_rows + s.k_rows) * 4 + 31) / 16 * 16;
+  s.bytes = s.scores_at + s.q_rows * s.pitch * 4;
+  return s;
+}
+
+template <int KEYS>
+int launch_choose(const ChooseArgs& a, cudaStream_t s) {
+  block_choose<KEYS><<<(unsigned)((a.rows + kChooseWarps - 1) / kChooseWarps),
+                          kChooseWarps * 32, 0, s>>>(a);
+  return check_launch("h3b_select_key_blocks");
+}
+
+template <bool FP16, int D>
+int launch_all(const MeanArgs& m, const ScoreArgs& sc, const ChooseArgs& a, int64_t products,
+               cudaStream_t s) {
+  const int64_t blocks = m.side[0].blocks_total + m.side[1].blocks_total;
+  const int warps = blocks >= (int64_t)num_sms() * 16 ? 1 : kMeanWarps;  // per block
+  const int64_t grid = (blocks * warps + kMeanWarps - 1) / kMeanWarps;
+  const int64_t m_tiles = (sc.m + kScoreM - 1) / kScoreM;
+  H3B_REQUIRE(grid <= 0x7fffffffLL && products <= 65535 && m_tiles <= 65535,
+              "select_key_blocks: shape exceeds launch limits");
+  constexpr int kSmem = 2 * (kScoreM + kScoreN) * 2 * D;
   static ContextSlot slots[kMaxDevices];
   cudaError_t e = cudaErrorInvalidDevice;
   if (context_cached(slots, [&]() -> void* {
-        e = cudaFuncSetAttribute(score_select<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 200 * 1024);
+        e = cudaFuncSetAttribute(block_scores<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
       }) == nullptr) {
     set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
               cudaGetErrorString(e));
     return H3B_ERR_CUDA;
   }
-  const int64_t grid = batch * a.heads * a.row_groups;
-  H3B_REQUIRE(grid <= 0x7fffffffLL, "select_key_blocks: shape exceeds launch limits");
-  score_select<D, ROWS><<<(unsigned)grid, SelectShape<D, ROWS>::kThreads, smem, s>>>(a);
-  return check_launch("h3b_select_key_blocks");
-}
-
-template <bool FP16, int D>
-int launch_all(const MeanArgs& m, SelectArgs a, int64_t batch, cudaStream_t s) {
-  const int64_t grid = (m.total + kMeanWarps - 1) / kMeanWarps;
-  H3B_REQUIRE(grid <= 0x7fffffffLL, "select_key_blocks: shape exceeds launch limits");
-  block_means<FP16, D><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
+  if (warps == 1)
+    block_means<FP16, D, 1><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
+  else
+    block_means<FP16, D, kMeanWarps><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
   int rc = check_launch("h3b_select_key_blocks");
   if (rc != H3B_OK) return rc;
-  // Query blocks per CTA: as many as there are and as shared memory holds; each reads the
-  // key means once.
-  int rows = 16;
-  while (rows > 1 && (rows / 2 >= a.nq || select_smem(D, rows, a.pitch) > 200 * 1024)) rows /= 4;
-  a.row_groups = (a.nq + rows - 1) / rows;
-  const size_t smem = select_smem(D, rows, a.pitch);
-  if (rows == 16) return launch_select<D, 16>(a, batch, smem, s);
-  if (rows == 4) return launch_select<D, 4>(a, batch, smem, s);
-  return launch_select<D, 1>(a, batch, smem, s);
+  const dim3 tiles((unsigned)(sc.pitch / kScoreN), (unsigned)m_tiles, (unsigned)products);
+  block_scores<D><<<tiles, kScoreThreads, kSmem, s>>>(sc);
+  if ((rc = check_launch("h3b_select_key_blocks")) != H3B_OK) return rc;
+  // Registers for a row's scores: as few as hold it, up to 128 a lane.
+  if (a.nk <= 8 * 32) return launch_choose<8>(a, s);
+  if (a.nk <= 16 * 32) return launch_choose<16>(a, s);
+  if (a.nk <= 32 * 32) return launch_choose<32>(a, s);
+  if (a.nk <= 64 * 32) return launch_choose<64>(a, s);
+  if (a.nk <= 128 * 32) return launch_choose<128>(a, s);
+  return launch_choose<0>(a, s);
 }
 
 }  // namespace select
@@ -553,8 +844,7 @@ extern "C" int h3b_select_key_blocks_workspace_size(int64_t batch, int64_t seq_q
                   head_dim >= 0 && block_q > 0 && block_k > 0,
               "select_key_blocks: negative shape");
   const int64_t nq = (seq_q + block_q - 1) / block_q, nk = (seq_k + block_k - 1) / block_k;
-  const int64_t pitch = (nk + 31) / 32 * 32;
-  *bytes_out = 4 * batch * head_dim * (heads * nq + kv_heads * pitch);
+  *bytes_out = h3b::select::sizes_of(batch, heads, kv_heads, head_dim, nq, nk).bytes;
   return H3B_OK;
 }
 
@@ -586,10 +876,6 @@ extern "C" int h3b_select_key_blocks(
   const int64_t nq = (seq_q + block_q - 1) / block_q, nk = (seq_k + block_k - 1) / block_k;
   H3B_REQUIRE(top_k >= 1 && top_k <= nk, "select_key_blocks: top_k (%lld) must be 1..%lld",
               (long long)top_k, (long long)nk);
-  if (nk > kMaxKeyBlocks) {
-    h3b::set_error("h3b_select_key_blocks: more than 24576 key blocks");
-    return H3B_ERR_UNSUPPORTED;
-  }
   H3B_REQUIRE(batch <= (1LL << 31) / heads && batch * heads <= (1LL << 31) / nq,
               "select_key_blocks: shape exceeds launch limits");
   H3B_REQUIRE(indices != nullptr && counts != nullptr && q != nullptr && k != nullptr,
@@ -605,21 +891,38 @@ extern "C" int h3b_select_key_blocks(
   if (rc != H3B_OK) return rc;
   H3B_REQUIRE(workspace != nullptr && workspace_bytes >= need && h3b::aligned16(workspace),
               "select_key_blocks: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
-  const int pitch = (int)((nk + 31) / 32 * 32);
-  float* q_mean = static_cast<float*>(workspace);
-  float* k_mean = q_mean + batch * heads * nq * head_dim;
+  const Sizes sz = sizes_of(batch, heads, kv_heads, head_dim, nq, nk);
+  char* at = static_cast<char*>(workspace);
+  auto take = [&](int64_t bytes) {
+    char* p = at;
+    at += bytes;
+    return p;
+  };
+  Means qm, km;
+  qm.mean = reinterpret_cast<float*>(take(sz.q_rows * head_dim * 4));
+  km.mean = reinterpret_cast<float*>(take(sz.k_rows * head_dim * 4));
+  qm.hi = reinterpret_cast<__nv_bfloat16*>(take(sz.q_rows * head_dim * 2));
+  qm.mid = reinterpret_cast<__nv_bfloat16*>(take(sz.q_rows * head_dim * 2));
+  km.hi = reinterpret_cast<__nv_bfloat16*>(take(sz.k_rows * head_dim * 2));
+  km.mid = reinterpret_cast<__nv_bfloat16*>(take(sz.k_rows * head_dim * 2));
+  qm.norm = reinterpret_cast<float*>(take(sz.q_rows * 4));
+  km.norm = reinterpret_cast<float*>(take(sz.k_rows * 4));
+  uint32_t* scores =
+      reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.scores_at);
   MeanArgs m{};
-  m.side[0] = MeanSide{q, q_mean, q_batch_stride, q_row_stride, q_head_stride, q_lens,
-                       (int)seq_q, (int)heads, (int)block_q, (int)nq, 0, false, batch * nq * heads};
-  m.side[1] = MeanSide{k, k_mean, k_batch_stride, k_row_stride, k_head_stride, k_lens,
-                       (int)seq_k, (int)kv_heads, (int)block_k, (int)nk, pitch, true,
-                       batch * nk * kv_heads};
-  m.total = m.side[0].warps + m.side[1].warps;
-  SelectArgs a{};
+  m.side[0] = MeanSide{q, qm, q_batch_stride, q_row_stride, q_head_stride, q_lens, (int)seq_q,
+                       (int)heads, (int)block_q, (int)nq, batch * nq * heads};
+  m.side[1] = MeanSide{k, km, k_batch_stride, k_row_stride, k_head_stride, k_lens, (int)seq_k,
+                       (int)kv_heads, (int)block_k, (int)nk, batch * nk * kv_heads};
+  // The heads of a group lie behind one another: one product per (batch, key head).
+  ScoreArgs sc{qm, km, reinterpret_cast<float*>(scores), (int)(heads / kv_heads * nq), (int)nk,
+               (int)sz.pitch};
+  ChooseArgs a{};
   a.indices = indices;
   a.counts = counts;
-  a.q_mean = q_mean;
-  a.k_mean = k_mean;
+  a.q = qm;
+  a.k = km;
+  a.scores = scores;
   a.q_lens = q_lens;
   a.k_lens = k_lens;
   a.keep = keep;
@@ -627,15 +930,17 @@ extern "C" int h3b_select_key_blocks(
   a.kv_heads = (int)kv_heads;
   a.seq_q = (int)seq_q;
   a.seq_k = (int)seq_k;
+  a.head_dim = (int)head_dim;
   a.block_q = (int)block_q;
   a.block_k = (int)block_k;
   a.nq = (int)nq;
   a.nk = (int)nk;
-  a.pitch = pitch;
+  a.pitch = (int)sz.pitch;
   a.top_k = (int)top_k;
+  a.rows = sz.q_rows;
   if (dtype == H3B_DTYPE_FP16)
-    return head_dim == 128 ? launch_all<true, 128>(m, a, batch, stream)
-                           : launch_all<true, 64>(m, a, batch, stream);
-  return head_dim == 128 ? launch_all<false, 128>(m, a, batch, stream)
-                         : launch_all<false, 64>(m, a, batch, stream);
+    return head_dim == 128 ? launch_all<true, 128>(m, sc, a, batch * kv_heads, stream)
+                           : launch_all<true, 64>(m, sc, a, batch * kv_heads, stream);
+  return head_dim == 128 ? launch_all<false, 128>(m, sc, a, batch * kv_heads, stream)
+                         : launch_all<false, 64>(m, sc, a, batch * kv_heads, stream);
 }

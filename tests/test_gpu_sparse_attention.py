@@ -267,8 +267,39 @@ def test_select_ties_kept_blocks_and_nan():
     assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
 
 
+@pytest.mark.parametrize("q_scale,k_scale", [(1e-32, 1.0), (1e-36, 1e30), (1e18, 1e19), (1e-20, 1e-19), (0.0, 1.0), (3e38, 1.0)])
+def test_select_extreme_scales(q_scale, k_scale):
+    """Means whose products leave fp32's range, or too small for their digits: fp64 decides."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    q, k = _randn((1, 300, 2, 64), 1, torch.float32), _randn((1, 5000, 2, 64), 2, torch.float32)
+    q = (q.clamp(-1, 1) * q_scale).to(torch.bfloat16)
+    k = (k.clamp(-1, 1) * k_scale).to(torch.bfloat16)
+    got, n = select_key_blocks(q, k, 11)
+    ref, ref_n = sparse_ref.select(q, k, 11)
+    assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
+
+
+def test_select_close_scores():
+    """Blocks that differ in the last bits of their means only, in groups of more and fewer than a warp."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    g = torch.Generator().manual_seed(5)
+    for groups in (40, 3):
+        base = torch.randn(1, groups, 1, 128, generator=g).repeat_interleave(120 // groups, 1)
+        k = base.repeat_interleave(64, 1).to(torch.bfloat16)
+        k[:, ::64, 0, :4] += torch.randint(-1, 2, (1, 120, 4), generator=g).to(torch.bfloat16) * 2.0**-7
+        q = torch.randn(1, 640, 1, 128, generator=g).to(torch.bfloat16)
+        for top_k in (1, 17, 50, 119):
+            got, n = select_key_blocks(q.cuda(), k.cuda(), top_k, block_k=64)
+            ref, ref_n = sparse_ref.select(q, k, top_k, block_k=64)
+            assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
+
+
 def test_select_long_rows():
-    """More key blocks than sixteen or four rows of scores fit beside each other."""
+    """More key blocks than a warp keeps in registers."""
 
     from h3_flash_b200.runtime.attention.sparse import select_key_blocks
 
