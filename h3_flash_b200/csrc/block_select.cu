@@ -160,7 +160,8 @@ constexpr int kScoreM = 64, kScoreN = 128, kScoreThreads = 256;
 
 struct ScoreArgs {
   Means q, k;
-  float* scores;  // [products][m][pitch]
+  float* scores;    // [products][m][pitch]
+  uint32_t* norms;  // [products][pitch / kScoreN]: bits of the largest |k| of a tile's columns
   int m, nk, pitch;
 };
 
@@ -207,9 +208,20 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores(const ScoreArgs a)
     copy16(dst, side.hi + off, there);
     copy16(dst + (is_a ? part_a : part_b), side.mid + off, there);
   }
-  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
+  asm volatile("cp.async.commit_group;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.y == 0 && warp == 0) {
+    uint32_t norm = 0u;  // the bits order like the values, NaN above all
+#pragma unroll
+    for (int i = 0; i < kScoreN / 32; ++i) {
+      const int c = n0 + 32 * i + lane;
+      if (c < a.nk) norm = max(norm, __float_as_uint(a.k.norm[product * a.nk + c]));
+    }
+    norm = __reduce_max_sync(0xffffffffu, norm);
+    if (lane == 0) a.norms[product * gridDim.x + blockIdx.x] = norm;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
   const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
   float acc[2][4][4] = {};
 #pragma unroll
@@ -255,12 +267,14 @@ struct ChooseArgs {
   int32_t* indices;
   int32_t* counts;
   Means q, k;
-  uint32_t* scores;  // [rows][pitch]: fp32 scores, overwritten with keys where these do not fit registers
+  uint32_t* scores;  // [rows][pitch]: fp32 scores, overwritten with keys by choose_any
+  const uint32_t* norms;  // [batch * kv_heads][norm_tiles]
+  int norm_tiles;
   const int32_t* q_lens;
   const int32_t* k_lens;
   const uint8_t* keep;
   int heads, kv_heads, seq_q, seq_k, head_dim, block_q, block_k, nq, nk, pitch, top_k;
-  int64_t rows;  // batch * heads * nq
+  uint32_t rows;  // batch * heads * nq
 };
 
 // Order-preserving keys of a score. -0 and +0 are the same score, NaN ranks as -inf.
@@ -312,32 +326,67 @@ constexpr int kChooseWarps = 8;
 
 // What a warp's row of scores is about.
 struct Row {
-  int64_t list, k_row0;  // which query block, and the first key block of its head
+  int64_t list, k_row0;  // which query block, and the first key block of its key head
   int k_blocks, want, kept;  // blocks that exist, places in the list, kept blocks
   float q_norm, k_norm;      // k_norm: the largest of the blocks that exist
 };
 
-// fp64 score of a column as an order-preserving key, the same sum in every lane.
-__device__ __forceinline__ unsigned long long exact_key(const ChooseArgs& a, const Row& r, int c,
-                                                        int lane) {
+// fp64 scores of four columns (c of lane 8g for group g of eight lanes) as order-preserving
+// keys, in all lanes of a group. Every column is summed in the same order.
+__device__ __forceinline__ unsigned long long exact_keys(const ChooseArgs& a, const Row& r, int c,
+                                                         int lane) {
   const float* q = a.q.mean + r.list * a.head_dim;
   const float* k = a.k.mean + (r.k_row0 + c) * a.head_dim;
-  double s = 0.0;
-  for (int d = lane; d < a.head_dim; d += 32) s = fma((double)q[d], (double)k[d], s);
+  float4 x[4], y[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  for (int i = 0; i < 4; ++i) {
+    const int d = 4 * (lane & 7) + 32 * i;
+    const bool there = d < a.head_dim;
+    x[i] = there ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    y[i] = there ? *reinterpret_cast<const float4*>(k + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fma((double)x[i].x, (double)y[i].x, s);
+    s = fma((double)x[i].y, (double)y[i].y, s);
+    s = fma((double)x[i].z, (double)y[i].z, s);
+    s = fma((double)x[i].w, (double)y[i].w, s);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return score_key(s);
 }
 
+// Of n columns (n <= 32, ascending or not), which are the `open` best by fp64 score, ties to
+// the lower column: a mask by position.
+__device__ __forceinline__ unsigned best_of(const ChooseArgs& a, const Row& r, const int* columns,
+                                            int n, int open, int lane) {
+  unsigned long long mine = 0ull;
+  for (int i = 0; i < n; i += 4) {
+    const unsigned long long s = exact_keys(a, r, columns[min(i + (lane >> 3), n - 1)], lane);
+    const unsigned long long at = __shfl_sync(0xffffffffu, s, (lane & 3) * 8);
+    if (lane >= i && lane < i + 4) mine = at;
+  }
+  const int column = columns[min(lane, n - 1)];
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    const unsigned long long s = __shfl_sync(0xffffffffu, mine, i);
+    const int c = __shfl_sync(0xffffffffu, column, i);
+    rank += s > mine || (s == mine && c < column);
+  }
+  return __ballot_sync(0xffffffffu, lane < n && rank < open);
+}
+
 // The bound on the difference of two scores from their fp32 values, 2E with
-//   E = 1e-4 |q| max|k| + 1e-35:
+//   E = 6e-5 |q| max|k| + 1e-35:
 // dropping mid mid and what two bf16 leave of a mean, 3 2^-18 of |q| |k| (Cauchy-Schwarz);
-// 384 products summed in fp32, 2^-23 each if every addition truncates; products below fp32's
-// range. Infinite where it does not hold: norms beyond fp32, and means too small for two bf16
+// 384 products summed in fp32, 2^-23 each if every addition truncates (1.14e-5 + 4.58e-5);
+// products below fp32's range. Infinite where it does not hold: norms beyond fp32, and means too small for two bf16
 // to hold their digits.
 __device__ __forceinline__ float twice_error(const Row& r) {
   const bool sound = (r.q_norm >= 1e-30f || r.q_norm == 0.f) && (r.k_norm >= 1e-30f || r.k_norm == 0.f);
-  return sound ? 2.02e-4f * r.q_norm * r.k_norm + 2e-35f : INFINITY;
+  return sound ? 1.21e-4f * r.q_norm * r.k_norm + 2e-35f : INFINITY;
 }
 
 // Any row: keys of the scores in the workspace, where each lane reads and writes columns
@@ -493,19 +542,8 @@ __device__ __noinline__ int choose_any(const ChooseArgs& a, const Row& r, uint32
     if (n_close == open) {
       least_in = lo;
     } else {
-      auto score = [&](int c) { return exact_key(a, r, c, lane); };
       if (n_close <= 32) {
-        unsigned long long mine = 0ull;
-        for (int i = 0; i < n_close; ++i) {
-          const unsigned long long s = score(close[i]);
-          if (i == lane) mine = s;
-        }
-        int rank = 0;  // close[] ascends: of equal scores the lower lane goes first
-        for (int i = 0; i < n_close; ++i) {
-          const unsigned long long s = __shfl_sync(0xffffffffu, mine, i);
-          rank += s > mine || (s == mine && i < lane);
-        }
-        const unsigned in = __ballot_sync(0xffffffffu, lane < n_close && rank < open);
+        const unsigned in = best_of(a, r, close, n_close, open, lane);
         for (int i = 0; i < n_close; ++i) {
           const int c = close[i];
           if (lane == (c & 31)) row[c] = (in >> i & 1u) ? kInKey : 0u;
@@ -518,7 +556,7 @@ __device__ __noinline__ int choose_any(const ChooseArgs& a, const Row& r, uint32
             unsigned mask = __ballot_sync(0xffffffffu, k >= lo && k <= hi);
             for (; mask != 0u; mask &= mask - 1u) {
               const int c = c0 - lane + __ffs((int)mask) - 1;
-              f(c, score(c));
+              f(c, exact_keys(a, r, c, lane));
             }
           });
         };
@@ -682,21 +720,13 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
       cut = __int_as_float(__float_as_int(cut) + (cut > 0.f ? -1 : 1));
       if (lo == 0.f) cut = -1e-45f;
     } else {
-      unsigned long long exact = 0ull;
-      for (unsigned m = near; m != 0u; m &= m - 1u) {
-        const int i = __ffs((int)m) - 1;
-        const unsigned long long s = exact_key(a, r, columns[i], lane);
-        if (lane == i) exact = s;
-      }
-      int exact_rank = 0;
-      for (unsigned m = near; m != 0u; m &= m - 1u) {
-        const int i = __ffs((int)m) - 1;
-        const unsigned long long s = __shfl_sync(0xffffffffu, exact, i);
-        exact_rank += s > exact || (s == exact && columns[i] < my_column);
-      }
-      const unsigned in = __ballot_sync(0xffffffffu, (near >> lane & 1u) && exact_rank < open);
-      for (unsigned m = near; m != 0u; m &= m - 1u) {
-        const int i = __ffs((int)m) - 1;
+      // The close columns move to the front of `columns`, each still in its owner's register.
+      const int n_close = __popc(near);
+      __syncwarp();
+      if (near >> lane & 1u) columns[__popc(near & ((1u << lane) - 1u))] = my_column;
+      __syncwarp();
+      const unsigned in = best_of(a, r, columns, n_close, open, lane);
+      for (int i = 0; i < n_close; ++i) {
         const int at = columns[i] - c0;
         const float mark = (in >> i & 1u) ? kBig : -kBig;
 #pragma unroll
@@ -734,27 +764,28 @@ __global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseAr
   __shared__ float values[kChooseWarps][32];
   __shared__ int gathered[kChooseWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t list = blockIdx.x * kChooseWarps + warp;
+  if (list >= a.rows) return;
+  const uint32_t bh = list / (uint32_t)a.nq, block = list % (uint32_t)a.nq;
+  const int head = (int)(bh % (uint32_t)a.heads), b = (int)(bh / (uint32_t)a.heads);
+  const int64_t kv = (int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads);
+  uint32_t norm = 0u;
+  for (int i = lane; i < a.norm_tiles; i += 32) norm = max(norm, a.norms[kv * a.norm_tiles + i]);
   Row r;
-  r.list = (int64_t)blockIdx.x * kChooseWarps + warp;
-  if (r.list >= a.rows) return;
-  const int block = (int)(r.list % a.nq);
-  const int head = (int)(r.list / a.nq % a.heads);
-  const int b = (int)(r.list / a.nq / a.heads);
-  r.k_row0 = ((int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads)) * a.nk;
+  r.list = list;
+  r.q_norm = a.q.norm[list];
+  r.k_row0 = kv * a.nk;
   r.k_blocks = (rows_of(a.k_lens, b, a.seq_k) + a.block_k - 1) / a.block_k;
-  r.want = block * a.block_q < rows_of(a.q_lens, b, a.seq_q) ? min(a.top_k, r.k_blocks) : 0;
+  r.want = (int)block * a.block_q < rows_of(a.q_lens, b, a.seq_q) ? min(a.top_k, r.k_blocks) : 0;
   r.kept = 0;
+  r.k_norm = __uint_as_float(__reduce_max_sync(0xffffffffu, norm));
   int done = 0;
   if (r.want > 0) {
-    uint32_t norm = 0u;  // bits of max |k|: they order like the values, NaN above all
-    for (int c = lane; c < r.k_blocks; c += 32)
-      norm = max(norm, __float_as_uint(a.k.norm[r.k_row0 + c]));
     if (a.keep != nullptr) {
+#pragma unroll 8
       for (int c = lane; c < r.k_blocks; c += 32) r.kept += a.keep[c] != 0;
       r.kept = __reduce_add_sync(0xffffffffu, r.kept);
     }
-    r.k_norm = __uint_as_float(__reduce_max_sync(0xffffffffu, norm));
-    r.q_norm = a.q.norm[r.list];
     done = -1;
     if constexpr (KEYS > 0) {
       if (r.kept <= r.want)
@@ -773,7 +804,7 @@ __global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseAr
 // ---- host side --------------------------------------------------------------
 
 struct Sizes {
-  int64_t q_rows, k_rows, pitch, scores_at, bytes;
+  int64_t q_rows, k_rows, pitch, norms_at, scores_at, bytes;
 };
 Sizes sizes_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t nq,
                int64_t nk) {
@@ -782,7 +813,8 @@ Sizes sizes_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
   s.k_rows = batch * kv_heads * nk;
   s.pitch = (nk + kScoreN - 1) / kScoreN * kScoreN;
   // Per row: D fp32, D + D bf16, a norm (rounded up so that every part starts on 16 bytes).
-  s.scores_at = (s.q_rows + s.k_rows) * head_dim * 8 + ((s.q_rows + s.k_rows) * 4 + 31) / 16 * 16;
+  s.norms_at = (s.q_rows + s.k_rows) * head_dim * 8 + ((s.q_rows + s.k_rows) * 4 + 31) / 16 * 16;
+  s.scores_at = s.norms_at + (batch * kv_heads * (s.pitch / kScoreN) * 4 + 15) / 16 * 16;
   s.bytes = s.scores_at + s.q_rows * s.pitch * 4;
   return s;
 }
@@ -876,7 +908,7 @@ extern "C" int h3b_select_key_blocks(
   const int64_t nq = (seq_q + block_q - 1) / block_q, nk = (seq_k + block_k - 1) / block_k;
   H3B_REQUIRE(top_k >= 1 && top_k <= nk, "select_key_blocks: top_k (%lld) must be 1..%lld",
               (long long)top_k, (long long)nk);
-  H3B_REQUIRE(batch <= (1LL << 31) / heads && batch * heads <= (1LL << 31) / nq,
+  H3B_REQUIRE(batch <= (1LL << 31) / heads && batch * heads <= ((1LL << 31) - 64) / nq,
               "select_key_blocks: shape exceeds launch limits");
   H3B_REQUIRE(indices != nullptr && counts != nullptr && q != nullptr && k != nullptr,
               "select_key_blocks: null argument");
@@ -907,15 +939,15 @@ extern "C" int h3b_select_key_blocks(
   km.mid = reinterpret_cast<__nv_bfloat16*>(take(sz.k_rows * head_dim * 2));
   qm.norm = reinterpret_cast<float*>(take(sz.q_rows * 4));
   km.norm = reinterpret_cast<float*>(take(sz.k_rows * 4));
-  uint32_t* scores =
-      reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.scores_at);
+  auto* norms = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.norms_at);
+  auto* scores = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.scores_at);
   MeanArgs m{};
   m.side[0] = MeanSide{q, qm, q_batch_stride, q_row_stride, q_head_stride, q_lens, (int)seq_q,
                        (int)heads, (int)block_q, (int)nq, batch * nq * heads};
   m.side[1] = MeanSide{k, km, k_batch_stride, k_row_stride, k_head_stride, k_lens, (int)seq_k,
                        (int)kv_heads, (int)block_k, (int)nk, batch * nk * kv_heads};
   // The heads of a group lie behind one another: one product per (batch, key head).
-  ScoreArgs sc{qm, km, reinterpret_cast<float*>(scores), (int)(heads / kv_heads * nq), (int)nk,
+  ScoreArgs sc{qm, km, reinterpret_cast<float*>(scores), norms, (int)(heads / kv_heads * nq), (int)nk,
                (int)sz.pitch};
   ChooseArgs a{};
   a.indices = indices;
@@ -923,6 +955,8 @@ extern "C" int h3b_select_key_blocks(
   a.q = qm;
   a.k = km;
   a.scores = scores;
+  a.norms = norms;
+  a.norm_tiles = (int)(sz.pitch / kScoreN);
   a.q_lens = q_lens;
   a.k_lens = k_lens;
   a.keep = keep;
@@ -937,7 +971,7 @@ extern "C" int h3b_select_key_blocks(
   a.nk = (int)nk;
   a.pitch = (int)sz.pitch;
   a.top_k = (int)top_k;
-  a.rows = sz.q_rows;
+  a.rows = (uint32_t)sz.q_rows;
   if (dtype == H3B_DTYPE_FP16)
     return head_dim == 128 ? launch_all<true, 128>(m, sc, a, batch * kv_heads, stream)
                            : launch_all<true, 64>(m, sc, a, batch * kv_heads, stream);
