@@ -140,7 +140,9 @@ def check(code: int, what: str) -> None:
 def call(name: str, *args: Any) -> None:
     """Call an entry point and raise on a failing status."""
 
-    check(getattr(load(), name)(*args), name)
+    code = getattr(_LIB or load(), name)(*args)
+    if code:
+        check(code, name)
 
 
 def reset_launch_count() -> None:

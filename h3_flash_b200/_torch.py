@@ -46,16 +46,15 @@ def check_inputs(op: str, allowed: tuple[torch.dtype, ...], tensors: tuple[torch
     take a few microseconds on the GPU."""
 
     first = tensors[0]
-    grad = torch.is_grad_enabled()
     if not isinstance(first, torch.Tensor) or not first.is_cuda:
         require_cuda(op, *tensors)
-    dtype, device = first.dtype, first.device
+    dtype, device = first.dtype, first.get_device()
     for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.device != device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != device:
             require_cuda(op, *tensors)
         if t.dtype is not dtype:
             raise TypeError(f"{op}: tensors have different types ({dtype}, {t.dtype})")
-        if grad and t.requires_grad:
+        if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{op}: inference only; call it under torch.no_grad() or on detached tensors")
     if dtype not in allowed:
         raise TypeError(f"{op}: expected {' or '.join(str(d) for d in allowed)} tensors, got {dtype}")
@@ -112,12 +111,11 @@ def call(name: str, *args) -> None:
     _lib.call(name, *args)
 
 
-def call_on(tensor: torch.Tensor, name: str, *args) -> None:
-    """``call`` with the tensor's device current, on its current stream (the last argument)."""
+def call_on(device: int, name: str, *args) -> None:
+    """``call`` with ``device`` current, on its current stream (the last argument)."""
 
-    device = tensor.get_device()
     if torch.cuda.current_device() == device:
-        _lib.call(name, *args, stream_of(tensor))
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream_of(tensor))
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))

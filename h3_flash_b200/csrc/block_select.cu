@@ -85,6 +85,7 @@ template <bool FP16, int D, int WARPS>
 __global__ void __launch_bounds__(kMeanWarps * 32) block_means(const MeanArgs a) {
   __shared__ double part[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
   const int warp = threadIdx.x >> 5 & (WARPS - 1), lane = threadIdx.x & 31;
+  grid_wait();
   int64_t w = (int64_t)blockIdx.x * (kMeanWarps / WARPS) + (threadIdx.x >> 5) / WARPS;
   if (w >= a.side[0].blocks_total + a.side[1].blocks_total) return;
   const bool is_k = w >= a.side[0].blocks_total;
@@ -131,14 +132,18 @@ __global__ void __launch_bounds__(kMeanWarps * 32) block_means(const MeanArgs a)
         for (int j = 0; j < 8; ++j) acc[j] += part[i][col + j];
     }
   }
+  grid_done();
   const int64_t out = ((int64_t)b * s.heads + head) * s.blocks + block;
   double square = 0.0;
   if (lane < kLanes) {
+    // (A power of two divides exactly as its reciprocal multiplies.)
+    const bool exact = (count & (count - 1)) == 0;
     const double n = count > 0 ? (double)count : 1.0;
+    const double inv = 1.0 / (double)(count > 0 ? count : 1);
     float m[8], hi[8], mid[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      m[j] = (float)(acc[j] / n);
+      m[j] = (float)(exact ? acc[j] * inv : acc[j] / n);
       hi[j] = __bfloat162float(__float2bfloat16_rn(m[j]));
       mid[j] = m[j] - hi[j];
       square += (double)m[j] * (double)m[j];
@@ -151,7 +156,9 @@ __global__ void __launch_bounds__(kMeanWarps * 32) block_means(const MeanArgs a)
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
-  if (lane == 0) s.out.norm[out] = (float)sqrt(square);
+  // (Squares of tiny or huge means leave fp32.)
+  if (lane == 0)
+    s.out.norm[out] = square > 1e-30 && square < 1e30 ? sqrtf((float)square) : (float)sqrt(square);
 }
 
 // ---- scores ---------------------------------------------------------------
@@ -196,6 +203,7 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores(const ScoreArgs a)
   const uint32_t tile_b = base + 2 * part_a;
   const int m0 = blockIdx.y * kScoreM, n0 = blockIdx.x * kScoreN;
   const int64_t product = blockIdx.z;
+  grid_wait();
   auto at = [&](int row, int chunk) { return row * kRowBytes + ((chunk ^ (row & 7)) << 4); };
   for (int i = threadIdx.x; i < (kScoreM + kScoreN) * kChunks; i += kScoreThreads) {
     const int row = i / kChunks, chunk = i % kChunks;
@@ -247,6 +255,7 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores(const ScoreArgs a)
         mma_bf16(acc[i][j], ah[i], bh[p][q], bh[p][q + 1]);
       }
   }
+  grid_done();
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -757,8 +766,11 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
 // k-th largest fp32 score and E its error (twice_error), blocks above T + 2E are in and blocks
 // below T - 2E are out whatever the rounding did; the few between are scored again in fp64 and
 // ranked.
+// CTAs per SM that the registers should allow: a row is a chain of short steps, and many rows at
+// once hide it.
 template <int KEYS>
-__global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseArgs a) {
+__global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 4 : KEYS <= 32 ? 3 : 1)
+    block_choose(const ChooseArgs a) {
   __shared__ uint32_t bins[kChooseWarps][kBins];
   __shared__ int columns[kChooseWarps][32];
   __shared__ float values[kChooseWarps][32];
@@ -769,6 +781,7 @@ __global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseAr
   const uint32_t bh = list / (uint32_t)a.nq, block = list % (uint32_t)a.nq;
   const int head = (int)(bh % (uint32_t)a.heads), b = (int)(bh / (uint32_t)a.heads);
   const int64_t kv = (int64_t)b * a.kv_heads + head / (a.heads / a.kv_heads);
+  grid_wait();
   uint32_t norm = 0u;
   for (int i = lane; i < a.norm_tiles; i += 32) norm = max(norm, a.norms[kv * a.norm_tiles + i]);
   Row r;
@@ -796,6 +809,7 @@ __global__ void __launch_bounds__(kChooseWarps * 32) block_choose(const ChooseAr
       done = choose_any(a, r, bins[warp], columns[warp], lane);
     }
   }
+  grid_done();
   int32_t* out = a.indices + r.list * a.top_k;
   for (int c = done + lane; c < a.top_k; c += 32) out[c] = -1;
   if (lane == 0) a.counts[r.list] = done;
@@ -821,8 +835,8 @@ Sizes sizes_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
 
 template <int KEYS>
 int launch_choose(const ChooseArgs& a, cudaStream_t s) {
-  block_choose<KEYS><<<(unsigned)((a.rows + kChooseWarps - 1) / kChooseWarps),
-                          kChooseWarps * 32, 0, s>>>(a);
+  launch_after(block_choose<KEYS>, dim3((a.rows + kChooseWarps - 1) / kChooseWarps),
+               kChooseWarps * 32, 0, s, a);
   return check_launch("h3b_select_key_blocks");
 }
 
@@ -847,13 +861,13 @@ int launch_all(const MeanArgs& m, const ScoreArgs& sc, const ChooseArgs& a, int6
     return H3B_ERR_CUDA;
   }
   if (warps == 1)
-    block_means<FP16, D, 1><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
+    launch_after(block_means<FP16, D, 1>, dim3((unsigned)grid), kMeanWarps * 32, 0, s, m);
   else
-    block_means<FP16, D, kMeanWarps><<<(unsigned)grid, kMeanWarps * 32, 0, s>>>(m);
+    launch_after(block_means<FP16, D, kMeanWarps>, dim3((unsigned)grid), kMeanWarps * 32, 0, s, m);
   int rc = check_launch("h3b_select_key_blocks");
   if (rc != H3B_OK) return rc;
   const dim3 tiles((unsigned)(sc.pitch / kScoreN), (unsigned)m_tiles, (unsigned)products);
-  block_scores<D><<<tiles, kScoreThreads, kSmem, s>>>(sc);
+  launch_after(block_scores<D>, tiles, kScoreThreads, kSmem, s, sc);
   if ((rc = check_launch("h3b_select_key_blocks")) != H3B_OK) return rc;
   // Registers for a row's scores: as few as hold it, up to 128 a lane.
   if (a.nk <= 8 * 32) return launch_choose<8>(a, s);

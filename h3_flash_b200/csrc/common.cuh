@@ -166,6 +166,36 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// ---- programmatic dependent launch -----------------------------------------
+//
+// A kernel launched with launch_after() may start while the kernel before it in the stream
+// drains: it must call grid_wait() before it touches global memory, and from then on sees
+// everything written before. grid_done() in the kernel before says that this CTA needs no
+// more of the GPU than it has; a kernel that never calls it counts as done when it ends.
+
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_done() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
+                         cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 inline int num_sms() {
   static int sms = 0;
   if (sms == 0) {

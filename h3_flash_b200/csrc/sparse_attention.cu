@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_wait();  // everything above touched nothing but this CTA's own memory
 
   auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, prm.status));
@@ -736,6 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  grid_done();
   if (*abort_flag != 0u) {
     // Unwinding: let copies in flight land before shared memory is given up.
     const unsigned long long t0 = globaltimer();
@@ -757,6 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kMaxParts = 32;
 template <bool FP16, int D>
 __global__ void __launch_bounds__(256) sparse_combine(const Params prm, int split_pairs) {
+  grid_wait();
   const int gw = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int pair_rows = min(prm.duo ? kTile : kTiles * kTile, prm.seq_q);
@@ -911,11 +914,13 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     return H3B_ERR_CUDA;
   }
   const unsigned grid = (unsigned)std::min(p.n_items, num_sms());
-  sparse_fwd<FP16, D, BK><<<grid, kThreads, Layout<D>::kSmemAlloc, stream>>>(qm, km, vm, p);
+  launch_after(sparse_fwd<FP16, D, BK>, dim3(grid), kThreads, Layout<D>::kSmemAlloc, stream, qm, km,
+               vm, p);
   int rc = check_launch("h3b_block_sparse_attention");
   if (rc != H3B_OK || split_pairs == 0) return rc;
   const int rows = split_pairs * std::min(p.duo ? kTile : kTiles * kTile, p.seq_q);
-  sparse_combine<FP16, D><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(p, split_pairs);
+  launch_after(sparse_combine<FP16, D>, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, p,
+               split_pairs);
   return check_launch("h3b_block_sparse_attention");
 }
 

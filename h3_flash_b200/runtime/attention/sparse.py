@@ -45,15 +45,16 @@ def _check_shapes(op: str, q: torch.Tensor, k: torch.Tensor, block_q: int, block
         raise ValueError(f"{op}: {h} query heads are not a multiple of {hk} key heads")
 
 
-def _strides(op: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
-    """(batch, row, head) strides of a view the kernels can address."""
+def _view(op: str, name: str, t: torch.Tensor) -> tuple[int, ...]:
+    """(address, batch stride, row stride, head stride) of a view the kernels can address."""
 
-    *strides, last = t.stride()
+    batch, row, head, last = t.stride()
+    address = t.data_ptr()
     if last != 1:
         raise ValueError(f"{op}: {name}: head_dim must be contiguous")
-    if t.data_ptr() % 16:
+    if address % 16:
         raise ValueError(f"{op}: {name}: base address must be 16-byte aligned")
-    return strides
+    return address, batch, row, head
 
 
 def _side_tensor(op: str, name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple[int, ...],
@@ -82,6 +83,34 @@ def _bytes(name: str, *shape: int) -> int:
     return value.value
 
 
+def _list_length(op: str, top_k: int, blocks: int) -> int:
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or top_k < 1:
+        raise ValueError(f"{op}: top_k must be a positive integer, got {top_k!r}")
+    return min(top_k, max(blocks, 1))
+
+
+def _select(dims, q, k, lists, lens, keep, code, workspace, need, device) -> None:
+    """One selection. dims: (batch, seq_q, seq_k, heads, kv_heads, head_dim, block_q, block_k,
+    top_k); q, k: ``_view``s; lists: the addresses of indices and counts."""
+
+    call_on(device, "h3b_select_key_blocks", *lists, q[0], k[0], *dims, *q[1:], *k[1:], *lens, keep, code,
+            workspace, need)
+
+
+def _attend(dims, entries, q, k, v, out, lse, lists, lens, scale, code, workspace, need, device) -> None:
+    """One attention over lists of ``entries``; dims as for ``_select`` without top_k."""
+
+    call_on(device, "h3b_block_sparse_attention", out[0], lse, q[0], k[0], v[0], *lists, entries, *dims, *q[1:],
+            *k[1:], *v[1:], *out[1:], *lens, scale, code, workspace, need)
+
+
+def _scale(op: str, softmax_scale: float | None, head_dim: int) -> float:
+    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{op}: softmax_scale must be positive and finite, got {scale}")
+    return scale
+
+
 def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: int = 128, block_k: int = 128,
                       q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
                       keep: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -95,27 +124,25 @@ def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: 
     equal inputs give equal lists on any device and in any batch."""
 
     op = "select_key_blocks"
-    dtype = check_inputs(op, _TYPES, (q, k))
+    code = check_inputs(op, _TYPES, (q, k))
     _check_shapes(op, q, k, block_q, block_k)
     (b, sq, h, d), (_, sk, hk, _) = q.shape, k.shape
     nq, nk = -(-sq // block_q), -(-sk // block_k)
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or top_k < 1:
-        raise ValueError(f"{op}: top_k must be a positive integer, got {top_k!r}")
-    top_k = min(top_k, max(nk, 1))
+    top_k = _list_length(op, top_k, nk)
     q_lens = _side_tensor(op, "q_lens", q_lens, torch.int32, (b,), q.device)
     k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
     keep = _side_tensor(op, "keep", keep, torch.bool, (nk,), q.device)
-    if b and sq and h and not sk:
-        raise ValueError(f"{op}: empty key sequence")
     indices = torch.empty((b, h, nq, top_k), dtype=torch.int32, device=q.device)
     counts = torch.empty((b, h, nq), dtype=torch.int32, device=q.device)
     if counts.numel() == 0:
         return indices, counts
+    if not sk:
+        raise ValueError(f"{op}: empty key sequence")
     need = _bytes("h3b_select_key_blocks_workspace_size", b, sq, sk, h, hk, d, block_q, block_k)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    call_on(q, "h3b_select_key_blocks", indices.data_ptr(), counts.data_ptr(), q.data_ptr(), k.data_ptr(), b, sq, sk,
-            h, hk, d, block_q, block_k, top_k, *_strides(op, "q", q), *_strides(op, "k", k), _opt(q_lens),
-            _opt(k_lens), _opt(keep), dtype, ws.data_ptr(), need)
+    _select((b, sq, sk, h, hk, d, block_q, block_k, top_k), _view(op, "q", q), _view(op, "k", k),
+            (indices.data_ptr(), counts.data_ptr()), (_opt(q_lens), _opt(k_lens)), _opt(keep), code, ws.data_ptr(),
+            need, q.get_device())
     return indices, counts
 
 
@@ -135,7 +162,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     the softmax sums."""
 
     op = "block_sparse_attention"
-    dtype = check_inputs(op, _TYPES, (q, k, v) if out is None else (q, k, v, out))
+    code = check_inputs(op, _TYPES, (q, k, v) if out is None else (q, k, v, out))
     _check_shapes(op, q, k, block_q, block_k)
     if v.shape != k.shape:
         raise ValueError(f"{op}: k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
@@ -153,21 +180,33 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     elif out.shape != q.shape:
         raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
     lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device) if return_lse else None
-    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(d)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"{op}: softmax_scale must be positive and finite, got {scale}")
-    if out.numel() and (sk == 0 or entries == 0):
+    scale = _scale(op, softmax_scale, d)
+    if b * sq * h and (sk == 0 or entries == 0):
         out.zero_()
         if lse is not None:
             lse.fill_(-math.inf)
-    elif out.numel():
+    elif b * sq * h:
         need = _bytes("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, entries)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        call_on(q, "h3b_block_sparse_attention", out.data_ptr(), _opt(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                indices.data_ptr(), _opt(counts), entries, b, sq, sk, h, hk, d, block_q, block_k,
-                *_strides(op, "q", q), *_strides(op, "k", k), *_strides(op, "v", v), *_strides(op, "out", out),
-                _opt(q_lens), _opt(k_lens), scale, dtype, _opt(ws), need)
+        _attend((b, sq, sk, h, hk, d, block_q, block_k), entries, _view(op, "q", q), _view(op, "k", k),
+                _view(op, "v", v), _view(op, "out", out), _opt(lse), (indices.data_ptr(), _opt(counts)),
+                (_opt(q_lens), _opt(k_lens)), scale, code, _opt(ws), need, q.get_device())
     return (out, lse) if return_lse else out
+
+
+def _select_and_attend(dims, top_k, q, k, v, out, lse, lens, keep, scale, code, device) -> None:
+    """Both steps; the lists and the workspaces are parts of one allocation that the two share."""
+
+    b, sq, sk, h, hk, d, block_q, block_k = dims
+    rows = b * h * -(-sq // block_q)
+    lists = (4 * rows * (top_k + 1) + 255) // 256 * 256
+    first = _bytes("h3b_select_key_blocks_workspace_size", *dims)
+    second = _bytes("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, top_k)
+    ws = torch.empty(lists + max(first, second), dtype=torch.uint8, device=device)
+    at = ws.data_ptr()
+    pair = (at, at + 4 * rows * top_k)
+    _select((*dims, top_k), q, k, pair, lens, keep, code, at + lists, first, device)
+    _attend(dims, top_k, q, k, v, out, lse, pair, lens, scale, code, at + lists, second, device)
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int, *, block_q: int = 128,
@@ -176,11 +215,30 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: i
                      out: torch.Tensor | None = None, return_lse: bool = False):
     """``select_key_blocks`` and then ``block_sparse_attention`` over its lists."""
 
-    indices, counts = select_key_blocks(q, k, top_k, block_q=block_q, block_k=block_k, q_lens=q_lens,
-                                        k_lens=k_lens, keep=keep)
-    return block_sparse_attention(q, k, v, indices, counts, block_q=block_q, block_k=block_k,
-                                  softmax_scale=softmax_scale, q_lens=q_lens, k_lens=k_lens, out=out,
-                                  return_lse=return_lse)
+    op = "sparse_attention"
+    code = check_inputs(op, _TYPES, (q, k, v) if out is None else (q, k, v, out))
+    _check_shapes(op, q, k, block_q, block_k)
+    if v.shape != k.shape:
+        raise ValueError(f"{op}: k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
+    (b, sq, h, d), (_, sk, hk, _) = q.shape, k.shape
+    nk = -(-sk // block_k)
+    top_k = _list_length(op, top_k, nk)
+    q_lens = _side_tensor(op, "q_lens", q_lens, torch.int32, (b,), q.device)
+    k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
+    keep = _side_tensor(op, "keep", keep, torch.bool, (nk,), q.device)
+    if out is None:
+        out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device) if return_lse else None
+    scale = _scale(op, softmax_scale, d)
+    if b * sq * h:
+        if not sk:
+            raise ValueError(f"{op}: empty key sequence")
+        _select_and_attend((b, sq, sk, h, hk, d, block_q, block_k), top_k, _view(op, "q", q), _view(op, "k", k),
+                           _view(op, "v", v), _view(op, "out", out), _opt(lse), (_opt(q_lens), _opt(k_lens)),
+                           _opt(keep), scale, code, q.get_device())
+    return (out, lse) if return_lse else out
 
 
 def packed_sparse_attention(packed: torch.Tensor, top_k: int, head_dim: int = HEAD_DIM, *, block_q: int = 128,
@@ -190,13 +248,37 @@ def packed_sparse_attention(packed: torch.Tensor, top_k: int, head_dim: int = HE
     """``sparse_attention`` over the packed receive buffer ``[S, hl, 3*D]`` (q | k | v per
     head), read in place. Returns ``[S, hl, D]`` (and lse ``[hl, S]``)."""
 
+    op = "packed_sparse_attention"
+    code = check_inputs(op, _TYPES, (packed,) if out is None else (packed, out))
     if packed.dim() != 3 or packed.shape[-1] != 3 * head_dim:
         raise ValueError(f"packed attention expects [S, hl, 3*{head_dim}], got {tuple(packed.shape)}")
-    if packed.stride(-1) != 1 or packed.stride(-2) != 3 * head_dim:
+    if head_dim not in HEAD_DIMS:
+        raise RuntimeError(f"{op}: head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+    if block_q not in BLOCK_Q or block_k not in BLOCK_K:
+        raise ValueError(f"{op}: block_q must be one of {BLOCK_Q} and block_k one of {BLOCK_K}, got "
+                         f"{block_q} and {block_k}")
+    s, hl, _ = packed.shape
+    row, head, last = packed.stride()
+    if last != 1 or head != 3 * head_dim or row % 8:
         packed = packed.contiguous()
-    q, k, v = (packed[..., i * head_dim : (i + 1) * head_dim].unsqueeze(0) for i in range(3))
+        row, head, last = packed.stride()
+    nk = -(-s // block_k)
+    top_k = _list_length(op, top_k, nk)
+    keep = _side_tensor(op, "keep", keep, torch.bool, (nk,), packed.device)
     if out is None:
-        out = torch.empty((packed.shape[0], packed.shape[1], head_dim), dtype=packed.dtype, device=packed.device)
-    result = sparse_attention(q, k, v, top_k, block_q=block_q, block_k=block_k, softmax_scale=softmax_scale,
-                              keep=keep, out=out.unsqueeze(0), return_lse=return_lse)
-    return (out, result[1][0]) if return_lse else out
+        out = torch.empty((s, hl, head_dim), dtype=packed.dtype, device=packed.device)
+    elif out.shape != (s, hl, head_dim):
+        raise ValueError(f"{op}: out must have shape {(s, hl, head_dim)}, got {tuple(out.shape)}")
+    lse = torch.empty((hl, s), dtype=torch.float32, device=packed.device) if return_lse else None
+    scale = _scale(op, softmax_scale, head_dim)
+    out_row, out_head, out_last = out.stride()
+    base, to = packed.data_ptr(), out.data_ptr()
+    if out_last != 1 or base % 16 or to % 16:
+        raise ValueError(f"{op}: packed and out must have a contiguous, 16-byte aligned last dimension")
+    if s * hl:
+        # (Sizes of one never step: any positive batch stride will do.)
+        views = [(base + 2 * i * head_dim, s * row, row, head) for i in range(3)]
+        _select_and_attend((1, s, s, hl, hl, head_dim, block_q, block_k), top_k, *views,
+                           (to, s * hl * head_dim, out_row, out_head), _opt(lse), (None, None), _opt(keep), scale,
+                           code, packed.get_device())
+    return (out, lse) if return_lse else out

@@ -96,7 +96,7 @@ def fused_residual_gate_rmsnorm_modulate(residual, branch, gate, weight, scale, 
 _FLOAT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _row_stride(t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
+def _rows_at(t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
     """The tensor as rows of ``columns`` (copied only if they do not step evenly) and the step."""
 
     if t.is_contiguous():
@@ -105,15 +105,24 @@ def _row_stride(t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int]:
     return t, t.stride(0)
 
 
-def _table(op: str, t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int, int]:
+def _table_at(op: str, t: torch.Tensor, columns: int) -> tuple[torch.Tensor, int, int]:
     """An AdaLN table, its row stride and its number of rows."""
 
-    if t.shape[-1] != columns:
+    shape = t.shape
+    if shape[-1] != columns:
         raise ValueError(f"{op}: tables must be {columns} wide")
-    if t.dim() == 2 and t.stride(1) == 1:
-        return t, t.stride(0), t.shape[0]
-    t, stride = table_rows(t)
-    return t, stride, 1 if t.dim() == 1 else t.shape[0]
+    if len(shape) == 2:
+        step, unit = t.stride()
+        if unit == 1:
+            return t, step, shape[0]
+    t, step = table_rows(t)
+    return t, step, 1 if t.dim() == 1 else t.shape[0]
+
+
+def _vector(op: str, name: str, t: torch.Tensor, columns: int) -> torch.Tensor:
+    if t.shape != (columns,):
+        raise ValueError(f"{op}: {name} must have shape ({columns},), got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps, residual_scale):
@@ -126,38 +135,36 @@ def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps
     if branch.shape != shape:
         raise ValueError(f"{op}: residual and branch must have the same shape")
     columns = shape[-1]
-    if post_weight.shape != (columns,):
-        raise ValueError(f"{op}: post_weight must have shape ({columns},), got {tuple(post_weight.shape)}")
-    gate, gate_stride, n_table = _table(op, gate, columns)
-    weight_ptr = scale_ptr = shift_ptr = normed_ptr = normed = None
-    scale_stride = shift_stride = 0
+    post_weight = _vector(op, "post_weight", post_weight, columns)
+    gate, gate_step, n_table = _table_at(op, gate, columns)
+    hidden = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+    normed = weight_ptr = scale_ptr = shift_ptr = normed_ptr = None
+    scale_step = shift_step = 0
     if pre is not None:
-        weight, scale, shift = pre
-        if weight.shape != (columns,):
-            raise ValueError(f"{op}: weight must have shape ({columns},), got {tuple(weight.shape)}")
-        weight = weight.contiguous()
-        scale, scale_stride, n_scale = _table(op, scale, columns)
-        shift, shift_stride, n_shift = _table(op, shift, columns)
+        weight = _vector(op, "weight", pre[0], columns)
+        scale, scale_step, n_scale = _table_at(op, pre[1], columns)
+        shift, shift_step, n_shift = _table_at(op, pre[2], columns)
         if n_scale != n_table or n_shift != n_table:
             raise ValueError(f"{op}: gate, scale and shift must have the same rows")
-        weight_ptr, scale_ptr, shift_ptr = weight.data_ptr(), scale.data_ptr(), shift.data_ptr()
         normed = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+        weight_ptr, scale_ptr, shift_ptr = weight.data_ptr(), scale.data_ptr(), shift.data_ptr()
         normed_ptr = normed.data_ptr()
-    hidden = torch.empty(shape, dtype=residual.dtype, device=residual.device)
     cells = hidden.numel()
     if cells == 0:
         return hidden, normed
-    idx = index64(index, residual.device)
-    n_index = idx.numel()
+    device = hidden.get_device()
+    if index is None or index.dtype is not torch.int64 or index.get_device() != device or \
+            not index.is_contiguous():
+        index = index64(index, residual.device)
+    n_index = index.numel()
     if n_index == 0 or n_table == 0:
         raise ValueError(f"{op}: empty index or table")
-    residual, residual_stride = _row_stride(residual, columns)
-    branch, branch_stride = _row_stride(branch, columns)
-    post_weight = post_weight.contiguous()
-    call_on(hidden, "h3b_sandwich_residual_rmsnorm_modulate", hidden.data_ptr(), normed_ptr, residual.data_ptr(),
+    residual, residual_step = _rows_at(residual, columns)
+    branch, branch_step = _rows_at(branch, columns)
+    call_on(device, "h3b_sandwich_residual_rmsnorm_modulate", hidden.data_ptr(), normed_ptr, residual.data_ptr(),
             branch.data_ptr(), post_weight.data_ptr(), gate.data_ptr(), weight_ptr, scale_ptr, shift_ptr,
-            idx.data_ptr(), cells // columns, columns, n_index, n_table, residual_stride, branch_stride, columns,
-            gate_stride, scale_stride, shift_stride, residual_scale, post_eps, eps, code)
+            index.data_ptr(), cells // columns, columns, n_index, n_table, residual_step, branch_step, columns,
+            gate_step, scale_step, shift_step, residual_scale, post_eps, eps, code)
     return hidden, normed
 
 
