@@ -17,6 +17,8 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from dataclasses import dataclass, field
+from typing import Any
 
 import torch
 
@@ -282,3 +284,98 @@ def packed_sparse_attention(packed: torch.Tensor, top_k: int, head_dim: int = HE
                            (to, s * hl * head_dim, out_row, out_head), _opt(lse), (None, None), _opt(keep), scale,
                            code, packed.get_device())
     return (out, lse) if return_lse else out
+
+
+# Where ``install_sparse_attention`` leaves its settings on an attention module, and the packed
+# attention forward looks for them.
+SPARSE_ATTRIBUTE = "_h3b_sparse_attention"
+
+
+@dataclass
+class SparseAttention:
+    """How the packed attention of one transformer is made sparse: every block of ``block_q``
+    queries attends to a ``density`` share of the blocks of ``block_k`` keys (at least
+    ``min_blocks``, and all blocks that hold any of the last ``keep_last_rows`` rows: text and
+    audio rows behind the video)."""
+
+    density: float
+    block_q: int = 128
+    block_k: int = 128
+    keep_last_rows: int = 0
+    min_blocks: int = 1
+    calls: int = 0
+    _keep: dict[tuple[int, int], torch.Tensor] = field(default_factory=dict, repr=False)
+
+    def __post_init__(self) -> None:
+        if not 0.0 < self.density <= 1.0:
+            raise ValueError(f"sparse attention: density must be in (0, 1], got {self.density}")
+        if self.block_q not in BLOCK_Q or self.block_k not in BLOCK_K:
+            raise ValueError(f"sparse attention: block_q must be one of {BLOCK_Q} and block_k one of {BLOCK_K}, got "
+                             f"{self.block_q} and {self.block_k}")
+        if self.keep_last_rows < 0 or self.min_blocks < 1:
+            raise ValueError("sparse attention: keep_last_rows must not be negative, min_blocks at least 1")
+
+    def list_length(self, rows: int) -> int:
+        """Key blocks per list for a sequence of ``rows``."""
+
+        blocks = -(-rows // self.block_k)
+        return min(blocks, max(math.ceil(self.density * blocks), self.min_blocks, self._kept(rows)))
+
+    def _kept(self, rows: int) -> int:
+        kept_rows = min(self.keep_last_rows, rows)
+        return -(-rows // self.block_k) - (rows - kept_rows) // self.block_k if kept_rows else 0
+
+    def _keep_mask(self, rows: int, device: torch.device) -> torch.Tensor | None:
+        if not self.keep_last_rows or not rows:
+            return None
+        key = (rows, device.index)
+        mask = self._keep.get(key)
+        if mask is None:
+            blocks = -(-rows // self.block_k)
+            mask = torch.arange(blocks, device=device) >= blocks - self._kept(rows)
+            if not torch.cuda.is_current_stream_capturing():
+                # Kept for later calls, on whatever stream they run (a captured mask exists
+                # only when its graph has run, and stays the graph's own).
+                torch.cuda.current_stream(device).synchronize()
+                self._keep = {key: mask}  # one sequence length at a time
+        return mask
+
+    def attend(self, packed: torch.Tensor, head_dim: int) -> torch.Tensor:
+        """``packed_sparse_attention`` over the receive buffer [S, hl, 3*D]."""
+
+        rows = packed.shape[0]
+        self.calls += 1
+        return packed_sparse_attention(packed, self.list_length(rows), head_dim, block_q=self.block_q,
+                                       block_k=self.block_k, keep=self._keep_mask(rows, packed.device))
+
+
+def install_sparse_attention(transformer: Any, *, density: float = 0.1, block_q: int = 128, block_k: int = 128,
+                             keep_last_rows: int = 0, min_blocks: int = 1) -> dict[str, Any]:
+    """Make the packed attention of every block sparse (see ``SparseAttention``).
+
+    Call it after ``install_transformer_fusions`` (with ``qknorm_rope``) or
+    ``install_packed_ulysses``: their attention forwards read the settings, also when they are
+    installed again later. On several ranks each selects for its own heads over the whole
+    sequence, so the ranks need not agree on anything. Returns the installation's metadata; its
+    ``"runtime"`` counts calls. ``remove_sparse_attention`` goes back to dense attention."""
+
+    runtime = SparseAttention(density, block_q, block_k, keep_last_rows, min_blocks)
+    modules = [block.attn for block in transformer.transformer_blocks]
+    for attention in modules:
+        if not getattr(attention.__dict__.get("forward"), "h3b_packed", False):
+            raise RuntimeError("sparse attention needs the packed attention forward: call install_transformer_fusions "
+                               "or install_packed_ulysses first")
+        if attention.head_dim not in HEAD_DIMS:
+            raise RuntimeError(f"sparse attention: head_dim must be one of {HEAD_DIMS}, got {attention.head_dim}")
+    for attention in modules:
+        setattr(attention, SPARSE_ATTRIBUTE, runtime)
+    return {"backend": "h3b_block_sparse", "semantics": "sparse", "modules": len(modules), "density": density,
+            "block_q": block_q, "block_k": block_k, "keep_last_rows": keep_last_rows, "runtime": runtime}
+
+
+def remove_sparse_attention(transformer: Any) -> None:
+    """Dense attention again."""
+
+    for block in transformer.transformer_blocks:
+        if hasattr(block.attn, SPARSE_ATTRIBUTE):
+            delattr(block.attn, SPARSE_ATTRIBUTE)

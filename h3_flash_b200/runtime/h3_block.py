@@ -9,6 +9,9 @@ exercised and benchmarked without Diffusers:
   block.norm1, block.norm2                          RMSNorm(d) (weight, eps)
   block.attn.{to_q,to_k,to_v,norm_q,norm_k,to_out,heads,head_dim,processor}
   block.ff.net = [activation-with-.proj, Dropout, Linear]   (GELU-tanh or SwiGLU)
+  block.norm1_post, block.norm2_post, block.residual_scale  (sandwich_norm only: an RMSNorm after
+                                                    each branch, before its gate, and the
+                                                    factor of the residual)
 
 Its own ``forward`` methods are the eager upstream-style math (what a model
 looks like before ``install_transformer_fusions`` / ``install_packed_ulysses``
@@ -144,24 +147,37 @@ class FeedForward(nn.Module):
 class H3TransformerBlock(nn.Module):
     def __init__(self, dim: int = 3072, heads: int = 24, head_dim: int = 128, ffn_inner: int = 12288,
                  activation: str = "gelu-tanh", n_table: int = 3, eps: float = 1e-6, qk_eps: float = 1e-6,
-                 bias: bool = True, **factory) -> None:
+                 bias: bool = True, sandwich_norm: bool = False, residual_scale: float = 1.0, **factory) -> None:
         super().__init__()
+        if residual_scale != 1.0 and not sandwich_norm:
+            raise ValueError("residual_scale needs sandwich_norm")
         self.adaln_proj = AdaLNTable(n_table, dim, **factory)
         self.norm1 = RMSNorm(dim, eps, **factory)
         self.attn = Attention(dim, heads, head_dim, qk_eps, bias, **factory)
         self.norm2 = RMSNorm(dim, eps, **factory)
         self.ff = FeedForward(dim, ffn_inner, activation, bias, **factory)
+        self.residual_scale = residual_scale
+        self.norm1_post = RMSNorm(dim, eps, **factory) if sandwich_norm else None
+        self.norm2_post = RMSNorm(dim, eps, **factory) if sandwich_norm else None
 
     def forward(self, hidden_states, temb, adaln_indices, rotary_emb, attention_mask=None):
-        """Upstream eager math (kernels/transformer.py:70-74, :103-111, :121-126)."""
+        """Upstream eager math (kernels/transformer.py:70-74, :103-111, :121-126); with
+        sandwich_norm each branch passes its own norm before the gate."""
 
         shift_msa, scale_msa, gate_msa, shift_mlp, scale_mlp, gate_mlp = self.adaln_proj(temb)
         pick = lambda t: t.index_select(0, adaln_indices)  # noqa: E731
         normed = self.norm1(hidden_states) * (1.0 + pick(scale_msa)) + pick(shift_msa)
         attention_output = self.attn(normed, rotary_emb, attention_mask)
+        if self.norm1_post is not None:
+            attention_output = self.norm1_post(attention_output)
+            hidden_states = self.residual_scale * hidden_states
         hidden_states = hidden_states + pick(gate_msa) * attention_output
         normed = self.norm2(hidden_states) * (1.0 + pick(scale_mlp)) + pick(shift_mlp)
-        return hidden_states + pick(gate_mlp) * self.ff(normed)
+        feed_forward_output = self.ff(normed)
+        if self.norm2_post is not None:
+            feed_forward_output = self.norm2_post(feed_forward_output)
+            hidden_states = self.residual_scale * hidden_states
+        return hidden_states + pick(gate_mlp) * feed_forward_output
 
 
 class H3BlockStack(nn.Module):

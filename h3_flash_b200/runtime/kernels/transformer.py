@@ -13,6 +13,13 @@ Block math (kernels/transformer.py:50-126):
   h, normed = h + gate_msa[idx]*a, RMSNorm(h)*(1+scale_mlp)+shift_mlp  (fused_residual_gate_rmsnorm_modulate)
   f       = ff(normed)          # SwiGLU (H3) or GELU-tanh (benchmark) activation fused
   return h + gate_mlp[idx]*f                                           (fused_gated_residual)
+
+A block whose branches end in a norm (``block.norm1_post`` and ``block.norm2_post``, a residual
+factor ``block.residual_scale``, as ``H3TransformerBlock(sandwich_norm=True)`` has them) takes
+  h, normed = s*h + gate_msa[idx]*RMSNorm(a), RMSNorm(h)*(1+scale_mlp)+shift_mlp
+                                                       (fused_sandwich_residual_rmsnorm_modulate)
+  return s*h + gate_mlp[idx]*RMSNorm(f)                (fused_sandwich_residual)
+in place of the last two residual lines (inference only).
 """
 
 from __future__ import annotations
@@ -31,6 +38,8 @@ from .fusions import (
     fused_linear_swiglu,
     fused_residual_gate_rmsnorm_modulate,
     fused_rmsnorm_modulate,
+    fused_sandwich_residual,
+    fused_sandwich_residual_rmsnorm_modulate,
     fused_swiglu,
     gemm_supported,
     interleave_swiglu,
@@ -167,6 +176,9 @@ def fused_block_forward(block: Any, hidden_states: torch.Tensor, temb: Any, adal
         normed = normed * (1.0 + scale_msa.index_select(0, adaln_indices)) + shift_msa.index_select(0, adaln_indices)
     attention_output = block.attn(normed, rotary_emb, attention_mask)
     residual_input = hidden_states
+    if getattr(block, "norm1_post", None) is not None:
+        return _sandwich_rest(block, residual_input, attention_output, (gate_msa, scale_mlp, shift_mlp, gate_mlp),
+                              adaln_indices, modulate, swiglu, gate, gemm_epilogue)
     if modulate:
         with TIMER.section("elementwise"):
             hidden_states, normed = fused_residual_gate_rmsnorm_modulate(
@@ -202,6 +214,34 @@ def fused_block_forward(block: Any, hidden_states: torch.Tensor, temb: Any, adal
     return hidden_states + gate_mlp.index_select(0, adaln_indices) * feed_forward_output
 
 
+def _sandwich_rest(block: Any, residual: torch.Tensor, attention_output: torch.Tensor, tables: tuple, indices: torch.Tensor,
+                   modulate: bool, swiglu: bool, gate: dict | None, gemm_epilogue: bool) -> torch.Tensor:
+    """Everything after attention in a block whose branches end in a norm."""
+
+    gate_msa, scale_mlp, shift_mlp, gate_mlp = tables
+    scale_by = float(getattr(block, "residual_scale", 1.0))
+    if modulate:
+        with TIMER.section("elementwise"):
+            hidden, normed = fused_sandwich_residual_rmsnorm_modulate(
+                residual, attention_output, block.norm1_post.weight, gate_msa, block.norm2.weight, scale_mlp,
+                shift_mlp, indices, block.norm1_post.eps, block.norm2.eps, residual_scale=scale_by)
+    if not modulate or (gate is not None and "sandwich_chain" not in gate):
+        eager_hidden = scale_by * residual + gate_msa.index_select(0, indices) * block.norm1_post(attention_output)
+        eager_normed = block.norm2(eager_hidden) * (1.0 + scale_mlp.index_select(0, indices)) + \
+            shift_mlp.index_select(0, indices)
+        if modulate:
+            gate["sandwich_output"] = _error_metrics(hidden, eager_hidden)
+            gate["sandwich_chain"] = _error_metrics(normed, eager_normed)
+        else:
+            hidden, normed = eager_hidden, eager_normed
+    branch = feed_forward(block.ff, normed, swiglu, gate, gemm_epilogue)
+    if modulate:
+        with TIMER.section("elementwise"):
+            return fused_sandwich_residual(hidden, branch, block.norm2_post.weight, gate_mlp, indices,
+                                           block.norm2_post.eps, residual_scale=scale_by)
+    return scale_by * hidden + gate_mlp.index_select(0, indices) * block.norm2_post(branch)
+
+
 def _patch_blocks(transformer: Any, modulate: bool, swiglu: bool, runtime: dict[str, Any]) -> None:
     gemm_epilogue = bool(runtime.get("gemm_epilogue", False))
     for block_index, block in enumerate(transformer.transformer_blocks):
@@ -230,6 +270,7 @@ def _patch_attention(transformer: Any, runtime: dict[str, Any], gemm_pack: bool 
             return ulysses_attention_forward(attention, hidden_states, rotary_emb, attention_mask,
                                              gemm_pack=gemm_pack)
 
+        forward.h3b_packed = True
         attention.forward = forward
 
 

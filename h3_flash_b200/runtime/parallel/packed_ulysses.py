@@ -35,6 +35,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from ..attention.dense import packed_attention
+from ..attention.sparse import SPARSE_ATTRIBUTE, SparseAttention
 from ..kernels.fusions import (
     fused_qknorm_rope,
     fused_qknorm_rope_pack,
@@ -246,7 +247,8 @@ def ulysses_attention_forward(attention: Any, hidden_states: torch.Tensor, rotar
     """The patched ``attn.forward`` body (packed_ulysses.py:150-215). ``runtime=None``
     runs the same data path on one GPU (no exchange). ``gemm_pack``: where the shapes
     allow it, the QKV projection, QK-norm + RoPE and the pack (and, with the p2p
-    exchange, the QKV exchange) run as one GEMM kernel."""
+    exchange, the QKV exchange) run as one GEMM kernel. An attention module that
+    ``install_sparse_attention`` has marked attends to its selected key blocks only."""
 
     if attention_mask is not None:
         raise RuntimeError("packed Ulysses requires padless dense attention")
@@ -260,17 +262,18 @@ def ulysses_attention_forward(attention: Any, hidden_states: torch.Tensor, rotar
     norm_q, norm_k = _norm_params(attention.norm_q), _norm_params(attention.norm_k)
     cos, sin = rotary_emb if rotary_emb is not None else (None, None)
     x2d = hidden_states.reshape(rows_local, -1)
+    sparse = getattr(attention, SPARSE_ATTRIBUTE, None)
     fused_norms = fused_qknorm_rope and norm_q is not None and norm_k is not None
     stacked = qkv_weights(attention) if (gemm_pack and fused_norms) else None
     use_gemm = stacked is not None and qkv_gemm_pack_supported(x2d, stacked[0], heads, head_dim, cos)
     peer = world > 1 and runtime.peer is not None and fused_norms and _p2p_supported(head_dim, cos)
     if peer:
         if use_gemm:
-            output = _peer_attention_gemm(runtime, x2d, stacked, norm_q, norm_k, cos, sin, heads, head_dim)
+            output = _peer_attention_gemm(runtime, x2d, stacked, norm_q, norm_k, cos, sin, heads, head_dim, sparse)
         else:
             with TIMER.section("gemm"):
                 q, k, v = qkv_projection(attention, x2d)
-            output = _peer_attention(runtime, q, k, v, norm_q, norm_k, cos, sin, rows_local, head_dim)
+            output = _peer_attention(runtime, q, k, v, norm_q, norm_k, cos, sin, rows_local, head_dim, sparse)
         output = output.reshape(batch, rows_local, heads * head_dim).type_as(hidden_states)
         runtime.attention_calls += 1
         with TIMER.section("gemm"):
@@ -301,7 +304,7 @@ def ulysses_attention_forward(attention: Any, hidden_states: torch.Tensor, rotar
     else:
         packed = send.view(rows_local, heads, 3 * head_dim)
     with TIMER.section("attention"):
-        output = packed_attention(packed, head_dim)
+        output = packed_attention(packed, head_dim) if sparse is None else sparse.attend(packed, head_dim)
     if world > 1:
         with TIMER.section("all_to_all"):
             output = _packed_output_all_to_all(output, rows_local, runtime)
@@ -318,7 +321,7 @@ def _p2p_supported(head_dim: int, cos: Any) -> bool:
 
 
 def _peer_attention_gemm(runtime: PackedUlyssesRuntime, x2d, stacked, norm_q, norm_k, cos, sin,
-                         heads: int, head_dim: int) -> torch.Tensor:
+                         heads: int, head_dim: int, sparse: SparseAttention | None = None) -> torch.Tensor:
     """qkv_gemm_pack_p2p (projection + QK-norm + RoPE + QKV exchange) -> barrier ->
     attention_p2p (or attention -> scatter_p2p) -> barrier. Returns [r, H, D]."""
 
@@ -327,24 +330,26 @@ def _peer_attention_gemm(runtime: PackedUlyssesRuntime, x2d, stacked, norm_q, no
     with TIMER.section("qkv_gemm_pack"):
         peer.pack_gemm(x2d, stacked[0], stacked[1], norm_q[0], norm_k[0], cos, sin, norm_q[1],
                        norm_k[1], heads, counts)
-    return _peer_exchange_rest(runtime, counts, heads // runtime.world, head_dim)
+    return _peer_exchange_rest(runtime, counts, heads // runtime.world, head_dim, sparse)
 
 
 def _peer_exchange_rest(runtime: PackedUlyssesRuntime, counts: list[int], heads_local: int,
-                        head_dim: int) -> torch.Tensor:
-    """Everything after the pack: barrier, attention with the output exchange, barrier."""
+                        head_dim: int, sparse: SparseAttention | None = None) -> torch.Tensor:
+    """Everything after the pack: barrier, attention with the output exchange, barrier. Sparse
+    attention writes its rows locally and a scatter kernel sends them."""
 
     peer = runtime.peer
     with TIMER.section("all_to_all"):
         peer.barrier()
-    if runtime.fuse_output_exchange:
+    if runtime.fuse_output_exchange and sparse is None:
         with TIMER.section("attention"):
             merged = peer.attention(counts, heads_local, head_dim)
         with TIMER.section("all_to_all"):
             peer.barrier()
         return merged
     with TIMER.section("attention"):
-        output = packed_attention(peer.recv_view(sum(counts), heads_local, head_dim), head_dim)
+        packed = peer.recv_view(sum(counts), heads_local, head_dim)
+        output = packed_attention(packed, head_dim) if sparse is None else sparse.attend(packed, head_dim)
     with TIMER.section("all_to_all"):
         merged = peer.scatter(output, counts)
         peer.barrier()
@@ -352,7 +357,7 @@ def _peer_exchange_rest(runtime: PackedUlyssesRuntime, counts: list[int], heads_
 
 
 def _peer_attention(runtime: PackedUlyssesRuntime, q, k, v, norm_q, norm_k, cos, sin,
-                    rows_local: int, head_dim: int) -> torch.Tensor:
+                    rows_local: int, head_dim: int, sparse: SparseAttention | None = None) -> torch.Tensor:
     """pack_p2p -> barrier -> attention_p2p (output exchange in its epilogue) ->
     barrier, or with ``fuse_output_exchange=False`` attention -> scatter_p2p in
     place of attention_p2p. Returns [r, H, D]."""
@@ -361,7 +366,7 @@ def _peer_attention(runtime: PackedUlyssesRuntime, q, k, v, norm_q, norm_k, cos,
     counts = runtime.row_counts(rows_local)
     with TIMER.section("qknorm_rope_pack"):
         peer.pack(q, k, v, norm_q[0], norm_k[0], cos, sin, norm_q[1], norm_k[1], counts)
-    return _peer_exchange_rest(runtime, counts, q.shape[1] // runtime.world, head_dim)
+    return _peer_exchange_rest(runtime, counts, q.shape[1] // runtime.world, head_dim, sparse)
 
 
 def _single_node_cuda_group(group: Any) -> bool:
@@ -406,6 +411,7 @@ def install_packed_ulysses(transformer: Any, *, group: Any = None, fused_qknorm_
                     runtime=runtime, fused_qknorm_rope=fused_qknorm_rope, gemm_pack=gemm_pack,
                 )
 
+            forward.h3b_packed = True
             attention.forward = forward
 
     with_context_parallel_reapplied(transformer, apply)
