@@ -31,7 +31,9 @@
 // O, so the softmax of unit u + 1 has its scores while P V of unit u and the scores of u + 2
 // are computed; with units of 128 keys TMEM holds one buffer, and each tile's softmax and
 // MMAs wait for one another. The price is that an N = 64 score MMA reads its Q operand from
-// shared memory for half as many columns.
+// shared memory for half as many columns. Measured on 592 pairs of tiles x 4, 64 blocks a
+// list, under the power cap: 590 us with one list per pair and 640 us with a list per tile,
+// against 678 and 694 us with units of 128 keys.
 //
 // TMEM (512 columns): S of tile t, buffer b at 128 t + 64 b; O of tile t at 256 + 128 t.
 //
