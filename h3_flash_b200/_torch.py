@@ -107,6 +107,12 @@ def ptr(t: torch.Tensor) -> int:
     return t.data_ptr()
 
 
+def scratch(size: int, device: torch.device) -> torch.Tensor:
+    """``size`` bytes of device memory. (empty_strided parses a call in two thirds of empty's time.)"""
+
+    return torch.empty_strided((size,), (1,), dtype=torch.uint8, device=device)
+
+
 def call(name: str, *args) -> None:
     _lib.call(name, *args)
 

@@ -22,7 +22,7 @@ from typing import Any
 
 import torch
 
-from ..._torch import call, call_on, check_inputs, require_cuda
+from ..._torch import call, call_on, check_inputs, require_cuda, scratch
 from .dense import HEAD_DIM
 
 BLOCK_Q = (128, 256)
@@ -85,6 +85,12 @@ def _bytes(name: str, *shape: int) -> int:
     return value.value
 
 
+def _new_out(q: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor like q. (empty_like of a contiguous one takes half empty's host time.)"""
+
+    return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
 def _list_length(op: str, top_k: int, blocks: int) -> int:
     if isinstance(top_k, bool) or not isinstance(top_k, int) or top_k < 1:
         raise ValueError(f"{op}: top_k must be a positive integer, got {top_k!r}")
@@ -134,14 +140,15 @@ def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: 
     q_lens = _side_tensor(op, "q_lens", q_lens, torch.int32, (b,), q.device)
     k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
     keep = _side_tensor(op, "keep", keep, torch.bool, (nk,), q.device)
-    indices = torch.empty((b, h, nq, top_k), dtype=torch.int32, device=q.device)
-    counts = torch.empty((b, h, nq), dtype=torch.int32, device=q.device)
+    indices = torch.empty_strided((b, h, nq, top_k), (h * nq * top_k, nq * top_k, top_k, 1), dtype=torch.int32,
+                                  device=q.device)
+    counts = torch.empty_strided((b, h, nq), (h * nq, nq, 1), dtype=torch.int32, device=q.device)
     if counts.numel() == 0:
         return indices, counts
     if not sk:
         raise ValueError(f"{op}: empty key sequence")
     need = _bytes("h3b_select_key_blocks_workspace_size", b, sq, sk, h, hk, d, block_q, block_k)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws = scratch(need, q.device)
     _select((b, sq, sk, h, hk, d, block_q, block_k, top_k), _view(op, "q", q), _view(op, "k", k),
             (indices.data_ptr(), counts.data_ptr()), (_opt(q_lens), _opt(k_lens)), _opt(keep), code, ws.data_ptr(),
             need, q.get_device())
@@ -178,10 +185,11 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     q_lens = _side_tensor(op, "q_lens", q_lens, torch.int32, (b,), q.device)
     k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
     if out is None:
-        out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+        out = _new_out(q)
     elif out.shape != q.shape:
         raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
-    lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty_strided((b, h, sq), (h * sq, sq, 1), dtype=torch.float32,
+                              device=q.device) if return_lse else None
     scale = _scale(op, softmax_scale, d)
     if b * sq * h and (sk == 0 or entries == 0):
         out.zero_()
@@ -189,7 +197,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
             lse.fill_(-math.inf)
     elif b * sq * h:
         need = _bytes("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, entries)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        ws = scratch(need, q.device) if need else None
         _attend((b, sq, sk, h, hk, d, block_q, block_k), entries, _view(op, "q", q), _view(op, "k", k),
                 _view(op, "v", v), _view(op, "out", out), _opt(lse), (indices.data_ptr(), _opt(counts)),
                 (_opt(q_lens), _opt(k_lens)), scale, code, _opt(ws), need, q.get_device())
@@ -204,11 +212,11 @@ def _select_and_attend(dims, top_k, q, k, v, out, lse, lens, keep, scale, code, 
     lists = (4 * rows * (top_k + 1) + 255) // 256 * 256
     first = _bytes("h3b_select_key_blocks_workspace_size", *dims)
     second = _bytes("h3b_block_sparse_attention_workspace_size", b, sq, h, d, block_k, top_k)
-    ws = torch.empty(lists + max(first, second), dtype=torch.uint8, device=device)
+    ws = scratch(lists + max(first, second), device)
     at = ws.data_ptr()
     pair = (at, at + 4 * rows * top_k)
-    _select((*dims, top_k), q, k, pair, lens, keep, code, at + lists, first, device)
-    _attend(dims, top_k, q, k, v, out, lse, pair, lens, scale, code, at + lists, second, device)
+    _select((*dims, top_k), q, k, pair, lens, keep, code, at + lists, first, device.index)
+    _attend(dims, top_k, q, k, v, out, lse, pair, lens, scale, code, at + lists, second, device.index)
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int, *, block_q: int = 128,
@@ -229,17 +237,18 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: i
     k_lens = _side_tensor(op, "k_lens", k_lens, torch.int32, (b,), q.device)
     keep = _side_tensor(op, "keep", keep, torch.bool, (nk,), q.device)
     if out is None:
-        out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+        out = _new_out(q)
     elif out.shape != q.shape:
         raise ValueError(f"{op}: out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
-    lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty_strided((b, h, sq), (h * sq, sq, 1), dtype=torch.float32,
+                              device=q.device) if return_lse else None
     scale = _scale(op, softmax_scale, d)
     if b * sq * h:
         if not sk:
             raise ValueError(f"{op}: empty key sequence")
         _select_and_attend((b, sq, sk, h, hk, d, block_q, block_k), top_k, _view(op, "q", q), _view(op, "k", k),
                            _view(op, "v", v), _view(op, "out", out), _opt(lse), (_opt(q_lens), _opt(k_lens)),
-                           _opt(keep), scale, code, q.get_device())
+                           _opt(keep), scale, code, q.device)
     return (out, lse) if return_lse else out
 
 
@@ -282,7 +291,7 @@ def packed_sparse_attention(packed: torch.Tensor, top_k: int, head_dim: int = HE
         views = [(base + 2 * i * head_dim, s * row, row, head) for i in range(3)]
         _select_and_attend((1, s, s, hl, hl, head_dim, block_q, block_k), top_k, *views,
                            (to, s * hl * head_dim, out_row, out_head), _opt(lse), (None, None), _opt(keep), scale,
-                           code, packed.get_device())
+                           code, packed.device)
     return (out, lse) if return_lse else out
 
 

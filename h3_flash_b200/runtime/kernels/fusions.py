@@ -137,7 +137,9 @@ def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps
     columns = shape[-1]
     post_weight = _vector(op, "post_weight", post_weight, columns)
     gate, gate_step, n_table = _table_at(op, gate, columns)
-    hidden = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+    # (empty_like of a contiguous tensor takes half the host time of empty.)
+    hidden = torch.empty_like(residual) if residual.is_contiguous() else torch.empty(
+        shape, dtype=residual.dtype, device=residual.device)
     normed = weight_ptr = scale_ptr = shift_ptr = normed_ptr = None
     scale_step = shift_step = 0
     if pre is not None:
@@ -146,7 +148,7 @@ def _sandwich(op, residual, branch, post_weight, gate, pre, index, post_eps, eps
         shift, shift_step, n_shift = _table_at(op, pre[2], columns)
         if n_scale != n_table or n_shift != n_table:
             raise ValueError(f"{op}: gate, scale and shift must have the same rows")
-        normed = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+        normed = torch.empty_like(hidden)
         weight_ptr, scale_ptr, shift_ptr = weight.data_ptr(), scale.data_ptr(), shift.data_ptr()
         normed_ptr = normed.data_ptr()
     cells = hidden.numel()
