@@ -929,8 +929,9 @@ extern "C" int h3b_select_key_blocks(
   H3B_REQUIRE(h3b::aligned16(q) && h3b::aligned16(k), "select_key_blocks: q and k must be 16-byte aligned");
   const int64_t strides[6] = {q_batch_stride, q_row_stride, q_head_stride,
                               k_batch_stride, k_row_stride, k_head_stride};
+  const int64_t sizes[6] = {batch, seq_q, heads, batch, seq_k, kv_heads};
   for (int i = 0; i < 6; ++i)
-    H3B_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0,
+    H3B_REQUIRE(sizes[i] == 1 || (strides[i] % 8 == 0 && strides[i] >= 0),
                 "select_key_blocks: strides must be multiples of 8 elements");
   int rc = h3b_select_key_blocks_workspace_size(batch, seq_q, seq_k, heads, kv_heads, head_dim,
                                                 block_q, block_k, &need);

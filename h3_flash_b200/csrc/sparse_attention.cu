@@ -983,7 +983,7 @@ extern "C" int h3b_block_sparse_attention(
               (long long)heads, (long long)kv_heads);
   H3B_REQUIRE(softmax_scale > 0.f && std::isfinite(softmax_scale),
               "block_sparse_attention: softmax_scale must be positive and finite");
-  H3B_REQUIRE(seq_q < (1LL << 31) - 256 && seq_k < (1LL << 31) - 256 && list_len < (1LL << 30) &&
+  H3B_REQUIRE(seq_q < (1LL << 31) - 256 && seq_k < (1LL << 31) - 256 && list_len <= (1LL << 20) &&
                   batch <= (1LL << 24) / heads &&
                   ((seq_q + 255) / 256) * heads * batch < (1LL << 30),
               "block_sparse_attention: shape exceeds launch limits");

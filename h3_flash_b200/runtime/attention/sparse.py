@@ -167,7 +167,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     first ``counts`` entries of a list count (all of them without ``counts``), in any order. An
     entry outside the key blocks adds nothing, an entry that is there twice counts twice. Query
     rows that have no key, and rows behind ``q_lens``, get zeros (lse -inf). Returns
-    [B, Sq, H, D] (``out`` if given), and with ``return_lse`` the fp32 [B, H, Sq] logarithms of
+    [B, Sq, H, D] (``out`` if given, which must not overlap an input), and with ``return_lse`` the fp32 [B, H, Sq] logarithms of
     the softmax sums."""
 
     op = "block_sparse_attention"
@@ -328,7 +328,8 @@ class SparseAttention:
         """Key blocks per list for a sequence of ``rows``."""
 
         blocks = -(-rows // self.block_k)
-        return min(blocks, max(math.ceil(self.density * blocks), self.min_blocks, self._kept(rows)))
+        share = math.ceil(self.density * blocks - 1e-9)  # 0.1 * 30 is a little more than 3
+        return min(blocks, max(share, self.min_blocks, self._kept(rows)))
 
     def _kept(self, rows: int) -> int:
         kept_rows = min(self.keep_last_rows, rows)

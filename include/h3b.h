@@ -325,7 +325,8 @@ int h3b_select_key_blocks_workspace_size(int64_t batch, int64_t seq_q, int64_t s
 /* out = softmax(q k^T * softmax_scale) v over the keys of the listed blocks.
  * indices int32 [batch, heads, nq, list_len]: the first counts[...] entries of a list
  * count (counts int32 [batch, heads, nq], or NULL: all of them), in any order; an
- * entry outside [0, nk) adds nothing, an entry that is there twice counts twice.
+ * entry outside [0, nk) adds nothing, an entry that is there twice counts twice; list_len is
+ * at most 2^20. out must not overlap an input.
  * Query rows that have no key, and rows behind q_lens, get zeros. lse (fp32
  * [batch, heads, seq_q], or NULL) gets log(sum(exp(score))), -inf for those rows.
  * softmax_scale must be positive and finite. workspace as for h3b_attention

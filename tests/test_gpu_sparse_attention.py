@@ -182,6 +182,80 @@ def test_padded_batch_with_nan(d, block_k):
     _check(block_sparse_attention(q, k, v, got, n, **kw), None, q, k, v, got, n, **kw)
 
 
+@pytest.mark.parametrize("sq", [1, 100, 129, 300, 385, 640])
+def test_lists_per_256_rows_with_odd_tiles(sq):
+    """A list that serves one tile only (the other lies behind the rows), whole and split; a
+    padded batch on top."""
+
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention, select_key_blocks
+
+    b, sk, h = 3, 1100, 2
+    q, k, v = _randn((b, sq, h, 128), 1), _randn((b, sk, h, 128), 2), _randn((b, sk, h, 128), 3)
+    q_lens = torch.tensor([sq, max(0, sq - 130), sq // 2], dtype=torch.int32, device="cuda")
+    k_lens = torch.tensor([sk, 700, 1000], dtype=torch.int32, device="cuda")
+    for block_k in (64, 128):
+        indices, counts = _lists(b, h, -(-sq // 256), -(-sk // block_k), 7, 4)
+        kw = dict(block_q=256, block_k=block_k)
+        out, lse = block_sparse_attention(q, k, v, indices, counts, return_lse=True, **kw)
+        _check(out, lse, q, k, v, indices, counts, **kw)
+        out, lse = block_sparse_attention(q, k, v, indices, counts, q_lens=q_lens, k_lens=k_lens, return_lse=True, **kw)
+        _check(out, lse, q, k, v, indices, counts, q_lens=q_lens, k_lens=k_lens, **kw)
+        got, n = select_key_blocks(q, k, 5, q_lens=q_lens, k_lens=k_lens, **kw)
+        ref, ref_n = sparse_ref.select(q, k, 5, q_lens=q_lens, k_lens=k_lens, **kw)
+        assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
+
+
+@pytest.mark.parametrize("sq", [1, 200, 700])
+def test_without_a_workspace(sq):
+    """A caller of the C entry point that gives none: every list whole, the same result."""
+
+    from h3_flash_b200 import _lib
+
+    h, sk, n = 3, 2000, 12
+    q, k, v = _randn((1, sq, h, 128), 1), _randn((1, sk, h, 128), 2), _randn((1, sk, h, 128), 3)
+    indices, _ = _lists(1, h, -(-sq // 128), -(-sk // 128), n, 4)
+    for missing in (True, False):
+        out, lse = torch.empty_like(q), torch.empty(1, h, sq, device="cuda")
+        ws = torch.empty(64, dtype=torch.uint8, device="cuda")  # too short
+        _lib.call("h3b_block_sparse_attention", out.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  indices.data_ptr(), None, n, 1, sq, sk, h, h, 128, 128, 128, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                  *out.stride()[:3], None, None, 128**-0.5, 0, None if missing else ws.data_ptr(), 0 if missing else 64,
+                  torch.cuda.current_stream().cuda_stream)
+        _check(out, lse, q, k, v, indices, None)
+
+
+def test_large_batch_of_single_rows():
+    """More items than SMs, each one query row: halves of a list on the two tiles of an item."""
+
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
+
+    b, h, hk, sk = 40, 8, 2, 520
+    q, k, v = _randn((b, 1, h, 64), 1), _randn((b, sk, hk, 64), 2), _randn((b, sk, hk, 64), 3)
+    indices, counts = _lists(b, h, 1, 9, 9, 4)
+    k_lens = torch.randint(0, sk + 1, (b,), device="cuda", generator=torch.Generator("cuda").manual_seed(5)).int()
+    out, lse = block_sparse_attention(q, k, v, indices, counts, block_k=64, k_lens=k_lens, return_lse=True)
+    _check(out, lse, q, k, v, indices, counts, block_k=64, k_lens=k_lens)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams do not share scratch."""
+
+    from h3_flash_b200.runtime.attention.sparse import sparse_attention
+
+    sets = [tuple(_randn((1, 3000, 4, 128), 10 * i + j) for j in range(3)) for i in range(2)]
+    want = [sparse_attention(*s, 5) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (stream, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append(sparse_attention(*s, 5))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_entries_outside_and_twice():
     from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
 

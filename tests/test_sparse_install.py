@@ -18,6 +18,7 @@ def _stack(**kw):
 def test_list_length():
     s = SparseAttention(0.1)
     assert [s.list_length(n) for n in (1, 128, 129, 1280, 51200)] == [1, 1, 1, 1, 40]
+    assert SparseAttention(0.1).list_length(30 * 128) == 3
     s = SparseAttention(0.1, block_k=64, keep_last_rows=130, min_blocks=5)
     assert s.list_length(64 * 100) == 10
     assert s.list_length(64 * 10) == 5

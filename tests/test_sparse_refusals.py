@@ -68,6 +68,8 @@ def test_attend_refusals():
             _attend(scale=scale)
     with pytest.raises(ValueError, match="empty lists"):
         _attend(n=0)
+    with pytest.raises(ValueError, match="launch limits"):
+        _attend(n=2**20 + 1)
     with pytest.raises(ValueError, match="positive multiples of 8"):
         _attend(strides=(8, 8, 8, 8, 0, 8, 8, 8, 8, 8, 8, 8))
     with pytest.raises(ValueError, match="null argument"):
