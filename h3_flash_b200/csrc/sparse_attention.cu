@@ -8,11 +8,14 @@
 // The unit of work along a list is 64 keys: a listed block of 64, or half of one of 128. A
 // work item is a pair of neighbouring 128-row query tiles of one (batch, head), or a range
 // of units of such a pair; where the queries are one tile (a few rows against a long list)
-// the two tiles of an item are that tile with two ranges of its list. CTAs are persistent:
-// item i runs on CTA i mod gridDim, and the loads of an item start while the one before ends.
+// the two tiles of an item are that tile with two ranges of its list. The grid has a CTA per
+// item, but a CTA that nears its item's end takes over the next one that has not started
+// (cluster launch control), and its loads start while the one before ends: lists and padded
+// batches are uneven, and items that are dealt out beforehand leave SMs idle (a batch of 4097,
+// 0, 3700 and 2900 rows with lists of 0 to 12 blocks: 32 us dealt out, DYNAMIC_US us taken over).
 //
-//   warp 8      loads: what an item is, read from global memory one item ahead and handed to
-//               the other warps through shared memory; its Q tiles; then a ring of slots. Slot u of a tile holds
+//   warp 8      loads: what an item is, read from global memory and handed to the other warps
+//               through shared memory; its Q tiles; then a ring of slots. Slot u of a tile holds
 //               V of unit u and K of unit u + 2, which the tile's MMA warp reads one after
 //               the other (a first slot holds K of units 0 and 1). Where the tiles of a pair
 //               have one list (block_q = 256) one slot serves both; with lists of their own
@@ -78,7 +81,7 @@ constexpr float kRescaleThreshold = 8.0f;
 
 // What the MMA and softmax warps know of an item.
 struct Info {
-  int batch, head, row0[kTiles];  // first query row of the tiles
+  int batch, head, row0[kTiles];  // first query row of the tiles; batch < 0: no more items
   int q_rows;                     // rows of the batch entry that exist
   int units[kTiles];
   int part;  // workspace part of tile 0 (tile 1: the next), or -1: rows are final
@@ -98,9 +101,10 @@ struct Layout {
   static constexpr uint32_t kSmemQ = 0;
   static constexpr uint32_t kSmemRing = kTiles * kQBytes;
   static constexpr uint32_t kSmemBar = kSmemRing + kSlots * kSlotBytes;
-  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2][2] fix ifull[2] iempty[2] full[slots] empty[slots]
-  static constexpr int kNumBars = 21 + 2 * kSlots;
-  static constexpr uint32_t kSmemInfo = kSmemBar + kNumBars * 8;           // Info[2]
+  // qfull[2] qempty[2] s[2][2] p[2][2] pv[2][2] fix ifull[2] iempty[2] next full[slots] empty[slots]
+  static constexpr int kNumBars = 22 + 2 * kSlots;
+  static constexpr uint32_t kSmemNext = (kSmemBar + kNumBars * 8 + 15) / 16 * 16;  // 16 bytes
+  static constexpr uint32_t kSmemInfo = kSmemNext + 16;                    // Info[2]
   static constexpr uint32_t kSmemKeys = kSmemInfo + 2 * sizeof(Info);      // u8 [2][kKeyRing]
   static constexpr uint32_t kSmemTag = kSmemKeys + kTiles * kKeyRing;      // u32 [slots]
   static constexpr uint32_t kSmemTail = kSmemTag + 4 * kSlots;             // tmem slot, abort flag
@@ -209,7 +213,8 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return pack_bf16(lo, hi);
 }
 
-template <bool FP16, int D, int BK>
+// SHARED: the tiles of a pair have one list (block_q = 256), and one slot serves both.
+template <bool FP16, int D, int BK, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
     sparse_fwd(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map, const Params prm) {
@@ -229,8 +234,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t bar_fix = bars + 8u * 16;
   auto bar_ifull = [&](uint32_t i) { return bars + 8u * (17 + (i & 1)); };
   auto bar_iempty = [&](uint32_t i) { return bars + 8u * (19 + (i & 1)); };
-  auto bar_full = [&](int s) { return bars + 8u * (21 + s); };
-  auto bar_empty = [&](int s) { return bars + 8u * (21 + kSlots + s); };
+  const uint32_t bar_next = bars + 8u * 21;
+  auto bar_full = [&](int s) { return bars + 8u * (22 + s); };
+  auto bar_empty = [&](int s) { return bars + 8u * (22 + kSlots + s); };
   volatile Info* info = reinterpret_cast<volatile Info*>(smem + L::kSmemInfo);
   volatile uint8_t* key_ring = smem + L::kSmemKeys;  // [tile][unit % kKeyRing]
   volatile uint32_t* slot_tag = reinterpret_cast<uint32_t*>(smem + L::kSmemTag);
@@ -253,9 +259,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(bar_full(s), 1);
       slot_tag[s] = 0xffffffffu;
-      mbar_init(bar_empty(s), prm.duo ? 1 : prm.tiles_per_list);  // the tiles that read a slot
+      mbar_init(bar_empty(s), SHARED ? 2 : 1);  // the tiles that read a slot
     }
     mbar_init(bar_fix, 1);
+    mbar_init(bar_next, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_ifull(i), 1);
       mbar_init(bar_iempty(i), kSoftmaxWarps + kTiles);
@@ -287,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Slots are filled and read in one order; `pos` counts them since the start.
   auto slot_of = [](uint32_t pos) { return (int)(pos % kSlots); };
   auto phase_of = [](uint32_t pos) { return (pos / kSlots) & 1u; };
-  const bool shared = prm.tiles_per_list == kTiles && !prm.duo;  // one slot serves both tiles
   // The next item of this warp, `i` counting them: read from shared memory, then released.
+  // False at the end.
   auto take_info = [&](uint32_t i, Info& it) -> bool {
     if (!wait_all(bar_ifull(i), (i >> 1) & 1)) return false;
     const volatile Info& src = info[i & 1];
@@ -302,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     it.part = src.part;
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_iempty(i));
-    return true;
+    return it.batch >= 0;
   };
 
   if (warp == kLoadWarp) {
@@ -320,12 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     Walk walk[kTiles];
     walk[0].keys_at = walk[1].keys_at = 0;
-    Item following;
-    if ((int)blockIdx.x < prm.n_items) following.load(prm, blockIdx.x, lane);
     uint32_t n_items = 0;
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
-      const Item it = following;
-      if (item + (int)gridDim.x < prm.n_items) following.load(prm, item + gridDim.x, lane);
+    uint32_t next_phase = 0;
+    for (int item = blockIdx.x; item >= 0 && ok; ++n_items) {
+      Item it;
+      it.load(prm, item, lane);
       const int kv_head = it.head / prm.group;
       const int k_rows = it.k_rows(prm);
       auto entry = [&](Walk& w, int unit) -> int {  // called with ascending units
@@ -351,7 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         w.e[1] = entry(w, 1);
         w.e[2] = entry(w, 2);
       }
-      if (!wait_all(bar_iempty(n_items), ((n_items >> 1) & 1) ^ 1)) break;
+      ok = wait_all(bar_iempty(n_items), ((n_items >> 1) & 1) ^ 1);
+      if (!ok) break;
       if (lane == 0) {
         volatile Info& dst = info[n_items & 1];
         dst.batch = it.batch;
@@ -391,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           reader.keys_at += (first ? 1u : 0u) + (two ? 1u : 0u);
         };
         hand_keys(w, t);
-        if (shared && walk[1].units > 0) hand_keys(walk[1], 1);
+        if (SHARED && walk[1].units > 0) hand_keys(walk[1], 1);
         if (elect_one()) {
           slot_tag[slot] = pos;
           const uint32_t bar = cut ? bar_fix : full;
@@ -442,19 +449,60 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.row0[t], it.batch);
         }
         __syncwarp();
-        if (t == 0 || !shared) ok = push(t, -1);
+        if (t == 0 || !SHARED) ok = push(t, -1);
       }
       const int units = max(walk[0].units, walk[1].units);
+      // Asks for the next item two units before the last: late enough to leave it to a CTA
+      // that is free sooner, early enough to have the answer when this item's loads are out.
+      const int ask = max(units - 2, 0);
+      auto request = [&]() {
+        if (elect_one()) {
+          mbar_expect_tx(bar_next, 16);
+          asm volatile(
+              "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+              "[%0], [%1];" ::"r"(sbase + L::kSmemNext),
+              "r"(bar_next)
+              : "memory");
+        }
+        __syncwarp();
+      };
+      if (units == 0) request();
       for (int u = 0; u < units && ok; ++u) {
+        if (u == ask) request();
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           Walk& w = walk[t];
-          if (u < w.units && ok && (t == 0 || !shared)) ok = push(t, u);
+          if (u < w.units && ok && (t == 0 || !SHARED)) ok = push(t, u);
           w.e[0] = w.e[1];
           w.e[1] = w.e[2];
           w.e[2] = entry(w, u + 3);
         }
       }
+      ok = ok && wait_all(bar_next, next_phase);
+      if (!ok) break;
+      next_phase ^= 1;
+      uint32_t taken, cta;
+      asm volatile(
+          "{\n\t.reg .b128 answer;\n\t.reg .pred p;\n\t"
+          "ld.shared.b128 answer, [%2];\n\t"
+          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t"
+          "mov.u32 %1, 0;\n\t"
+          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, answer;\n\t}"
+          : "=r"(taken), "=r"(cta)
+          : "r"(sbase + L::kSmemNext)
+          : "memory");
+      // The answer has been read before the next one may be written.
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      item = taken ? (int)cta : -1;
+    }
+    if (ok && wait_all(bar_iempty(n_items), ((n_items >> 1) & 1) ^ 1)) {
+      if (lane == 0) {
+        info[n_items & 1].batch = -1;
+        mbar_arrive(bar_ifull(n_items));
+      }
+      __syncwarp();
     }
   } else if (warp >= kMmaWarp) {
     // ---------------- MMA issuer of tile t ----------------
@@ -475,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // parity of that phase is the one it would take for its own: the tag comes first.
     auto wait_slot = [&](uint32_t at) -> bool {
       const int slot = slot_of(at);
-      if (!shared && __any_sync(0xffffffffu, slot_tag[slot] != at)) {
+      if (!SHARED && __any_sync(0xffffffffu, slot_tag[slot] != at)) {
         const unsigned long long t0 = globaltimer();
         while (__any_sync(0xffffffffu, slot_tag[slot] != at)) {
           const bool late = globaltimer() - t0 > kWaitLimitNs;
@@ -500,8 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mma_commit(bar_s(t, n_s & 1));
     };
-    uint32_t n_items = 0;
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
+    for (uint32_t n_items = 0; ok; ++n_items) {
       Info it;
       if (!take_info(n_items, it)) break;
       const int units0 = it.units[0], units1 = it.units[1];
@@ -509,14 +556,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Where this tile's slots are: its first at base + lead, slot u at `next`, which steps
       // over the other tile's while that has units left.
       const int other = t == 0 ? units1 : units0;
-      const uint32_t lead = t == 1 && !shared && units0 > 0 ? 1u : 0u;
-      const uint32_t firsts = shared ? 1u : (units0 > 0) + (units1 > 0);
-      uint32_t next = base + firsts + (t == 1 && !shared && units0 > 0 ? 1u : 0u);
+      const uint32_t lead = t == 1 && !SHARED && units0 > 0 ? 1u : 0u;
+      const uint32_t firsts = SHARED ? 1u : (units0 > 0) + (units1 > 0);
+      uint32_t next = base + firsts + (t == 1 && !SHARED && units0 > 0 ? 1u : 0u);
       const uint32_t slots = units0 == 0 && units1 == 0 ? 0u
-                             : firsts + (shared ? max(units0, units1) : units0 + units1);
+                             : firsts + (SHARED ? max(units0, units1) : units0 + units1);
       auto release = [&](int slot) {  // one lane
         mma_commit(bar_empty(slot));
-        if (shared && other == 0) mma_commit(bar_empty(slot));  // nobody else reads it
+        if (SHARED && other == 0) mma_commit(bar_empty(slot));  // nobody else reads it
       };
       if (units > 0) {
         const uint32_t first = base + lead;
@@ -559,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n_pv;
         if (u + 2 < units) ++n_s;
         // Slots in order: unit u of tile 0, of tile 1, unit u + 1 of tile 0, ...
-        if (shared) {
+        if (SHARED) {
           next += 1;
         } else {
           next += 1u + (t == 0 ? u < other : u + 1 < other);
@@ -578,8 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 c2 = make_float2(c, c);
     uint32_t n = 0;  // units so far: buffer n & 1, phase n >> 1
     bool ok = true;
-    uint32_t n_items = 0;
-    for (int item = blockIdx.x; item < prm.n_items && ok; item += gridDim.x, ++n_items) {
+    for (uint32_t n_items = 0; ok; ++n_items) {
       Info it;
       if (!take_info(n_items, it)) break;
       const int units = t == 0 ? it.units[0] : it.units[1];
@@ -594,11 +640,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         mbar_arrive(bar_p(t, n & 1));
       }
+      // Whether this unit's scores were seen complete halfway through the last one's
+      // exponentials: a wait costs 90 to 180 clocks even where nothing is left to wait for.
+      // With shared slots a test that does not suspend is the faster one, with slots per tile
+      // the one that may (565 and 587 us against 637 and 609 us; without either 580 and 628).
+      bool ready = false;
       for (int u = 0; !idle && u < units; ++u, ++n) {
         const uint32_t t_s = tmem + lanes + kTmemS + t * 128 + (n & 1) * 64;
         // tcgen05.ld/st below are warp-collective.
-        ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
-        if (!ok) break;
+        if (!__all_sync(0xffffffffu, ready)) {
+          ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
+          if (!ok) break;
+        }
         tc_fence_after();
         const int keys = key_ring[t * kKeyRing + n % kKeyRing];
         uint32_t sv[2][32];
@@ -651,6 +704,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
+          if (i == 16) {
+            const uint32_t bar = bar_s(t, (n + 1) & 1), parity = ((n + 1) >> 1) & 1;
+            ready = u + 1 < units && (SHARED ? mbar_test(bar, parity) : mbar_try(bar, parity));
+          }
           const uint32_t* src = sv[i >> 4] + 2 * (i & 15);
           const float2 x = __ffma2_rn(
               make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, nm2);
@@ -900,13 +957,13 @@ int make_map(CUtensorMap* map, const void* base, int64_t batch, int64_t seq, int
   return H3B_OK;
 }
 
-template <bool FP16, int D, int BK>
+template <bool FP16, int D, int BK, bool SHARED>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p,
            int split_pairs, cudaStream_t stream) {
   static ContextSlot slots[kMaxDevices];
   cudaError_t e = cudaErrorInvalidDevice;
   if (context_cached(slots, [&]() -> void* {
-        e = cudaFuncSetAttribute(sparse_fwd<FP16, D, BK>,
+        e = cudaFuncSetAttribute(sparse_fwd<FP16, D, BK, SHARED>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)Layout<D>::kSmemAlloc);
         return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
@@ -915,8 +972,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
               cudaGetErrorString(e));
     return H3B_ERR_CUDA;
   }
-  const unsigned grid = (unsigned)std::min(p.n_items, num_sms());
-  launch_after(sparse_fwd<FP16, D, BK>, dim3(grid), kThreads, Layout<D>::kSmemAlloc, stream, qm, km,
+  launch_after(sparse_fwd<FP16, D, BK, SHARED>, dim3((unsigned)p.n_items), kThreads, Layout<D>::kSmemAlloc, stream, qm, km,
                vm, p);
   int rc = check_launch("h3b_block_sparse_attention");
   if (rc != H3B_OK || split_pairs == 0) return rc;
@@ -926,14 +982,22 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   return check_launch("h3b_block_sparse_attention");
 }
 
+template <bool FP16, int D, int BK>
+int launch_lists(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
+                 const Params& p, int split_pairs, cudaStream_t s) {
+  return p.tiles_per_list == kTiles && !p.duo
+             ? launch<FP16, D, BK, true>(qm, km, vm, p, split_pairs, s)
+             : launch<FP16, D, BK, false>(qm, km, vm, p, split_pairs, s);
+}
+
 template <bool FP16>
 int launch_dims(int64_t head_dim, int64_t block_k, const CUtensorMap& qm, const CUtensorMap& km,
                 const CUtensorMap& vm, const Params& p, int split_pairs, cudaStream_t s) {
   if (head_dim == 128)
-    return block_k == 128 ? launch<FP16, 128, 128>(qm, km, vm, p, split_pairs, s)
-                          : launch<FP16, 128, 64>(qm, km, vm, p, split_pairs, s);
-  return block_k == 128 ? launch<FP16, 64, 128>(qm, km, vm, p, split_pairs, s)
-                        : launch<FP16, 64, 64>(qm, km, vm, p, split_pairs, s);
+    return block_k == 128 ? launch_lists<FP16, 128, 128>(qm, km, vm, p, split_pairs, s)
+                          : launch_lists<FP16, 128, 64>(qm, km, vm, p, split_pairs, s);
+  return block_k == 128 ? launch_lists<FP16, 64, 128>(qm, km, vm, p, split_pairs, s)
+                        : launch_lists<FP16, 64, 64>(qm, km, vm, p, split_pairs, s);
 }
 
 }  // namespace sparse
