@@ -12,7 +12,7 @@
 // item, but a CTA that nears its item's end takes over the next one that has not started
 // (cluster launch control), and its loads start while the one before ends: lists and padded
 // batches are uneven, and items that are dealt out beforehand leave SMs idle (a batch of 4097,
-// 0, 3700 and 2900 rows with lists of 0 to 12 blocks: 32 us dealt out, DYNAMIC_US us taken over).
+// 0, 3700 and 2900 rows with lists of 0 to 12 blocks: 33 us dealt out, 26.5 us taken over).
 //
 //   warp 8      loads: what an item is, read from global memory and handed to the other warps
 //               through shared memory; its Q tiles; then a ring of slots. Slot u of a tile holds
@@ -34,16 +34,17 @@
 // O, so the softmax of unit u + 1 has its scores while P V of unit u and the scores of u + 2
 // are computed; with units of 128 keys TMEM holds one buffer, and each tile's softmax and
 // MMAs wait for one another. The price is that an N = 64 score MMA reads its Q operand from
-// shared memory for half as many columns. Measured on 592 pairs of tiles x 4, 64 blocks a
-// list, under the power cap: 590 us with one list per pair and 640 us with a list per tile,
-// against 678 and 694 us with units of 128 keys.
+// shared memory for half as many columns. Measured on 592 pairs of tiles, 64 blocks a list,
+// under the power cap: 590 us with one list per pair and 640 us with a list per tile, against
+// 678 and 694 us with units of 128 keys (before the steps noted below, now 556 and 580 us).
 //
 // TMEM (512 columns): S of tile t, buffer b at 128 t + 64 b; O of tile t at 256 + 128 t.
 //
 // What does not exist is never read into a result: list entries outside the sequence load
-// zeros (a TMA box behind the end of the tensor), and their scores are replaced by -inf. Keys behind k_lens inside a block may hold NaN:
-// their scores are replaced, and their V rows are overwritten with zeros in shared memory
-// before the tensor core sees them (0 * NaN is NaN).
+// zeros (a TMA box behind the end of the tensor), and their scores are replaced by -inf.
+// Keys behind k_lens inside a block may hold NaN: their scores are replaced, and their V rows
+// are overwritten with zeros in shared memory before the tensor core sees them (0 * NaN is
+// NaN).
 //
 // Every mbarrier wait is bounded; on expiry the status word gets kStatusAttentionTimeout,
 // the CTA's abort flag is raised and all roles unwind, free TMEM and return.
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_qempty(t), 1);
       for (int buf = 0; buf < 2; ++buf) {
         mbar_init(bar_s(t, buf), 1);
-        mbar_init(bar_p(t, buf), 4 * 32);
+        mbar_init(bar_p(t, buf), 4);
         mbar_init(bar_pv(t, buf), 1);
       }
     }
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int u = 0; u < units; ++u) {
         const int slot = slot_of(next);
-        ok = wait_slot(next) && wait_all(bar_p(t, n_pv & 1), (n_pv >> 1) & 1);
+        ok = wait_all(bar_p(t, n_pv & 1), (n_pv >> 1) & 1) && wait_slot(next);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -638,12 +639,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int u = 0; idle && u < units; ++u, ++n) {
         ok = wait_all(bar_s(t, n & 1), (n >> 1) & 1);
         if (!ok) break;
-        mbar_arrive(bar_p(t, n & 1));
+        if (lane == 0) mbar_arrive(bar_p(t, n & 1));
       }
-      // Whether this unit's scores were seen complete halfway through the last one's
-      // exponentials: a wait costs 90 to 180 clocks even where nothing is left to wait for.
-      // With shared slots a test that does not suspend is the faster one, with slots per tile
-      // the one that may (565 and 587 us against 637 and 609 us; without either 580 and 628).
+      // Whether this unit's scores were seen complete during the last one's
+      // exponentials: a wait costs 90 to 180 clocks even where nothing is left to wait for
+      // (561 against 580 us with one list per pair, 593 against 597 us with a list per tile).
       bool ready = false;
       for (int u = 0; !idle && u < units; ++u, ++n) {
         const uint32_t t_s = tmem + lanes + kTmemS + t * 128 + (n & 1) * 64;
@@ -704,9 +704,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          if (i == 16) {
-            const uint32_t bar = bar_s(t, (n + 1) & 1), parity = ((n + 1) >> 1) & 1;
-            ready = u + 1 < units && (SHARED ? mbar_test(bar, parity) : mbar_try(bar, parity));
+          if (i == 8) {
+            ready = u + 1 < units && mbar_try(bar_s(t, (n + 1) & 1), ((n + 1) >> 1) & 1);
           }
           const uint32_t* src = sv[i >> 4] + 2 * (i & 15);
           const float2 x = __ffma2_rn(
@@ -717,11 +716,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           acc[i & 1] = __fadd2_rn(acc[i & 1], p);
           pk[i] = pack_pair<FP16>(p.x, p.y);
         }
-        // P over the first 32 of the unit's S columns, all of them read.
+        // P over the first 32 of the unit's S columns, all of them read. One arrival per warp:
+        // with one per thread, and the MMA warps waiting for the slot before P, 560 and 601 us
+        // against 556 and 580.
         tmem_st32(t_s, pk);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(bar_p(t, n & 1));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p(t, n & 1));
         l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       }
       // ---------------- epilogue ----------------
