@@ -331,6 +331,11 @@ __device__ __forceinline__ unsigned long long kth_key(unsigned long long common,
 }
 
 constexpr int kBins = 256;
+// Bins for a row of 32 KEYS columns: three of them should rarely hold more than a warp ranks
+// (2036 columns, 6108 rows: 27 on average around the best tenth with 256 bins; 288 us with
+// these, 98 us with twice as many).
+template <int KEYS>
+constexpr int kBinsOf = KEYS <= 32 ? kBins : kBins * KEYS / 32;
 constexpr int kChooseWarps = 8;
 
 // What a warp's row of scores is about.
@@ -603,59 +608,104 @@ __device__ __noinline__ int choose_any(const ChooseArgs& a, const Row& r, uint32
   return done;
 }
 
-// A row of at most 32 KEYS finite scores, KEYS columns in the registers of each lane: counts
-// them in bins of their range, gathers the bin that holds the k-th and its neighbours, and
-// ranks these, one a lane. Returns -1 where that does not settle it (scores bunched in a bin,
-// all alike, a border wider than a bin): choose_any does.
+// Eight floats, 32-byte aligned.
+__device__ __forceinline__ void ld_floats8(const float* p, float* v) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
+                 "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
+}
+// The smallest and the largest of three, NaN passed over.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A row of at most 32 KEYS finite scores, KEYS neighbouring columns in the registers of each
+// lane: counts them in bins of their range, gathers the bin that holds the k-th and its
+// neighbours, and ranks these, one a lane. Sets of columns are bit masks, a word for 32 columns
+// of a lane. Returns -1 where that does not settle it (scores bunched in a bin, all alike, a
+// border wider than a bin): choose_any does. (Bound by the latency of its steps, 80 registers:
+// 24 rows at once on an SM. 9600 rows of 800 columns: 37 us, with floats instead of masks and
+// 16-byte loads 51 us.)
 template <int KEYS>
 __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, uint32_t* bins,
-                                           int* columns, float* values, int* gathered, int lane) {
-  constexpr float kBig = 3.4028235e38f;  // above every score: in; -kBig: out
+                                           int* columns, int* gathered, int lane) {
+  constexpr int kWords = (KEYS + 31) / 32;
+  constexpr int kBins = kBinsOf<KEYS>, kHeld = kBins / 32;
   const float* row = reinterpret_cast<const float*>(a.scores) + r.list * a.pitch;
   const int c0 = lane * KEYS;
-  const float twice = twice_error(r);
-  float v[KEYS];
-  float low = kBig, high = -kBig;
+  const int mine = min(max(r.k_blocks - c0, 0), KEYS);  // columns of this lane that exist
+  const int left = r.want - r.kept;
+  uint32_t in[kWords];  // columns of this lane that are in
 #pragma unroll
-  for (int i = 0; i < KEYS; i += 4) {
-    const float4 s = c0 + i < a.pitch ? __ldcg(reinterpret_cast<const float4*>(row + c0 + i))
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-    v[i] = s.x;
-    v[i + 1] = s.y;
-    v[i + 2] = s.z;
-    v[i + 3] = s.w;
-  }
+  for (int w = 0; w < kWords; ++w) in[w] = 0u;
+  if (r.kept > 0) {
+#pragma unroll 8
+    for (int i = 0; i < mine; ++i) {
+      const uint32_t bit = (a.keep[c0 + i] != 0 ? 1u : 0u) << (i & 31);
 #pragma unroll
-  for (int i = 0; i < KEYS; ++i) {
-    const int c = c0 + i;
-    if (c >= r.k_blocks) {
-      v[i] = -kBig;
-    } else if (r.kept > 0 && a.keep[c] != 0) {
-      v[i] = kBig;
-    } else {
-      low = fminf(low, v[i]);
-      high = fmaxf(high, v[i]);
+      for (int w = 0; w < kWords; ++w) in[w] |= i >> 5 == w ? bit : 0u;
     }
   }
-  float cut = 0.f;  // scores above are in
-  if (r.want == r.kept || r.want == r.k_blocks) {
+  if (r.want == r.k_blocks) {
 #pragma unroll
-    for (int i = 0; i < KEYS; ++i)
-      v[i] = v[i] == kBig || (r.want == r.k_blocks && c0 + i < r.k_blocks) ? kBig : -kBig;
-  } else {
+    for (int w = 0; w < kWords; ++w)
+      in[w] = mine >= 32 * w + 32 ? ~0u : mine <= 32 * w ? 0u : (1u << (mine - 32 * w)) - 1u;
+  } else if (left > 0) {
+    const float twice = twice_error(r);
+    const float nan = __int_as_float(0x7fffffff);
+    float v[KEYS];  // NaN where a column does not compete: it is in no range and in no bin
+#pragma unroll
+    for (int i = 0; i < KEYS; i += 8) {
+      if (mine > 0 && c0 + i < a.pitch) {
+        ld_floats8(row + c0 + i, v + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i + j] = nan;
+      }
+    }
+    if (r.k_blocks % KEYS != 0) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) v[i] = i < mine ? v[i] : nan;
+    }
+    if (r.kept > 0) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) v[i] = in[i >> 5] >> (i & 31) & 1u ? nan : v[i];
+    }
+    float low = nan, high = nan;
+#pragma unroll
+    for (int i = 0; i < KEYS; i += 2) {
+      low = min3(low, v[i], v[i + 1]);
+      high = max3(high, v[i], v[i + 1]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
       high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
-    const float scale = 255.8f / (high - low);
-    // (An error below 1e30 keeps every score well below the marks.)
-    if (!(twice < 1e30f) || !(scale < 1e30f) || !(scale > 1e-30f)) return -1;
-    const float shift = 0.1f - low * scale;
-    // Never decreases with the score; the marks fall outside.
-    auto bin_of = [&](float s) { return __float2int_rd(fmaf(s, scale, shift)); };
+    const float scale = (float)(kBins - 3) / (high - low);
+    // The bin is what s scale + shift rounds to, 0 to kBins - 1: read from the low bits of a float in
+    // [2^23, 2^24), where the rounding is to integers, that of `shift` too. It never decreases
+    // with the score. (A range that small beside the scores is within their error.)
+    if (!(twice < INFINITY) || !(scale < 1e30f) || !(scale > 1e-30f) || !(fabsf(low) * scale < 1e6f))
+      return -1;
+    constexpr float kOne = 12582912.f;  // 1.5 2^23
+    const float shift = kOne + (1.f - low * scale);
+    auto place = [&](float s) { return fmaf(s, scale, shift); };  // kOne + bin
+    auto bin_of = [&](float s) {  // (of a score of the row, or NaN)
+      return __float_as_int(place(s)) - __float_as_int(kOne);
+    };
 #pragma unroll
-    for (int i = 0; i < kBins / 32; ++i) bins[32 * i + lane] = 0u;
+    for (int i = 0; i < kBins / 128; ++i)
+      *reinterpret_cast<uint4*>(bins + 128 * i + 4 * lane) = make_uint4(0u, 0u, 0u, 0u);
     if (lane == 0) *gathered = 0;
     __syncwarp();
 #pragma unroll
@@ -664,13 +714,16 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
       if ((unsigned)bin < (unsigned)kBins) atomicAdd(&bins[bin], 1u);
     }
     __syncwarp();
-    // From the top, the bin that reaches the k-th: lane l looks at bins [8l, 8l + 8).
-    const int left = r.want - r.kept;
-    int mine[kBins / 32], sum = 0;
+    // From the top, the bin that reaches the k-th: lane l looks at kHeld neighbouring bins.
+    int held[kHeld], sum = 0;
 #pragma unroll
-    for (int i = 0; i < kBins / 32; ++i) {
-      mine[i] = (int)bins[lane * (kBins / 32) + i];
-      sum += mine[i];
+    for (int i = 0; i < kHeld; i += 4) {
+      const int4 four = *reinterpret_cast<const int4*>(bins + kHeld * lane + i);
+      held[i] = four.x;
+      held[i + 1] = four.y;
+      held[i + 2] = four.z;
+      held[i + 3] = four.w;
+      sum += (four.x + four.y) + (four.z + four.w);
     }
     int up = sum;
 #pragma unroll
@@ -679,40 +732,43 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
       if (lane + o < 32) up += other;
     }
     const int total = __shfl_sync(0xffffffffu, up, 0);
-    if (total != r.k_blocks - r.kept) return -1;  // (a score that rounded out of the bins)
+    if (total != r.k_blocks - r.kept) return -1;  // (NaN)
     const unsigned reach = __ballot_sync(0xffffffffu, up >= left);
     const int owner = 31 - __clz((int)reach);
     int bin = 0, over = up - sum;
-    if (lane == owner) {
-      bool found = false;
+    bool found = false;
 #pragma unroll
-      for (int i = kBins / 32 - 1; i >= 0; --i) {
-        if (!found && over + mine[i] >= left) {
-          bin = lane * (kBins / 32) + i;
-          found = true;
-        }
-        if (!found) over += mine[i];
+    for (int i = kHeld - 1; i >= 0; --i) {
+      if (!found && over + held[i] >= left) {
+        bin = kHeld * lane + i;
+        found = true;
       }
+      if (!found) over += held[i];
     }
     bin = __shfl_sync(0xffffffffu, bin, owner);
     over = __shfl_sync(0xffffffffu, over, owner);  // scores in the bins above
     const int next = bin + 1 < kBins ? (int)bins[bin + 1] : 0;
     const int n = next + (int)bins[bin] + (bin > 0 ? (int)bins[bin - 1] : 0);
     if (n > 32) return -1;
+    uint32_t near[kWords];
 #pragma unroll
-    for (int i = 0; i < KEYS; ++i) {
-      if ((unsigned)bin_of(v[i]) - (unsigned)bin + 1u < 3u) {
-        const int at = atomicAdd(gathered, 1);
-        columns[at] = c0 + i;
-        values[at] = v[i];
-      }
+    for (int w = 0; w < kWords; ++w) near[w] = 0u;
+    const int below = bin - 1;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      if ((unsigned)(bin_of(v[i]) - below) < 3u) near[i >> 5] |= 1u << (i & 31);
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      if (near[w] == 0u) continue;
+      int at = atomicAdd(gathered, __popc(near[w]));
+      for (uint32_t m = near[w]; m != 0u; m &= m - 1u) columns[at++] = c0 + 32 * w + __ffs((int)m) - 1;
     }
     __syncwarp();
     const int my_column = lane < n ? columns[lane] : 0x7fffffff;
-    const float my_value = lane < n ? values[lane] : -kBig;
+    const float my_value = lane < n ? row[my_column] : -INFINITY;
     int rank = 0;
     for (int i = 0; i < n; ++i) {
-      const float s = values[i];
+      const float s = __shfl_sync(0xffffffffu, my_value, i);
       rank += s > my_value || (s == my_value && columns[i] < my_column);
     }
     const int first = over - next;  // scores above all that were gathered
@@ -720,34 +776,37 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
     const float t = __shfl_sync(0xffffffffu, my_value, __ffs((int)kth) - 1);
     const float hi = __fadd_ru(t, twice), lo = __fadd_rd(t, -twice);
     // All that is close has to be among the gathered.
-    if ((bin > 0 && bin_of(lo) < bin - 1) || (bin + 1 < kBins && bin_of(hi) > bin + 1)) return -1;
-    const unsigned near = __ballot_sync(0xffffffffu, lane < n && my_value >= lo && my_value <= hi);
+    if ((bin > 0 && place(lo) < kOne + (float)(bin - 1)) ||
+        (bin + 1 < kBins && place(hi) > kOne + (float)(bin + 1)))
+      return -1;
+    const unsigned close = __ballot_sync(0xffffffffu, lane < n && my_value >= lo && my_value <= hi);
     const int open = left - first - __popc(__ballot_sync(0xffffffffu, lane < n && my_value > hi));
-    if (__popc(near) == open) {
-      cut = lo;
-      // (>= lo below: take the next value down as the cut.)
-      cut = __int_as_float(__float_as_int(cut) + (cut > 0.f ? -1 : 1));
-      if (lo == 0.f) cut = -1e-45f;
-    } else {
-      // The close columns move to the front of `columns`, each still in its owner's register.
-      const int n_close = __popc(near);
-      __syncwarp();
-      if (near >> lane & 1u) columns[__popc(near & ((1u << lane) - 1u))] = my_column;
-      __syncwarp();
-      const unsigned in = best_of(a, r, columns, n_close, open, lane);
-      for (int i = 0; i < n_close; ++i) {
-        const int at = columns[i] - c0;
-        const float mark = (in >> i & 1u) ? kBig : -kBig;
+    const int n_close = __popc(close);
+    // In: what lies above hi, and where all the close ones fit, what reaches lo.
+    const bool all_close = n_close == open;
+    float least = lo;
+    if (!all_close)  // the next float above hi
+      least = hi == 0.f ? 1e-45f : __int_as_float(__float_as_int(hi) + (hi > 0.f ? 1 : -1));
 #pragma unroll
-        for (int j = 0; j < KEYS; ++j)
-          if (j == at) v[j] = mark;
+    for (int i = 0; i < KEYS; ++i)
+      if (v[i] >= least) in[i >> 5] |= 1u << (i & 31);
+    if (!all_close) {
+      // The close columns move to the front of `columns`.
+      __syncwarp();
+      if (close >> lane & 1u) columns[__popc(close & ((1u << lane) - 1u))] = my_column;
+      __syncwarp();
+      const unsigned best = best_of(a, r, columns, n_close, open, lane);
+      for (unsigned m = best; m != 0u; m &= m - 1u) {
+        const unsigned at = (unsigned)(columns[__ffs((int)m) - 1] - c0);
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+          if (at >> 5 == (unsigned)w && at < (unsigned)KEYS) in[w] |= 1u << (at & 31);
       }
-      cut = hi;
     }
   }
   int count = 0;
 #pragma unroll
-  for (int i = 0; i < KEYS; ++i) count += v[i] > cut;
+  for (int w = 0; w < kWords; ++w) count += __popc(in[w]);
   int before = count;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -757,8 +816,8 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
   const int done = __shfl_sync(0xffffffffu, before, 31);
   int32_t* out = a.indices + r.list * a.top_k + (before - count);
 #pragma unroll
-  for (int i = 0; i < KEYS; ++i)
-    if (v[i] > cut) *out++ = c0 + i;
+  for (int w = 0; w < kWords; ++w)
+    for (uint32_t m = in[w]; m != 0u; m &= m - 1u) *out++ = c0 + 32 * w + __ffs((int)m) - 1;
   return done;
 }
 
@@ -771,9 +830,8 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
 template <int KEYS>
 __global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 4 : KEYS <= 32 ? 3 : 1)
     block_choose(const ChooseArgs a) {
-  __shared__ uint32_t bins[kChooseWarps][kBins];
+  __shared__ __align__(16) uint32_t bins[kChooseWarps][kBinsOf<KEYS>];
   __shared__ int columns[kChooseWarps][32];
-  __shared__ float values[kChooseWarps][32];
   __shared__ int gathered[kChooseWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t list = blockIdx.x * kChooseWarps + warp;
@@ -802,7 +860,7 @@ __global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 4 : KEYS <= 32
     done = -1;
     if constexpr (KEYS > 0) {
       if (r.kept <= r.want)
-        done = choose_fast<KEYS>(a, r, bins[warp], columns[warp], values[warp], &gathered[warp], lane);
+        done = choose_fast<KEYS>(a, r, bins[warp], columns[warp], &gathered[warp], lane);
     }
     if (done < 0) {
       __syncwarp();
@@ -829,7 +887,8 @@ Sizes sizes_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
   // Per row: D fp32, D + D bf16, a norm (rounded up so that every part starts on 16 bytes).
   s.norms_at = (s.q_rows + s.k_rows) * head_dim * 8 + ((s.q_rows + s.k_rows) * 4 + 31) / 16 * 16;
   s.scores_at = s.norms_at + (batch * kv_heads * (s.pitch / kScoreN) * 4 + 15) / 16 * 16;
-  s.bytes = s.scores_at + s.q_rows * s.pitch * 4;
+  // Scores start at the next 32 bytes, wherever the workspace starts.
+  s.bytes = s.scores_at + 16 + s.q_rows * s.pitch * 4;
   return s;
 }
 
@@ -955,7 +1014,8 @@ extern "C" int h3b_select_key_blocks(
   qm.norm = reinterpret_cast<float*>(take(sz.q_rows * 4));
   km.norm = reinterpret_cast<float*>(take(sz.k_rows * 4));
   auto* norms = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.norms_at);
-  auto* scores = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sz.scores_at);
+  auto* scores = reinterpret_cast<uint32_t*>(
+      (reinterpret_cast<uintptr_t>(workspace) + (uintptr_t)sz.scores_at + 31) / 32 * 32);
   MeanArgs m{};
   m.side[0] = MeanSide{q, qm, q_batch_stride, q_row_stride, q_head_stride, q_lens, (int)seq_q,
                        (int)heads, (int)block_q, (int)nq, batch * nq * heads};

@@ -385,6 +385,24 @@ def test_select_long_rows():
             assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
 
 
+@pytest.mark.parametrize("nk,top_k", [(200, 20), (256, 255), (257, 26), (500, 90), (513, 1), (800, 80), (1025, 300), (2036, 204), (2049, 64), (3900, 390)])
+def test_select_row_lengths(nk, top_k):
+    """Rows of every size that a lane's registers come in, with kept blocks, a padded batch and
+    heads that share keys."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    sk = nk * 64 - 5
+    q, k = _randn((2, 300, 4, 64), 1), _randn((2, sk, 2, 64), 2)
+    k_lens = torch.tensor([sk, sk // 3], dtype=torch.int32, device="cuda")
+    keep = torch.zeros(nk, dtype=torch.bool, device="cuda")
+    keep[[0, nk // 5, nk - 1]] = True
+    for mask in (None, keep):
+        got, n = select_key_blocks(q, k, top_k, block_k=64, k_lens=k_lens, keep=mask)
+        ref, ref_n = sparse_ref.select(q, k, top_k, block_k=64, k_lens=k_lens, keep=mask)
+        assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
+
+
 def test_offsets_past_32_bits():
     """A key tensor of more than 2^32 bytes and 2^31 elements: the last blocks are read where they are."""
 
