@@ -13,16 +13,20 @@
 // only scores too close to the border for fp32 to tell are taken in fp64 (block_choose).
 //
 // Three kernels:
-//   block_means   reads q and k once; bound by HBM, and nearly all of the time at long
-//                 sequences. Heads of one block lie next to each other in
-//                 the grid, so that whole rows are read together. Leaves each mean in fp32, its norm, and
-//                 the mean as a sum of two bf16.
+//   block_means   reads q and k once; bound by HBM, and two thirds of the time at long
+//                 sequences. Heads of one block lie next to each other in the grid, so that
+//                 whole rows are read together. Leaves each mean in fp32, its norm, and the
+//                 mean as a sum of two bf16.
 //   block_scores  s in fp32 from the bf16 parts, hi hi + hi mid + mid hi, on the tensor cores
 //                 (mma.sync: a product of a few GFLOP, not worth a tcgen05 pipeline). The
 //                 query heads that share a key head are rows of one product.
 //   block_choose  a warp per query block, its scores in registers: counts them in bins, ranks
 //                 those next to the border. Rows that this does not settle, or of more than
 //                 4096 key blocks, go through the workspace (choose_any).
+// 24 heads of 51,200 rows, 80 of 800 blocks: 116, 30 and 30 us, 170 together, each kernel starting
+// while the one before drains. The steps of different groups of heads in one launch, to overlap
+// HBM and latencies, took 186 us with three groups and 192 us with four (173 us apart then): a
+// launch costs some 12 us however little it does.
 #include <cuda_fp16.h>
 
 #include <cstdio>
@@ -333,10 +337,10 @@ __device__ __forceinline__ unsigned long long kth_key(unsigned long long common,
 constexpr int kBins = 256;
 // Bins for a row of 32 KEYS columns: three of them should rarely hold more than a warp ranks
 // (2036 columns, 6108 rows: 27 on average around the best tenth with 256 bins; 288 us with
-// these, 98 us with twice as many).
+// these, 73 us with twice as many).
 template <int KEYS>
 constexpr int kBinsOf = KEYS <= 32 ? kBins : kBins * KEYS / 32;
-constexpr int kChooseWarps = 8;
+constexpr int kChooseWarps = 4;
 
 // What a warp's row of scores is about.
 struct Row {
@@ -632,9 +636,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // lane: counts them in bins of their range, gathers the bin that holds the k-th and its
 // neighbours, and ranks these, one a lane. Sets of columns are bit masks, a word for 32 columns
 // of a lane. Returns -1 where that does not settle it (scores bunched in a bin, all alike, a
-// border wider than a bin): choose_any does. (Bound by the latency of its steps, 80 registers:
-// 24 rows at once on an SM. 9600 rows of 800 columns: 37 us, with floats instead of masks and
-// 16-byte loads 51 us.)
+// border wider than a bin): choose_any does. (Bound by the latency of its steps.
+// 9600 rows of 800 columns: 30 us, with marked floats in place of masks and 16-byte loads 51 us.)
 template <int KEYS>
 __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, uint32_t* bins,
                                            int* columns, int* gathered, int lane) {
@@ -826,10 +829,12 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
 // below T - 2E are out whatever the rounding did; the few between are scored again in fp64 and
 // ranked.
 // CTAs per SM that the registers should allow: a row is a chain of short steps, and many rows at
-// once hide it.
+// once hide it (6108 rows of 2036 columns: two CTAs 63 us, three 48 us, four 43 us, five 43 us).
+// Eight warps a CTA are slower, 33 against 30 us for 9600 rows of 800: a CTA lasts as long as its
+// slowest row.
 template <int KEYS>
-__global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 4 : KEYS <= 32 ? 3 : 1)
-    block_choose(const ChooseArgs a) {
+__global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 8 : KEYS <= 32 ? 6 : KEYS <= 64 ? 4 : 3)
+    block_choose(const __grid_constant__ ChooseArgs a) {
   __shared__ __align__(16) uint32_t bins[kChooseWarps][kBinsOf<KEYS>];
   __shared__ int columns[kChooseWarps][32];
   __shared__ int gathered[kChooseWarps];
