@@ -84,9 +84,12 @@ __device__ __forceinline__ void add8(double (&acc)[8], uint4 u) {
 // WARPS warps per (batch, block, head) take turns at its rows: D/8 lanes hold the columns of a
 // row, the others further rows. One warp where there are blocks enough to fill the GPU (24
 // heads of 51,200 rows, 64-key blocks: 105 us, with four 155 us), four for short sequences
-// (4352 rows, three heads: 4.6 us, with one 9.3 us).
+// (4352 rows, three heads: 4.6 us, with one 9.3 us). Eight loads of 16 bytes a lane and seven
+// CTAs per SM keep HBM busy; four loads with eight CTAs (119 us), sixteen with five (122 us)
+// are slower than 116 us, and so are fewer conversions to fp64, whose unit is busy 71% of the
+// time: with some done on the bits by integer instructions 125 us and more.
 template <bool FP16, int D, int WARPS>
-__global__ void __launch_bounds__(kMeanWarps * 32) block_means(const MeanArgs a) {
+__global__ void __launch_bounds__(kMeanWarps * 32, 7) block_means(const MeanArgs a) {
   __shared__ double part[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
   const int warp = threadIdx.x >> 5 & (WARPS - 1), lane = threadIdx.x & 31;
   grid_wait();
