@@ -18,12 +18,12 @@
 //                 whole rows are read together. Leaves each mean in fp32, its norm, and the
 //                 mean as a sum of two bf16.
 //   block_scores  s in fp32 from the bf16 parts, hi hi + hi mid + mid hi, on the tensor cores
-//                 (mma.sync: a product of a few GFLOP, not worth a tcgen05 pipeline). The
-//                 query heads that share a key head are rows of one product.
+//                 (tcgen05, a tile per CTA). The query heads that share a key head are rows
+//                 of one product.
 //   block_choose  a warp per query block, its scores in registers: counts them in bins, ranks
 //                 those next to the border. Rows that this does not settle, or of more than
 //                 4096 key blocks, go through the workspace (choose_any).
-// 24 heads of 51,200 rows, 80 of 800 blocks: 116, 30 and 30 us, 170 together, each kernel starting
+// 24 heads of 51,200 rows, 80 of 800 blocks: 117, 24 and 31 us, 165 together, each kernel starting
 // while the one before drains. The steps of different groups of heads in one launch, to overlap
 // HBM and latencies, took 186 us with three groups and 192 us with four (173 us apart then): a
 // launch costs some 12 us however little it does.
@@ -31,6 +31,7 @@
 
 #include <cstdio>
 
+#include "attention_ptx.cuh"
 #include "common.cuh"
 
 namespace h3b {
@@ -170,28 +171,20 @@ __global__ void __launch_bounds__(kMeanWarps * 32, 7) block_means(const MeanArgs
 
 // ---- scores ---------------------------------------------------------------
 
-constexpr int kScoreM = 64, kScoreN = 128, kScoreThreads = 256;
+constexpr int kScoreM = 128, kScoreN = 128, kScoreThreads = 256;
+constexpr int kScoreDepth = 64;  // columns of the means in shared memory at a time
+constexpr uint32_t kScoreRow = 2 * kScoreDepth;  // bytes
+static_assert(kScoreM == 128 && kScoreDepth == 64, "the layout below");
+constexpr uint32_t kScoreBuffer = 2 * (kScoreM + kScoreN) * kScoreRow;
 
 struct ScoreArgs {
   Means q, k;
   float* scores;    // [products][m][pitch]
   uint32_t* norms;  // [products][pitch / kScoreN]: bits of the largest |k| of a tile's columns
+  unsigned int* status;
   int m, nk, pitch;
 };
 
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // 16 bytes into shared memory, or zeros where the row does not exist.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -199,82 +192,148 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
                : "memory");
 }
 
-// A 64 x 128 tile of scores per CTA, eight warps of 32 x 32; the whole depth D of both bf16
-// parts of both operands in shared memory, 16-byte chunks xor-swizzled by row.
-template <int D>
-__global__ void __launch_bounds__(kScoreThreads) block_scores(const ScoreArgs a) {
-  extern __shared__ __align__(128) uint8_t tiles[];
-  constexpr int kRowBytes = 2 * D, kChunks = D / 8;
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(tiles);
-  const uint32_t part_a = kScoreM * kRowBytes, part_b = kScoreN * kRowBytes;
-  const uint32_t tile_b = base + 2 * part_a;
-  const int m0 = blockIdx.y * kScoreM, n0 = blockIdx.x * kScoreN;
-  const int64_t product = blockIdx.z;
-  grid_wait();
-  auto at = [&](int row, int chunk) { return row * kRowBytes + ((chunk ^ (row & 7)) << 4); };
-  for (int i = threadIdx.x; i < (kScoreM + kScoreN) * kChunks; i += kScoreThreads) {
-    const int row = i / kChunks, chunk = i % kChunks;
-    const bool is_a = row < kScoreM;
-    const int r = is_a ? m0 + row : n0 + row - kScoreM;
-    const bool there = r < (is_a ? a.m : a.nk);
-    const Means& side = is_a ? a.q : a.k;
-    const int64_t off = there ? (product * (is_a ? a.m : a.nk) + r) * D + chunk * 8 : 0;
-    const uint32_t dst = is_a ? base + at(row, chunk) : tile_b + at(row - kScoreM, chunk);
-    copy16(dst, side.hi + off, there);
-    copy16(dst + (is_a ? part_a : part_b), side.mid + off, there);
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
+// A 128 x 128 tile of scores per CTA: tcgen05 products of 64 columns at a time, hi hi, hi mid
+// and mid hi into one accumulator of 128 TMEM columns. The parts lie in shared memory as the
+// tensor core reads them, rows of 128 bytes with 16-byte chunks xor-swizzled by row. With one
+// buffer of 64 columns (64 KB) three CTAs fit an SM and overlap their loads, products and
+// stores; where there is no more than a CTA per SM, a buffer for all columns lets all loads
+// start at once. Measured, one buffer against two at D = 128: 672 tiles 24 and 28 us, 32 tiles
+// 7.9 and 7.3 us (mma.sync on tiles of 64 x 128: 30 and 6.9 us).
+template <int D, int BUFFERS>
+__global__ void __launch_bounds__(kScoreThreads, BUFFERS == 1 ? 3 : 1)
+    block_scores(const __grid_constant__ ScoreArgs a) {
+  constexpr int kSteps = D / kScoreDepth;
+  static_assert(BUFFERS == 1 || BUFFERS == kSteps, "");
+  constexpr int N = kScoreN;
+  constexpr uint32_t kQPart = kScoreM * kScoreRow, kKPart = N * kScoreRow;
+  extern __shared__ uint8_t tiles[];
+  __shared__ __align__(8) uint64_t done_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_flag;
+  const uint32_t base = (attn::smem_u32(tiles) + 1023u) / 1024u * 1024u;
+  const uint32_t bar = attn::smem_u32(&done_bar);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    attn::mbar_init(bar, 1);
+    abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     attn::smem_u32(&tmem_slot)),
+                 "r"(N)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const int m0 = blockIdx.y * kScoreM, n0 = blockIdx.x * N;
+  const int64_t product = blockIdx.z;
+  attn::tc_fence_before();
+  __syncthreads();
+  attn::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  grid_wait();
+  // Parts of a buffer: q hi, q mid, k hi, k mid. Eight threads a row.
+  auto load = [&](int step) {
+    const uint32_t buffer = base + (BUFFERS > 1 ? step : 0) * kScoreBuffer;
+    const int chunk = threadIdx.x & 7;
+#pragma unroll
+    for (int i = 0; i < (kScoreM + N) * 8 / kScoreThreads; ++i) {
+      constexpr int kRows = kScoreThreads / 8;
+      const bool is_q = i < kScoreM / kRows;
+      const int row = (threadIdx.x >> 3) + (is_q ? i : i - kScoreM / kRows) * kRows;
+      const int r = (is_q ? m0 : n0) + row;
+      const bool there = r < (is_q ? a.m : a.nk);
+      const Means& side = is_q ? a.q : a.k;
+      const int64_t off =
+          there ? (product * (is_q ? a.m : a.nk) + r) * D + step * kScoreDepth + chunk * 8 : 0;
+      const uint32_t dst =
+          buffer + (is_q ? 0u : 2 * kQPart) + row * kScoreRow + (uint32_t)((chunk ^ (row & 7)) << 4);
+      copy16(dst, side.hi + off, there);
+      copy16(dst + (is_q ? kQPart : kKPart), side.mid + off, there);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  load(0);
+  if (BUFFERS > 1) load(1);
   if (blockIdx.y == 0 && warp == 0) {
     uint32_t norm = 0u;  // the bits order like the values, NaN above all
 #pragma unroll
-    for (int i = 0; i < kScoreN / 32; ++i) {
+    for (int i = 0; i < N / 32; ++i) {
       const int c = n0 + 32 * i + lane;
       if (c < a.nk) norm = max(norm, __float_as_uint(a.k.norm[product * a.nk + c]));
     }
     norm = __reduce_max_sync(0xffffffffu, norm);
     if (lane == 0) a.norms[product * gridDim.x + blockIdx.x] = norm;
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
-  float acc[2][4][4] = {};
+  bool ok = true;
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    uint32_t ah[2][4], am[2][4], bh[2][4], bm[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      // A: rows 0-15 by two chunks; B: rows (columns of the scores) 0-15 by two chunks.
-      const uint32_t oa = at(wm + 16 * i + (lane & 15), 2 * kk + (lane >> 4));
-      const uint32_t ob = at(wn + 16 * i + (lane & 7) + ((lane >> 4) << 3), 2 * kk + (lane >> 3 & 1));
-      ldmatrix4(base + oa, ah[i]);
-      ldmatrix4(base + part_a + oa, am[i]);
-      ldmatrix4(tile_b + ob, bh[i]);
-      ldmatrix4(tile_b + part_b + ob, bm[i]);
+  for (int step = 0; step < kSteps; ++step) {
+    if (BUFFERS == 1 && step > 0) {
+      // The products before have read their columns.
+      ok = __syncthreads_and(attn::wait_bar(bar, (step - 1) & 1, &abort_flag, a.status));
+      if (!ok) break;
+      load(step);
     }
+    if (BUFFERS > 1 && step == 0)
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+      if (attn::elect_one()) {
+        // kind::f16, bf16 operands, both with their columns innermost, f32 accumulator.
+        constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) |
+                                    ((uint32_t)(kScoreM >> 4) << 24);
+        const uint32_t buffer = base + (BUFFERS > 1 ? step : 0) * kScoreBuffer;
+        const uint64_t qd = attn::smem_desc(buffer, 16, 1024);
+        const uint64_t kd = attn::smem_desc(buffer + 2 * kQPart, 16, 1024);
+        auto q = [&](int n, int kk) { return qd + (uint64_t)((n * kQPart + kk * 32) >> 4); };
+        auto k = [&](int n, int kk) { return kd + (uint64_t)((n * kKPart + kk * 32) >> 4); };
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int p = j >> 1, q = (j & 1) * 2;
-        mma_bf16(acc[i][j], am[i], bh[p][q], bh[p][q + 1]);
-        mma_bf16(acc[i][j], ah[i], bm[p][q], bm[p][q + 1]);
-        mma_bf16(acc[i][j], ah[i], bh[p][q], bh[p][q + 1]);
+        for (int kk = 0; kk < kScoreDepth / 16; ++kk) {
+          attn::mma_ss(tmem, q(1, kk), k(0, kk), kIdesc, step > 0 || kk > 0 ? 1u : 0u);
+          attn::mma_ss(tmem, q(0, kk), k(1, kk), kIdesc, 1u);
+          attn::mma_ss(tmem, q(0, kk), k(0, kk), kIdesc, 1u);
+        }
+        if (BUFFERS == 1 || step + 1 == kSteps) attn::mma_commit(bar);
       }
+      __syncwarp();
+    }
   }
+  if (ok)
+    ok = __syncthreads_and(
+        attn::wait_bar(bar, BUFFERS == 1 ? (kSteps - 1) & 1 : 0, &abort_flag, a.status));
   grid_done();
+  if (ok) {
+    attn::tc_fence_after();
+    // Warp w: rows 32 (w & 3), half w >> 2 of the columns; a row a thread, 32-byte stores.
+    const int row = m0 + 32 * (warp & 3) + lane, column = N / 2 * (warp >> 2);
+    float* dst = a.scores + (product * a.m + row) * a.pitch + n0 + column;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int c = 0; c < N / 2; c += 32) {
+      uint32_t s[32];
+      attn::tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + column + c, s);
+      attn::tmem_ld_wait(s);
+      if (row < a.m) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = m0 + wm + 16 * i + 8 * half + lane / 4;
-        if (row < a.m)
-          *reinterpret_cast<float2*>(a.scores + (product * a.m + row) * a.pitch + n0 + wn + 8 * j +
-                                     (lane & 3) * 2) =
-              make_float2(acc[i][j][2 * half], acc[i][j][2 * half + 1]);
+        for (int i = 0; i < 32; i += 8)
+          st32(dst + c + i, Chunk32{make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]),
+                                    make_uint4(s[i + 4], s[i + 5], s[i + 6], s[i + 7])});
       }
+    }
+  }
+  if (!ok) {  // unwinding: let products in flight end before their memory is given up
+    const unsigned long long t0 = attn::globaltimer();
+    while (attn::globaltimer() - t0 < 200000ull) __nanosleep(1000);
+  }
+  attn::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    attn::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(N)
+                 : "memory");
+  }
 }
 
 // ---- choice ---------------------------------------------------------------
@@ -623,15 +682,10 @@ __device__ __forceinline__ void ld_floats8(const float* p, float* v) {
                : "l"(p)
                : "memory");
 }
-// The smallest and the largest of three, NaN passed over.
+// The smallest of three, NaN passed over (and max3, the largest).
 __device__ __forceinline__ float min3(float a, float b, float c) {
   float d;
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -690,7 +744,7 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
 #pragma unroll
     for (int i = 0; i < KEYS; i += 2) {
       low = min3(low, v[i], v[i + 1]);
-      high = max3(high, v[i], v[i + 1]);
+      high = attn::max3(high, v[i], v[i + 1]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -907,6 +961,26 @@ int launch_choose(const ChooseArgs& a, cudaStream_t s) {
   return check_launch("h3b_select_key_blocks");
 }
 
+template <int D, int BUFFERS>
+int launch_scores(const ScoreArgs& sc, int64_t m_tiles, int64_t products, cudaStream_t s) {
+  constexpr int kSmem = (int)(BUFFERS * kScoreBuffer + 1024);
+  static ContextSlot slots[kMaxDevices];
+  cudaError_t e = cudaErrorInvalidDevice;
+  if (context_cached(slots, [&]() -> void* {
+        e = cudaFuncSetAttribute(block_scores<D, BUFFERS>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
+      }) == nullptr) {
+    set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
+              cudaGetErrorString(e));
+    return H3B_ERR_CUDA;
+  }
+  launch_after(block_scores<D, BUFFERS>,
+               dim3((unsigned)(sc.pitch / kScoreN), (unsigned)m_tiles, (unsigned)products), kScoreThreads,
+               kSmem, s, sc);
+  return check_launch("h3b_select_key_blocks");
+}
+
 template <bool FP16, int D>
 int launch_all(const MeanArgs& m, const ScoreArgs& sc, const ChooseArgs& a, int64_t products,
                cudaStream_t s) {
@@ -916,26 +990,17 @@ int launch_all(const MeanArgs& m, const ScoreArgs& sc, const ChooseArgs& a, int6
   const int64_t m_tiles = (sc.m + kScoreM - 1) / kScoreM;
   H3B_REQUIRE(grid <= 0x7fffffffLL && products <= 65535 && m_tiles <= 65535,
               "select_key_blocks: shape exceeds launch limits");
-  constexpr int kSmem = 2 * (kScoreM + kScoreN) * 2 * D;
-  static ContextSlot slots[kMaxDevices];
-  cudaError_t e = cudaErrorInvalidDevice;
-  if (context_cached(slots, [&]() -> void* {
-        e = cudaFuncSetAttribute(block_scores<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        return e == cudaSuccess ? reinterpret_cast<void*>(1) : nullptr;
-      }) == nullptr) {
-    set_error(std::string("h3b_select_key_blocks: cannot reserve shared memory: ") +
-              cudaGetErrorString(e));
-    return H3B_ERR_CUDA;
-  }
   if (warps == 1)
     launch_after(block_means<FP16, D, 1>, dim3((unsigned)grid), kMeanWarps * 32, 0, s, m);
   else
     launch_after(block_means<FP16, D, kMeanWarps>, dim3((unsigned)grid), kMeanWarps * 32, 0, s, m);
   int rc = check_launch("h3b_select_key_blocks");
   if (rc != H3B_OK) return rc;
-  const dim3 tiles((unsigned)(sc.pitch / kScoreN), (unsigned)m_tiles, (unsigned)products);
-  launch_after(block_scores<D>, tiles, kScoreThreads, kSmem, s, sc);
-  if ((rc = check_launch("h3b_select_key_blocks")) != H3B_OK) return rc;
+  if (sc.pitch / kScoreN * m_tiles * products <= num_sms())
+    rc = launch_scores<D, D / kScoreDepth>(sc, m_tiles, products, s);
+  else
+    rc = launch_scores<D, 1>(sc, m_tiles, products, s);
+  if (rc != H3B_OK) return rc;
   // Registers for a row's scores: as few as hold it, up to 128 a lane.
   if (a.nk <= 8 * 32) return launch_choose<8>(a, s);
   if (a.nk <= 16 * 32) return launch_choose<16>(a, s);
@@ -1030,7 +1095,7 @@ extern "C" int h3b_select_key_blocks(
   m.side[1] = MeanSide{k, km, k_batch_stride, k_row_stride, k_head_stride, k_lens, (int)seq_k,
                        (int)kv_heads, (int)block_k, (int)nk, batch * nk * kv_heads};
   // The heads of a group lie behind one another: one product per (batch, key head).
-  ScoreArgs sc{qm, km, reinterpret_cast<float*>(scores), norms, (int)(heads / kv_heads * nq), (int)nk,
+  ScoreArgs sc{qm, km, reinterpret_cast<float*>(scores), norms, h3b::status_ptr(), (int)(heads / kv_heads * nq), (int)nk,
                (int)sz.pitch};
   ChooseArgs a{};
   a.indices = indices;
