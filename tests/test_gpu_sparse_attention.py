@@ -403,6 +403,23 @@ def test_select_row_lengths(nk, top_k):
         assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,sq,sk,h,hk", [(2, 700, 9000, 40, 40), (3, 500, 17000, 36, 12), (1, 17000, 300, 96, 96)])
+def test_select_many_heads(d, b, sq, sk, h, hk):
+    """More tiles of scores than SMs, ragged in both directions; heads that share keys cross tiles."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    q, k = _randn((b, sq, h, d), 1), _randn((b, sk, hk, d), 2)
+    top_k = max(1, sk // 64 // 9)
+    got, n = select_key_blocks(q, k, top_k, block_k=64)
+    # (the oracle walks head by head: a few of them, with their own keys)
+    for head in (0, h // 2 + 1, h - 1):
+        kv = head // (h // hk)
+        ref, ref_n = sparse_ref.select(q[:, :, head : head + 1], k[:, :, kv : kv + 1], top_k, block_k=64)
+        assert torch.equal(got[:, head : head + 1].cpu(), ref) and torch.equal(n[:, head : head + 1].cpu(), ref_n)
+
+
 def test_offsets_past_32_bits():
     """A key tensor of more than 2^32 bytes and 2^31 elements: the last blocks are read where they are."""
 
