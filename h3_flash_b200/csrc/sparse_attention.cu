@@ -890,8 +890,13 @@ struct Plan {
 };
 
 // Whole pairs of tiles fill waves of SMs; when the last wave would leave at least half of
-// them idle, its pairs are split along their lists, down to 128 keys per part. A query of
-// one tile is split in any case: half a list for each of the two tiles of an item.
+// them idle, its pairs may be split along their lists, down to 128 keys per part, and joined.
+// Queries of one tile are split in two even where SMs are short, half a list for each of the
+// two tiles of an item. Both only as far as an estimate says that it saves more than the join
+// costs: a step is one unit of 64 keys of both tiles (or of a lone one), the join another launch
+// and the parts written and read. Measured split into as many parts as fit, and whole (us):
+// 2048 rows, 6 heads, D = 64, lists of 256 keys 14.9 and 8.2, of 1536 keys 21.5 and 23.1, of
+// 8192 keys 50 and 100; one row, 6 heads, 256 keys 8.7 and 6.7, 768 keys 9.2 and 11.3.
 Plan make_plan(int64_t batch, int64_t seq_q, int64_t heads, int64_t head_dim, int64_t block_k,
                int64_t list_len, bool can_split) {
   Plan pl{};
@@ -901,28 +906,40 @@ Plan make_plan(int64_t batch, int64_t seq_q, int64_t heads, int64_t head_dim, in
   const int parts = (int)((list_len + least - 1) / least);
   const int sms = num_sms();
   pl.ws_rows = (int)std::min<int64_t>(kTile, seq_q);
-  // (While the workspace stays within 256 MB; more items than that fill the GPU anyway.)
-  pl.duo = can_split && seq_q <= kTile && parts >= 2 &&
-           (int64_t)pl.total * kTiles * pl.ws_rows * (head_dim + 4) * 4 <= (256ll << 20);
-  const int rem = pl.duo ? pl.total : pl.total % sms;
-  const int each = pl.duo ? kTiles : 1;  // ranges per item
   pl.splits = 1;
   pl.entries_per_split = (int)list_len;
   pl.n_full = pl.items = pl.total;
-  if (can_split && rem > 0 && parts >= 2 && (pl.duo || 2 * rem <= sms)) {
-    int want = std::min(std::min(std::max(sms / rem, 1) * each, kMaxParts), parts);
-    pl.entries_per_split = (parts + want - 1) / want * least;
-    want = (int)((list_len + pl.entries_per_split - 1) / pl.entries_per_split);
-    pl.splits = (want + each - 1) / each;
+  const int64_t units = list_len * block_k / kUnit;
+  constexpr int64_t kPairStepNs = 740, kTileStepNs = 580, kJoinNs = 4000, kJoinNsPerMb = 600;
+  const bool one_tile = seq_q <= kTile;
+  const int each = one_tile ? kTiles : 1;  // ranges per item
+  const int rem = one_tile ? pl.total : pl.total % sms;
+  auto waves = [&](int64_t items) { return (items + sms - 1) / sms; };
+  const int64_t part_bytes = (int64_t)pl.ws_rows * (head_dim + 4) * 4;
+  int64_t best = waves(rem) * units * (one_tile ? kTileStepNs : kPairStepNs);
+  const int most = rem == 0 || !can_split
+                       ? 0
+                       : std::min(std::min(std::max(sms / rem, 1) * each, kMaxParts), parts);
+  for (int want = 2; want <= most; ++want) {
+    const int entries = (parts + want - 1) / want * least;
+    const int ranges = (int)((list_len + entries - 1) / entries);
+    const int splits = (ranges + each - 1) / each;
+    const int64_t bytes = (int64_t)rem * splits * kTiles * part_bytes;
+    if (bytes > (256ll << 20)) break;
+    const int64_t ns = waves((int64_t)rem * splits) * (entries * block_k / kUnit) * kPairStepNs +
+                       kJoinNs + bytes * kJoinNsPerMb / 1000000;
+    if (ns < best) {
+      best = ns;
+      pl.duo = one_tile;
+      pl.splits = splits;
+      pl.entries_per_split = entries;
+    }
   }
   if (pl.duo || pl.splits >= 2) {
     pl.split_pairs = rem;
     pl.n_full = pl.total - rem;
     pl.items = pl.n_full + rem * pl.splits;
-    pl.ws_bytes = (int64_t)rem * pl.splits * kTiles * pl.ws_rows * (head_dim + 4) * 4;
-  } else {
-    pl.splits = 1;
-    pl.entries_per_split = (int)list_len;
+    pl.ws_bytes = (int64_t)rem * pl.splits * kTiles * part_bytes;
   }
   return pl;
 }
