@@ -86,6 +86,23 @@ def test_lengths(sq, sk, block_k):
     _check(out, lse, q, k, v, indices, None, block_k=block_k)
 
 
+@pytest.mark.parametrize("sq,block_k", [(1, 128), (5, 64), (128, 128)])
+def test_many_single_tiles(sq, block_k):
+    """More one-tile queries than SMs with long lists: two ranges per item and no more, counts of
+    every size, and a list of one entry beside them."""
+
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
+
+    b, h, sk = 16, 10, 1700
+    q, k, v = _randn((b, sq, h, 64), 1), _randn((b, sk, 1, 64), 2), _randn((b, sk, 1, 64), 3)
+    nk = -(-sk // block_k)
+    indices, counts = _lists(b, h, 1, nk, nk, 4)
+    out, lse = block_sparse_attention(q, k, v, indices, counts, block_k=block_k, return_lse=True)
+    _check(out, lse, q, k, v, indices, counts, block_k=block_k)
+    out, lse = block_sparse_attention(q, k, v, indices[..., :1].contiguous(), block_k=block_k, return_lse=True)
+    _check(out, lse, q, k, v, indices[..., :1], None, block_k=block_k)
+
+
 def test_many_items_per_cta():
     """More pairs of tiles than SMs, lists of very different lengths (none among them)."""
 
