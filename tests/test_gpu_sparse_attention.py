@@ -171,6 +171,30 @@ def test_long_lists_over_cold_keys(sq, block_k):
         _check(out[:, :, few], lse[:, few], q[:, :, few], k[:, :, few], v[:, :, few], indices[:, few], counts[:, few], block_k=block_k)
 
 
+@pytest.mark.parametrize("sq,block_k,padded", [(2944, 64, False), (2944, 128, True), (640, 64, True)])
+def test_lists_per_256_rows_without_a_second_tile(sq, block_k, padded):
+    """Far more pairs than SMs over keys that come from HBM, and some of the pairs have no second
+    tile (an odd number of tiles, rows behind q_lens): the CTA that takes one goes on to a pair that has."""
+
+    from h3_flash_b200.runtime.attention.sparse import block_sparse_attention
+
+    b, s, h = 2, 30000, 24
+    k, v = _randn((b, s, h, 128), 2), _randn((b, s, h, 128), 3)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    nq, nk = -(-sq // 256), -(-s // block_k)
+    q_lens = torch.tensor([sq, sq - 450], dtype=torch.int32, device="cuda") if padded else None
+    few = slice(0, 2)
+    for seed in range(2):
+        q = _randn((b, sq, h, 128), 10 + seed)
+        indices, counts = _lists(b, h, nq, nk, 40, seed)
+        kw = dict(block_q=256, block_k=block_k, q_lens=q_lens)
+        first, lse = block_sparse_attention(q, k, v, indices, counts, return_lse=True, **kw)
+        for _ in range(20):
+            flush.zero_()
+            assert torch.equal(first, block_sparse_attention(q, k, v, indices, counts, **kw))
+        _check(first[:, :, few], lse[:, few], q[:, :, few], k[:, :, few], v[:, :, few], indices[:, few], counts[:, few], **kw)
+
+
 @pytest.mark.parametrize("block_k", [64, 128])
 @pytest.mark.parametrize("d", [64, 128])
 def test_padded_batch_with_nan(d, block_k):
