@@ -17,7 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Any
 
 import torch
@@ -313,7 +313,6 @@ class SparseAttention:
     keep_last_rows: int = 0
     min_blocks: int = 1
     calls: int = 0
-    _keep: dict[tuple[int, int], torch.Tensor] = field(default_factory=dict, repr=False)
 
     def __post_init__(self) -> None:
         if not 0.0 < self.density <= 1.0:
@@ -336,18 +335,14 @@ class SparseAttention:
         return -(-rows // self.block_k) - (rows - kept_rows) // self.block_k if kept_rows else 0
 
     def _keep_mask(self, rows: int, device: torch.device) -> torch.Tensor | None:
+        """The kept blocks, made anew on the current stream by every call: a mask that outlived its call
+        could be replaced while another stream, or a captured graph, still reads it."""
+
         if not self.keep_last_rows or not rows:
             return None
-        key = (rows, device.index)
-        mask = self._keep.get(key)
-        if mask is None:
-            blocks = -(-rows // self.block_k)
-            mask = torch.arange(blocks, device=device) >= blocks - self._kept(rows)
-            if not torch.cuda.is_current_stream_capturing():
-                # Kept for later calls, on whatever stream they run (a captured mask exists
-                # only when its graph has run, and stays the graph's own).
-                torch.cuda.current_stream(device).synchronize()
-                self._keep = {key: mask}  # one sequence length at a time
+        blocks = -(-rows // self.block_k)
+        mask = torch.zeros(blocks, dtype=torch.bool, device=device)
+        mask[blocks - self._kept(rows):] = True
         return mask
 
     def attend(self, packed: torch.Tensor, head_dim: int) -> torch.Tensor:

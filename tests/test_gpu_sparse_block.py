@@ -165,6 +165,52 @@ def test_sparse_sandwich_stack_runs_captured_like_eagerly():
     assert torch.isfinite(replayed).all() and _lib.device_status() == 0
 
 
+def _packed(rows, seed):
+    return torch.randn(rows, 2, 384, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(torch.bfloat16)
+
+
+def test_captured_kept_blocks_outlive_other_lengths():
+    """Captured at one length after a warm-up, then run at others: replays still keep their blocks."""
+
+    from h3_flash_b200.runtime.attention.sparse import SparseAttention
+
+    runtime = SparseAttention(0.1, keep_last_rows=300)
+    packed = _packed(2000, 1)
+    runtime.attend(packed, 128)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = runtime.attend(packed, 128)
+    for i in range(20):
+        runtime.attend(_packed(900 + 128 * i, 2), 128)
+        full = [torch.full((512,), 255, dtype=torch.uint8, device="cuda") for _ in range(50)]
+    packed.copy_(_packed(2000, 3))
+    graph.replay()
+    torch.cuda.synchronize()
+    q, k, v = (packed[None, ..., i * 128:(i + 1) * 128] for i in range(3))
+    keep = torch.arange(16) >= 13  # rows 1700 to 1999 lie in blocks 13 to 15
+    indices, counts = sparse_ref.select(q, k, runtime.list_length(2000), keep=keep)
+    _check(out, sparse_ref.attend(q, k, v, indices, counts)[0][0].cuda())
+    assert torch.equal(out, runtime.attend(packed, 128)) and full
+
+
+def test_two_lengths_on_two_streams():
+    from h3_flash_b200.runtime.attention.sparse import SparseAttention
+
+    runtime = SparseAttention(0.2, block_k=64, keep_last_rows=100)
+    sets = [_packed(3000, 1), _packed(2100, 2)]
+    want = [runtime.attend(p, 128) for p in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (stream, p) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append(runtime.attend(p, 128))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
 def test_full_density_is_dense_attention():
     from h3_flash_b200.runtime.attention import install_sparse_attention
     from h3_flash_b200.runtime.kernels import install_transformer_fusions

@@ -28,6 +28,21 @@ def test_list_length():
     assert SparseAttention(0.01, keep_last_rows=1280).list_length(51200) == 10
 
 
+def test_no_mask_outlives_its_call():
+    """A mask that is kept for later calls could be replaced under a stream or a graph that reads it."""
+
+    s = SparseAttention(0.1, block_k=64, keep_last_rows=130)
+    before = dict(vars(s))
+    first = s._keep_mask(640, torch.device("cpu"))
+    assert first.tolist() == [False] * 7 + [True] * 3
+    assert s._keep_mask(640, torch.device("cpu")) is not first
+    assert s._keep_mask(64, torch.device("cpu")).tolist() == [True]
+    s.keep_last_rows = 1
+    assert s._keep_mask(640, torch.device("cpu")).tolist() == [False] * 9 + [True]
+    assert vars(s) == {**before, "keep_last_rows": 1}
+    assert s._keep_mask(0, torch.device("cpu")) is None
+
+
 @pytest.mark.parametrize("bad", [dict(density=0.0), dict(density=1.5), dict(density=0.1, block_q=64), dict(density=0.1, block_k=32),
                                  dict(density=0.1, keep_last_rows=-1), dict(density=0.1, min_blocks=0)])
 def test_settings_are_checked(bad):
