@@ -462,10 +462,12 @@ __device__ __forceinline__ unsigned best_of(const ChooseArgs& a, const Row& r, c
 //   E = 6e-5 |q| max|k| + 1e-35:
 // dropping mid mid and what two bf16 leave of a mean, 3 2^-18 of |q| |k| (Cauchy-Schwarz);
 // 384 products summed in fp32, 2^-23 each if every addition truncates (1.14e-5 + 4.58e-5);
-// products below fp32's range. Infinite where it does not hold: norms beyond fp32, and means too small for two bf16
-// to hold their digits.
+// products below fp32's range. Infinite where it does not hold: means too small for two bf16 to
+// hold their digits, and norms whose product is near or beyond fp32's range. (Below 1e38 no
+// partial sum leaves the range: by Cauchy-Schwarz they stay under 1.02 |q| |k|.)
 __device__ __forceinline__ float twice_error(const Row& r) {
-  const bool sound = (r.q_norm >= 1e-30f || r.q_norm == 0.f) && (r.k_norm >= 1e-30f || r.k_norm == 0.f);
+  const bool sound = (r.q_norm >= 1e-30f || r.q_norm == 0.f) && (r.k_norm >= 1e-30f || r.k_norm == 0.f) &&
+                     r.q_norm * r.k_norm < 1e38f;
   return sound ? 1.21e-4f * r.q_norm * r.k_norm + 2e-35f : INFINITY;
 }
 

@@ -396,6 +396,27 @@ def test_select_extreme_scales(q_scale, k_scale):
     assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
 
 
+@pytest.mark.parametrize("sk", [1500, 2048, 5000, 64 * 4200])
+@pytest.mark.parametrize("q_scale,k_scale", [(1e20, 1e20), (1e24, 1e17), (1e37, 3e3), (1e21, 1e20)])
+def test_select_scores_beyond_fp32(q_scale, k_scale, sk):
+    """Products of norms from 1e36 to 1e42: fp32 sums overflow on the way to scores that fp64 holds."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    q, k = _randn((1, 900, 2, 64), 1, torch.float32), _randn((1, sk, 2, 64), 2, torch.float32)
+    # (block sizes over three decades: in a row, some sums overflow and others do not)
+    size = 10.0 ** -(3 * torch.rand(1, -(-sk // 64), 1, 1, device="cuda", generator=torch.Generator("cuda").manual_seed(3)))
+    k = k * size.repeat_interleave(64, 1)[:, :sk]
+    q = (q.clamp(-3, 3) * q_scale).to(torch.bfloat16)
+    k = (k.clamp(-3, 3) * k_scale).to(torch.bfloat16)
+    assert torch.isfinite(q).all() and torch.isfinite(k).all()
+    blocks = -(-sk // 64)
+    for top_k in (3, blocks // 4, blocks // 2):
+        got, n = select_key_blocks(q, k, top_k, block_k=64)
+        ref, ref_n = sparse_ref.select(q, k, top_k, block_k=64)
+        assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
+
+
 def test_select_close_scores():
     """Blocks that differ in the last bits of their means only, in groups of more and fewer than a warp."""
 
