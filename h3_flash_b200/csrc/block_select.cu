@@ -117,7 +117,10 @@ __global__ void __launch_bounds__(kMeanWarps * 32, 7) block_means(const MeanArgs
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int r = r0 + i * kRows;
-      u[i] = r < count ? ld_cached(base + 2 * (int64_t)r * s.row_stride) : make_uint4(0, 0, 0, 0);
+      // (Not through the read-only path: a kernel before this one in the stream may have written
+      // these rows while this grid had already started.)
+      u[i] = r < count ? *reinterpret_cast<const uint4*>(base + 2 * (int64_t)r * s.row_stride)
+                       : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) add8<FP16>(acc, u[i]);
