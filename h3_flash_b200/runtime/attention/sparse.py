@@ -304,14 +304,17 @@ SPARSE_ATTRIBUTE = "_h3b_sparse_attention"
 class SparseAttention:
     """How the packed attention of one transformer is made sparse: every block of ``block_q``
     queries attends to a ``density`` share of the blocks of ``block_k`` keys (at least
-    ``min_blocks``, and all blocks that hold any of the last ``keep_last_rows`` rows: text and
-    audio rows behind the video)."""
+    ``min_blocks``), and among them always to all blocks that hold any of the first
+    ``keep_first_rows`` or the last ``keep_last_rows`` rows. The rows are those of the whole sequence:
+    ``H3Transformer`` has text first, then video, then audio, so its text is kept by
+    ``keep_first_rows`` and its audio by ``keep_last_rows``."""
 
     density: float
     block_q: int = 128
     block_k: int = 128
     keep_last_rows: int = 0
     min_blocks: int = 1
+    keep_first_rows: int = 0
     calls: int = 0
 
     def __post_init__(self) -> None:
@@ -320,8 +323,9 @@ class SparseAttention:
         if self.block_q not in BLOCK_Q or self.block_k not in BLOCK_K:
             raise ValueError(f"sparse attention: block_q must be one of {BLOCK_Q} and block_k one of {BLOCK_K}, got "
                              f"{self.block_q} and {self.block_k}")
-        if self.keep_last_rows < 0 or self.min_blocks < 1:
-            raise ValueError("sparse attention: keep_last_rows must not be negative, min_blocks at least 1")
+        if self.keep_first_rows < 0 or self.keep_last_rows < 0 or self.min_blocks < 1:
+            raise ValueError("sparse attention: keep_first_rows and keep_last_rows must not be negative, min_blocks at "
+                             "least 1")
 
     def list_length(self, rows: int) -> int:
         """Key blocks per list for a sequence of ``rows``."""
@@ -330,19 +334,28 @@ class SparseAttention:
         share = math.ceil(self.density * blocks - 1e-9)  # 0.1 * 30 is a little more than 3
         return min(blocks, max(share, self.min_blocks, self._kept(rows)))
 
+    def _kept_ends(self, rows: int) -> tuple[int, int]:
+        """Kept key blocks at the start and at the end of a sequence of ``rows``."""
+
+        last = min(self.keep_last_rows, rows)
+        return (-(-min(self.keep_first_rows, rows) // self.block_k),
+                -(-rows // self.block_k) - (rows - last) // self.block_k if last else 0)
+
     def _kept(self, rows: int) -> int:
-        kept_rows = min(self.keep_last_rows, rows)
-        return -(-rows // self.block_k) - (rows - kept_rows) // self.block_k if kept_rows else 0
+        return min(sum(self._kept_ends(rows)), -(-rows // self.block_k))
 
     def _keep_mask(self, rows: int, device: torch.device) -> torch.Tensor | None:
         """The kept blocks, made anew on the current stream by every call: a mask that outlived its call
         could be replaced while another stream, or a captured graph, still reads it."""
 
-        if not self.keep_last_rows or not rows:
+        first, last = self._kept_ends(rows)
+        if not first and not last:
             return None
-        blocks = -(-rows // self.block_k)
-        mask = torch.zeros(blocks, dtype=torch.bool, device=device)
-        mask[blocks - self._kept(rows):] = True
+        mask = torch.zeros(-(-rows // self.block_k), dtype=torch.bool, device=device)
+        if first:
+            mask[:first] = True
+        if last:
+            mask[-last:] = True
         return mask
 
     def attend(self, packed: torch.Tensor, head_dim: int) -> torch.Tensor:
@@ -355,7 +368,7 @@ class SparseAttention:
 
 
 def install_sparse_attention(transformer: Any, *, density: float = 0.1, block_q: int = 128, block_k: int = 128,
-                             keep_last_rows: int = 0, min_blocks: int = 1) -> dict[str, Any]:
+                             keep_last_rows: int = 0, min_blocks: int = 1, keep_first_rows: int = 0) -> dict[str, Any]:
     """Make the packed attention of every block sparse (see ``SparseAttention``).
 
     Call it after ``install_transformer_fusions`` (with ``qknorm_rope``) or
@@ -364,7 +377,7 @@ def install_sparse_attention(transformer: Any, *, density: float = 0.1, block_q:
     sequence, so the ranks need not agree on anything. Returns the installation's metadata; its
     ``"runtime"`` counts calls. ``remove_sparse_attention`` goes back to dense attention."""
 
-    runtime = SparseAttention(density, block_q, block_k, keep_last_rows, min_blocks)
+    runtime = SparseAttention(density, block_q, block_k, keep_last_rows, min_blocks, keep_first_rows)
     modules = [block.attn for block in transformer.transformer_blocks]
     for attention in modules:
         if not getattr(attention.__dict__.get("forward"), "h3b_packed", False):
@@ -375,7 +388,8 @@ def install_sparse_attention(transformer: Any, *, density: float = 0.1, block_q:
     for attention in modules:
         setattr(attention, SPARSE_ATTRIBUTE, runtime)
     return {"backend": "h3b_block_sparse", "semantics": "sparse", "modules": len(modules), "density": density,
-            "block_q": block_q, "block_k": block_k, "keep_last_rows": keep_last_rows, "runtime": runtime}
+            "block_q": block_q, "block_k": block_k, "keep_first_rows": keep_first_rows, "keep_last_rows": keep_last_rows,
+            "runtime": runtime}
 
 
 def remove_sparse_attention(transformer: Any) -> None:

@@ -211,6 +211,92 @@ def test_two_lengths_on_two_streams():
     assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
 
 
+def _record(runtime):
+    """What the runtime's attention calls get and give, in order."""
+
+    calls, attend = [], runtime.attend
+    runtime.attend = lambda packed, head_dim: calls.append((packed.clone(), attend(packed, head_dim))) or calls[-1][1]
+    return calls
+
+
+def _check_call(packed, out, runtime, keep):
+    """Every row of one packed attention call, against the lists that the oracle chooses from the same rows.
+
+    The bound: weights rounded once (half a step each), the output once, and what fp32 leaves of scores
+    and exponentials (128 products that truncate, 2^-18)."""
+
+    q, k, v = (packed[None, ..., i * 128:(i + 1) * 128] for i in range(3))
+    kw = dict(block_q=runtime.block_q, block_k=runtime.block_k)
+    indices, counts = sparse_ref.select(q, k, runtime.list_length(packed.shape[0]), keep=keep, **kw)
+    ref, _, weight_abs, score_abs = sparse_ref.attend(q, k, v, indices, counts, **kw)
+    u = torch.finfo(packed.dtype).eps / 2
+    slack = 128 * 2.0**-23 * score_abs + 2.0**-18
+    bound = (u + 2 * slack.transpose(1, 2)[..., None]) * weight_abs + u * ref.abs() * (1 + 2.0**-6) + 2.0**-24
+    assert ((out[None].double().cpu() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("block_q,block_k,first,last", [(128, 128, 0, 0), (256, 64, 0, 70), (128, 64, 130, 0), (256, 128, 1, 300)])
+def test_every_row_of_the_module_follows_its_list(block_q, block_k, first, last):
+    from h3_flash_b200.runtime.attention import install_sparse_attention
+    from h3_flash_b200.runtime.kernels import install_transformer_fusions
+
+    rows = 1300
+    stack, hidden, idx, rope = _setup(rows, 256, 2)
+    attention = stack.transformer_blocks[0].attn
+    install_transformer_fusions(stack)
+    runtime = install_sparse_attention(stack, density=0.3, block_q=block_q, block_k=block_k, keep_first_rows=first,
+                                       keep_last_rows=last)["runtime"]
+    calls = _record(runtime)
+    x = torch.randn(1, rows, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(torch.bfloat16)
+    with torch.no_grad():
+        got = attention.forward(x, rope)
+    starts = torch.arange(0, rows, block_k)
+    keep = (starts < first) | ((starts + block_k).clamp(max=rows) > rows - last)
+    (packed, out), = calls
+    _check_call(packed, out, runtime, keep)
+    o = attention.to_out[0]
+    _check(got[0], out.reshape(rows, -1).double() @ o.weight.double().T + o.bias.double())
+
+
+def test_transformer_keeps_its_text_and_audio():
+    """A whole transformer: text first, then video, then audio; text and audio are attended to by all rows."""
+
+    from h3_flash_b200.runtime.attention import install_sparse_attention
+    from h3_flash_b200.runtime.h3_model import H3Transformer, make_inputs
+    from h3_flash_b200.runtime.kernels import install_transformer_fusions
+
+    torch.manual_seed(0)
+    model = H3Transformer(256, 2, 128, 512, 2, text_dim=64, video_channels=32, audio_channels=16, freq_dim=64, freqs_per_axis=16)
+    with torch.no_grad():
+        for name, p in model.named_parameters():
+            if "norm" in name and name.endswith("weight") and p.dim() == 1:
+                p.copy_(1.0 + 0.02 * torch.randn_like(p))
+            else:
+                p.normal_(0.0, 0.05)
+    model = model.to("cuda", torch.bfloat16).eval()
+    n_text, n_video, n_audio = 77, 6 * 12 * 16, 30
+    inputs = make_inputs(model, n_text=n_text, n_video=n_video, n_audio=n_audio, text_dim=64, grid=(6, 12, 16), device="cuda",
+                         dtype=torch.bfloat16)
+    install_transformer_fusions(model)
+    with torch.no_grad():
+        dense = model(**inputs)
+        runtime = install_sparse_attention(model, density=0.25, block_k=64, keep_first_rows=n_text,
+                                           keep_last_rows=n_audio)["runtime"]
+        calls = _record(runtime)
+        sparse = model(**inputs)
+    rows = n_text + n_video + n_audio
+    starts = torch.arange(0, rows, 64)
+    keep = (starts < n_text) | ((starts + 64).clamp(max=rows) > n_text + n_video)
+    assert keep.tolist() == [True] * 2 + [False] * (len(keep) - 3) + [True] and runtime.list_length(rows) == 5
+    assert len(calls) == 2
+    for packed, out in calls:
+        _check_call(packed, out, runtime, keep)
+    assert torch.isfinite(sparse.sample).all() and not torch.equal(sparse.sample, dense.sample)
+    with torch.no_grad():
+        runtime.density = 1.0
+        _check(model(**inputs).sample, dense.sample)
+
+
 def test_full_density_is_dense_attention():
     from h3_flash_b200.runtime.attention import install_sparse_attention
     from h3_flash_b200.runtime.kernels import install_transformer_fusions

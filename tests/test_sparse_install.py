@@ -43,6 +43,29 @@ def test_no_mask_outlives_its_call():
     assert s._keep_mask(0, torch.device("cpu")) is None
 
 
+def test_rows_at_both_ends_are_kept():
+    """Text stands first in the sequence, audio last."""
+
+    s = SparseAttention(0.1, block_k=64, keep_first_rows=65, keep_last_rows=1)
+    cpu = torch.device("cpu")
+    assert s._keep_mask(641, cpu).tolist() == [True] * 2 + [False] * 8 + [True]
+    assert s.list_length(641) == 3 and s.list_length(6400) == 10
+    assert s._keep_mask(128, cpu).tolist() == [True] * 2 and s.list_length(128) == 2
+    assert s._keep_mask(3, cpu).tolist() == [True] and s.list_length(3) == 1
+    assert SparseAttention(0.1, keep_first_rows=1)._keep_mask(256, cpu).tolist() == [True, False]
+    assert SparseAttention(0.1, keep_first_rows=10**6, keep_last_rows=10**6).list_length(51200) == 400
+    assert SparseAttention(0.1)._keep_mask(256, cpu) is None
+    with pytest.raises(ValueError, match="keep_first_rows"):
+        SparseAttention(0.1, keep_first_rows=-1)
+    stack = _stack()
+    from h3_flash_b200.runtime.kernels.transformer import _patch_attention
+
+    _patch_attention(stack, {})
+    meta = install_sparse_attention(stack, keep_first_rows=77, keep_last_rows=5)
+    assert meta["keep_first_rows"] == meta["runtime"].keep_first_rows == 77
+    assert meta["keep_last_rows"] == meta["runtime"].keep_last_rows == 5
+
+
 @pytest.mark.parametrize("bad", [dict(density=0.0), dict(density=1.5), dict(density=0.1, block_q=64), dict(density=0.1, block_k=32),
                                  dict(density=0.1, keep_last_rows=-1), dict(density=0.1, min_blocks=0)])
 def test_settings_are_checked(bad):
