@@ -243,6 +243,9 @@ def _sandwich_rest(block: Any, residual: torch.Tensor, attention_output: torch.T
 
 
 def _patch_blocks(transformer: Any, modulate: bool, swiglu: bool, runtime: dict[str, Any]) -> None:
+    for block in transformer.transformer_blocks:
+        if (getattr(block, "norm1_post", None) is None) != (getattr(block, "norm2_post", None) is None):
+            raise RuntimeError("transformer fusions: a block needs norm1_post and norm2_post together, or neither")
     gemm_epilogue = bool(runtime.get("gemm_epilogue", False))
     for block_index, block in enumerate(transformer.transformer_blocks):
 

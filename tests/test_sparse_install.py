@@ -147,3 +147,23 @@ def test_sandwich_block_eager_math():
     with pytest.raises(ValueError, match="needs sandwich_norm"):
         H3TransformerBlock(dim=64, heads=1, head_dim=64, ffn_inner=128, residual_scale=0.5)
     assert block.norm1_post is not None and H3TransformerBlock(dim=64, heads=1, head_dim=64, ffn_inner=128).norm1_post is None
+
+
+@pytest.mark.parametrize("missing", ["norm1_post", "norm2_post"])
+@pytest.mark.parametrize("gone", [False, True])
+def test_a_block_with_one_post_norm_is_refused_when_installed(missing, gone):
+    """Not in the middle of a forward pass (norm2_post missing), and not run without its norm (norm1_post missing)."""
+
+    from h3_flash_b200.runtime.kernels.transformer import _patch_blocks
+
+    stack = H3BlockStack([H3TransformerBlock(dim=64, heads=1, head_dim=64, ffn_inner=128, sandwich_norm=True) for _ in range(2)])
+    last = stack.transformer_blocks[1]
+    if gone:
+        delattr(last, missing)
+    else:
+        setattr(last, missing, None)
+    with pytest.raises(RuntimeError, match="norm1_post and norm2_post together"):
+        _patch_blocks(stack, True, True, {"gate": {}})
+    assert all("forward" not in vars(block) for block in stack.transformer_blocks)
+    _patch_blocks(H3BlockStack([stack.transformer_blocks[0]]), True, True, {"gate": {}})
+    assert "forward" in vars(stack.transformer_blocks[0])
