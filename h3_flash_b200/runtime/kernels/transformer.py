@@ -237,9 +237,14 @@ def _sandwich_rest(block: Any, residual: torch.Tensor, attention_output: torch.T
     branch = feed_forward(block.ff, normed, swiglu, gate, gemm_epilogue)
     if modulate:
         with TIMER.section("elementwise"):
-            return fused_sandwich_residual(hidden, branch, block.norm2_post.weight, gate_mlp, indices,
-                                           block.norm2_post.eps, residual_scale=scale_by)
-    return scale_by * hidden + gate_mlp.index_select(0, indices) * block.norm2_post(branch)
+            output = fused_sandwich_residual(hidden, branch, block.norm2_post.weight, gate_mlp, indices,
+                                             block.norm2_post.eps, residual_scale=scale_by)
+    if not modulate or (gate is not None and "sandwich_closing" not in gate):
+        eager_output = scale_by * hidden + gate_mlp.index_select(0, indices) * block.norm2_post(branch)
+        if not modulate:
+            return eager_output
+        gate["sandwich_closing"] = _error_metrics(output, eager_output)
+    return output
 
 
 def _patch_blocks(transformer: Any, modulate: bool, swiglu: bool, runtime: dict[str, Any]) -> None:

@@ -138,6 +138,29 @@ def test_sandwich_block(rows, dim, heads, activation, scale):
         _check(plain(hidden, None, idx, rope), ref)
 
 
+def test_the_first_call_compares_every_sandwich_step():
+    from h3_flash_b200.runtime.kernels import install_transformer_fusions, transformer
+
+    stack, hidden, idx, rope = _setup(300, 256, 2, sandwich_norm=True, residual_scale=0.5)
+    runtime = install_transformer_fusions(stack)
+    with torch.no_grad():
+        first = stack(hidden, None, idx, rope)
+        assert {"sandwich_output", "sandwich_chain", "sandwich_closing"} <= set(runtime["gate"])
+        assert runtime["gate"]["sandwich_closing"]["cosine"] > 0.9999
+        seen = dict(runtime["gate"])
+        assert torch.equal(stack(hidden, None, idx, rope), first) and runtime["gate"] == seen
+        # a closing step that is off shows
+        other, _, _, _ = _setup(300, 256, 2, sandwich_norm=True, residual_scale=0.5)
+        runtime = install_transformer_fusions(other)
+        right = transformer.fused_sandwich_residual
+        transformer.fused_sandwich_residual = lambda *a, residual_scale: right(*a, residual_scale=1.0)
+        try:
+            other(hidden, None, idx, rope)
+        finally:
+            transformer.fused_sandwich_residual = right
+    assert runtime["gate"]["sandwich_closing"]["relative_l2"] > 0.1
+
+
 def test_sparse_sandwich_stack_runs_captured_like_eagerly():
     """Two blocks with everything installed: selection, sparse attention, sandwich norms, GEMMs;
     replayed from a graph on new rows it gives the bits of the eager run."""
