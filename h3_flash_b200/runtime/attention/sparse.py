@@ -129,7 +129,8 @@ def select_key_blocks(q: torch.Tensor, k: torch.Tensor, top_k: int, *, block_q: 
     list holds before any other (audio or text rows, say). Returns ``indices`` int32
     [B, H, ceil(Sq / block_q), top_k], ascending and -1 behind the last, and ``counts`` int32
     [B, H, ceil(Sq / block_q)]. Scores are compared in 64 bits, ties go to the lowest index:
-    equal inputs give equal lists on any device and in any batch."""
+    equal inputs give equal lists in any batch (bf16: as long as the nonzero values of a column
+    of a block lie within a factor of 2^37; beyond that its 64-bit sum may round differently)."""
 
     op = "select_key_blocks"
     code = check_inputs(op, _TYPES, (q, k))

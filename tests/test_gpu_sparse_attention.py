@@ -417,6 +417,32 @@ def test_select_scores_beyond_fp32(q_scale, k_scale, sk):
         assert torch.equal(got.cpu(), ref) and torch.equal(n.cpu(), ref_n)
 
 
+@pytest.mark.parametrize("dtype,low,high", [(torch.float16, -24, 15), (torch.bfloat16, -20, 17)])
+def test_lists_do_not_depend_on_the_batch(dtype, low, high):
+    """Columns that mix magnitudes as far apart as fp64 sums hold exactly, and cancel: an entry alone (means
+    of few blocks, four warps each) chooses like the same entry in a large batch (a warp each)."""
+
+    from h3_flash_b200.runtime.attention.sparse import select_key_blocks
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    b, s, h, d = 12, 1600, 8, 64
+
+    def mixed(seq):
+        sign = torch.randint(0, 2, (b, seq, h, d), generator=g, device="cuda") * 2 - 1
+        x = sign * 2.0 ** torch.randint(low, high + 1, (b, seq, h, d), generator=g, device="cuda").float()
+        x[:, 1::2] = torch.where(torch.rand(b, seq // 2, h, d, generator=g, device="cuda") < 0.9, -x[:, 0::2], x[:, 1::2])
+        return x.to(dtype)
+
+    q, k = mixed(s), mixed(s)
+    assert b * h * (-(-s // 128) + -(-s // 64)) > 148 * 16 > h * (-(-s // 128) + -(-s // 64))
+    got, _ = select_key_blocks(q, k, 5, block_k=64)
+    for i in range(b):
+        alone, _ = select_key_blocks(q[i : i + 1], k[i : i + 1], 5, block_k=64)
+        assert torch.equal(alone[0], got[i])
+    ref, _ = sparse_ref.select(q[:1], k[:1], 5, block_k=64)
+    assert torch.equal(got[:1].cpu(), ref)
+
+
 def test_select_close_scores():
     """Blocks that differ in the last bits of their means only, in groups of more and fewer than a warp."""
 
