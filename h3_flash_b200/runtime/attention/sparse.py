@@ -364,7 +364,8 @@ class SparseAttention:
 
         rows = packed.shape[0]
         self.calls += 1
-        return packed_sparse_attention(packed, self.list_length(rows), head_dim, block_q=self.block_q,
+        # (A sequence without rows has lists of no blocks, and the op answers it as the dense one does.)
+        return packed_sparse_attention(packed, max(self.list_length(rows), 1), head_dim, block_q=self.block_q,
                                        block_k=self.block_k, keep=self._keep_mask(rows, packed.device))
 
 

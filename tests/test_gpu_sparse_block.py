@@ -217,6 +217,21 @@ def test_captured_kept_blocks_outlive_other_lengths():
     assert torch.equal(out, runtime.attend(packed, 128)) and full
 
 
+@pytest.mark.parametrize("rows", [0, 1, 127, 129])
+def test_shortest_sequences(rows):
+    """None to a few rows: what the dense op answers (all blocks are kept, or there is one)."""
+
+    from h3_flash_b200.runtime.attention.dense import packed_attention
+    from h3_flash_b200.runtime.attention.sparse import SparseAttention
+
+    packed = _packed(rows, 5)
+    out = SparseAttention(0.1, keep_first_rows=100, keep_last_rows=3).attend(packed, 128)
+    dense = packed_attention(packed)
+    assert out.shape == dense.shape == (rows, 2, 128) and torch.isfinite(out).all()
+    if rows:
+        _check(out, dense)
+
+
 def test_two_lengths_on_two_streams():
     from h3_flash_b200.runtime.attention.sparse import SparseAttention
 
