@@ -899,6 +899,10 @@ __device__ __forceinline__ int choose_fast(const ChooseArgs& a, const Row& r, ui
 // once hide it (6108 rows of 2036 columns: two CTAs 63 us, three 48 us, four 43 us, five 43 us).
 // Eight warps a CTA are slower, 33 against 30 us for 9600 rows of 800: a CTA lasts as long as its
 // slowest row.
+// Rows of 32, 64 and 128 columns a lane spill 60, 84 and 124 bytes a thread under these bounds. Rows of
+// more than 4096 columns (KEYS = 0) are slow: every pass of choose_any reads them from global
+// memory. 24 heads of 354,206 rows: 0.90 ms for lists of 138 of 2768 blocks (128 columns a lane), 5.0
+// ms for 276 of 5535 blocks (choose_any), beside an HBM pass of 0.7 ms.
 template <int KEYS>
 __global__ void __launch_bounds__(kChooseWarps * 32, KEYS <= 16 ? 8 : KEYS <= 32 ? 6 : KEYS <= 64 ? 4 : 3)
     block_choose(const __grid_constant__ ChooseArgs a) {

@@ -123,7 +123,9 @@ __device__ __forceinline__ float cta_sum(float v, float* red) {
   return s;
 }
 
-// Any width and alignment: one CTA per row, scalar accesses, hidden recomputed from L1/L2.
+// Any width and alignment: one CTA per row, scalar accesses, hidden recomputed from L1/L2. Bound by
+// its 2- and 4-byte accesses: 51,200 rows of 3071 take 757 us in bf16 and 767 us in fp32 (455 and 500 us
+// without the second norm), where their bytes take 192 and 384 us.
 constexpr int kScalarWarps = 8;
 template <class T>
 __global__ void __launch_bounds__(kScalarWarps * 32) sandwich_scalar(SandwichArgs a) {

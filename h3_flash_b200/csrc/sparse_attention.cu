@@ -36,7 +36,7 @@
 // MMAs wait for one another. The price is that an N = 64 score MMA reads its Q operand from
 // shared memory for half as many columns. Measured on 592 pairs of tiles, 64 blocks a list,
 // under the power cap: 590 us with one list per pair and 640 us with a list per tile, against
-// 678 and 694 us with units of 128 keys (before the steps noted below, now 556 and 580 us).
+// 678 and 694 us with units of 128 keys (before the steps noted below, now 538 and 581 us).
 //
 // TMEM (512 columns): S of tile t, buffer b at 128 t + 64 b; O of tile t at 256 + 128 t.
 //
@@ -904,7 +904,9 @@ struct Plan {
 // Queries of one tile are split in two even where SMs are short, half a list for each of the
 // two tiles of an item. Both only as far as an estimate says that it saves more than the join
 // costs: a step is one unit of 64 keys of both tiles (or of a lone one), the join another launch
-// and the parts written and read. Measured split into as many parts as fit, and whole (us):
+// and the parts written and read. (Whole lists of 16 and 128 units on 2048 rows, 6 heads, at full
+// clock: 0.74 us a step with D = 64, 0.76 to 0.80 with D = 128; long calls that draw the power cap take
+// more, but they fill the SMs without a split.) Measured split into as many parts as fit, and whole (us):
 // 2048 rows, 6 heads, D = 64, lists of 256 keys 14.9 and 8.2, of 1536 keys 21.5 and 23.1, of
 // 8192 keys 50 and 100; one row, 6 heads, 256 keys 8.7 and 6.7, 768 keys 9.2 and 11.3.
 Plan make_plan(int64_t batch, int64_t seq_q, int64_t heads, int64_t head_dim, int64_t block_k,
