@@ -164,12 +164,12 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     """softmax(q k^T * scale) v over the keys of every query block's listed key blocks.
 
     q [B, Sq, H, D], k and v [B, Sk, Hk, D] (strided views with a contiguous, 16-byte aligned
-    head_dim of 64 or 128; bf16 or fp16). ``indices`` int32 [B, H, ceil(Sq / block_q), n]: the
+    head_dim of 64 or 128, no expanded dimensions; bf16 or fp16). ``indices`` int32 [B, H, ceil(Sq / block_q), n]: the
     first ``counts`` entries of a list count (all of them without ``counts``), in any order. An
     entry outside the key blocks adds nothing, an entry that is there twice counts twice. Query
     rows that have no key, and rows behind ``q_lens``, get zeros (lse -inf). Returns
-    [B, Sq, H, D] (``out`` if given, which must not overlap an input), and with ``return_lse`` the fp32 [B, H, Sq] logarithms of
-    the softmax sums."""
+    [B, Sq, H, D] (``out`` if given, which must not overlap an input), and with ``return_lse`` the
+    fp32 [B, H, Sq] logarithms of the softmax sums."""
 
     op = "block_sparse_attention"
     code = check_inputs(op, _TYPES, (q, k, v) if out is None else (q, k, v, out))

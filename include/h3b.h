@@ -298,6 +298,8 @@ int h3b_attention_noalloc(void* out, const void* q, const void* k, const void* v
  * 128 (else H3B_ERR_UNSUPPORTED). q_lens / k_lens (int32 [batch], or NULL: all
  * rows) give the rows of each batch entry that exist; what lies behind them may
  * be anything, NaN included. nq = ceil(seq_q / block_q), nk = ceil(seq_k / block_k).
+ * Strides of dimensions larger than one are multiples of 8 elements, and for the attention
+ * positive (rows shared by several batch entries or heads are not expressed by a stride of 0).
  * No reference counterpart: the reference's attention is dense.
  * ------------------------------------------------------------------------- */
 
