@@ -390,17 +390,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait_all(bar_empty(slot), phase_of(pos) ^ 1)) return false;
         const uint32_t dst = sbase + L::kSmemRing + slot * L::kSlotBytes;
         const uint32_t full = bar_full(slot);
-        // Visible to the softmax through this slot's barrier, the MMA warp and its commit.
-        auto hand_keys = [&](Walk& reader, int tile) {
-          if (lane == 0) {
-            if (first) key_ring[tile * kKeyRing + reader.keys_at % kKeyRing] = (uint8_t)keys0;
-            if (two) key_ring[tile * kKeyRing + (reader.keys_at + (first ? 1 : 0)) % kKeyRing] = (uint8_t)keys1;
-          }
-          reader.keys_at += (first ? 1u : 0u) + (two ? 1u : 0u);
+        // Visible to the softmax through this slot's barrier, the MMA warp and its commit: written by the
+        // lane that arms the barrier.
+        auto hand_keys = [&](const Walk& reader, int tile) {
+          if (first) key_ring[tile * kKeyRing + reader.keys_at % kKeyRing] = (uint8_t)keys0;
+          if (two) key_ring[tile * kKeyRing + (reader.keys_at + (first ? 1 : 0)) % kKeyRing] = (uint8_t)keys1;
         };
-        hand_keys(w, t);
-        if (SHARED && walk[1].units > 0) hand_keys(walk[1], 1);
+        const bool both = SHARED && walk[1].units > 0;
         if (elect_one()) {
+          hand_keys(w, t);
+          if (both) hand_keys(walk[1], 1);
           slot_tag[slot] = pos;
           const uint32_t bar = cut ? bar_fix : full;
           mbar_expect_tx(bar, two ? L::kSlotBytes : L::kPartBytes);
@@ -416,6 +415,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();
+        const uint32_t handed = (first ? 1u : 0u) + (two ? 1u : 0u);
+        w.keys_at += handed;
+        if (both) walk[1].keys_at += handed;
         if (cut) {
           // V rows behind the last key: zeros, then hand the slot over.
           if (!wait_all(bar_fix, fix_phase)) return false;
